@@ -217,6 +217,165 @@ int rmsnorm_local_backward(void* dx, void* dw, const void* dy, const void* x, co
                            int64_t rows, int64_t hidden, int dtype, float eps, void* workspace,
                            size_t workspace_bytes, void* stream);
 
+/* ---- query / key heads, paged cache, single-token attention -----------------
+ * The operators between the two norms of a transformer block, on the heads of
+ * one rank (they exchange nothing). No counterpart in the reference, which has
+ * the norms alone.
+ *
+ * Every function is stream-ordered on `stream`, capturable in a CUDA graph,
+ * runs on device `device` of its arguments (whichever device is current), and
+ * keeps nothing between calls. Strides are in elements; the last dimension of
+ * every tensor has stride 1. */
+
+/* Element type of the cache beside enum rmsnorm_tp_dtype: e4m3 codes, with one
+ * fp32 scale for each (token, head). */
+#define RMSNORM_KV_E4M3 3
+
+#define RMSNORM_HEAD_DIM_MAX 512   /* rotation and norm; the attention takes up to 256 */
+
+/* A paged cache: k and v are [num_pages, kv_heads, page_size, head_dim]
+ * contiguous, of `dtype` (enum rmsnorm_tp_dtype) or RMSNORM_KV_E4M3, then with
+ * k_scale and v_scale [num_pages, kv_heads, page_size] fp32. A row x is held as
+ *   scale = max(amax|x|, 2^-100) / 448, code = e4m3(x * (448 / max(amax|x|, 2^-100)))
+ * and stands for code * scale. head_dim a multiple of 16, at most 256; k and v
+ * 16-byte aligned. */
+typedef struct rmsnorm_kv_cache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int64_t num_pages;
+  int32_t page_size;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t dtype;
+} rmsnorm_kv_cache;
+
+/* Arguments of rmsnorm_qk_rope_forward and rmsnorm_qk_rope_write.
+ *   y = R(position) (x * rsqrt(mean over head_dim of x^2 + eps) * weight)
+ * for every query and key head of every token. R turns the pairs (i, i +
+ * rotary_dim / 2) (interleaved: (2i, 2i + 1)), i < rotary_dim / 2, by the angle
+ * whose cosine and sine are rope[position][i] and rope[position][rotary_dim / 2
+ * + i]; the elements from rotary_dim on are not turned. Without weights (both
+ * NULL) there is no norm, R alone. fp32 throughout, rounded once.
+ * A position outside [0, max_positions) makes the turned elements NaN. */
+typedef struct rmsnorm_qk_rope_args {
+  const void* q;              /* [tokens, q_heads, head_dim] */
+  const void* k;              /* [tokens, kv_heads, head_dim] */
+  const void* v;              /* write: [tokens, kv_heads, head_dim]; else NULL */
+  void* q_out;                /* may be q itself (same strides); no other overlap */
+  void* k_out;                /* forward: may be k itself; write: NULL */
+  const void* q_weight;       /* [head_dim], or NULL with k_weight */
+  const void* k_weight;
+  const float* rope;          /* [max_positions, rotary_dim] fp32: cosines, then sines */
+  const int64_t* positions;   /* [tokens] */
+  int64_t q_strides[2];       /* token, head */
+  int64_t k_strides[2];
+  int64_t v_strides[2];
+  int64_t q_out_strides[2];
+  int64_t k_out_strides[2];
+  int64_t tokens;
+  int64_t max_positions;
+  /* rmsnorm_qk_rope_write only: the cache and the
+   * slot page * page_size + offset of each token, distinct within the call; a
+   * slot outside the cache (-1, say) leaves the cache as it is */
+  const rmsnorm_kv_cache* cache;
+  const int64_t* slots;       /* [tokens] */
+  int32_t q_heads;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t rotary_dim;         /* even, in [2, head_dim] */
+  int32_t dtype;              /* of q, k, v, the outputs and the weights */
+  int32_t interleaved;
+  float eps;
+  int32_t device;
+} rmsnorm_qk_rope_args;
+
+int rmsnorm_qk_rope_forward(const rmsnorm_qk_rope_args* args, void* stream);
+
+/* The same pass; the key heads go into the cache instead of k_out, and v beside
+ * them. The cache is of the call's dtype, or e4m3 (quantised from the fp32
+ * values, so K is rounded once). */
+int rmsnorm_qk_rope_write(const rmsnorm_qk_rope_args* args, void* stream);
+
+/* Gradients of rmsnorm_qk_rope_forward, with g = R^T dy and inv the forward's
+ * factor: dx = inv g w - x inv^3 mean(g w x), dw = sum over tokens and heads of
+ * g x inv (without weights dx = g, and q, k may be NULL). dq and dk are
+ * contiguous [tokens, heads, head_dim] and overlap no input; dweight holds the
+ * query weight's gradient, then the key weight's ([2 * head_dim]). workspace:
+ * rmsnorm_qk_rope_backward_workspace_bytes(head_dim) bytes of device memory
+ * (fp32 partials of dweight, summed in a fixed order: deterministic). */
+typedef struct rmsnorm_qk_rope_backward_args {
+  const void* dq_out;         /* [tokens, q_heads, head_dim] */
+  const void* dk_out;         /* [tokens, kv_heads, head_dim] */
+  const void* q;
+  const void* k;
+  void* dq;
+  void* dk;
+  void* dweight;              /* NULL without weights */
+  const void* q_weight;
+  const void* k_weight;
+  const float* rope;
+  const int64_t* positions;
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t dq_out_strides[2];
+  int64_t dk_out_strides[2];
+  int64_t q_strides[2];
+  int64_t k_strides[2];
+  int64_t tokens;
+  int64_t max_positions;
+  int32_t q_heads;
+  int32_t kv_heads;
+  int32_t head_dim;
+  int32_t rotary_dim;
+  int32_t dtype;
+  int32_t interleaved;
+  float eps;
+  int32_t device;
+} rmsnorm_qk_rope_backward_args;
+
+size_t rmsnorm_qk_rope_backward_workspace_bytes(int32_t head_dim);
+int rmsnorm_qk_rope_backward(const rmsnorm_qk_rope_backward_args* args, void* stream);
+
+/* k_out and v_out [count, kv_heads, head_dim] contiguous of `dtype`: the cache's
+ * rows at `slots` (code * scale for an e4m3 cache, rounded once); a slot outside
+ * the cache gives zeros. */
+int rmsnorm_kv_read(const rmsnorm_kv_cache* cache, void* k_out, void* v_out, const int64_t* slots,
+                    int64_t count, int dtype, int device, void* stream);
+
+/* Attention of one new token of each sequence over its cached tokens:
+ *   o[b, h] = sum over j < seq_lens[b] of softmax_j(scale q[b, h] . k[j, h']) v[j, h'],
+ * h' = h / (q_heads / kv_heads); token j of sequence b lies in page
+ * page_table[b][j / page_size]. A length is cut to max_pages * page_size; tokens
+ * in a page outside [0, num_pages) are left out; a sequence with no tokens gives
+ * zeros and lse = -inf. lse (optional): the natural logarithm of the sum of the
+ * exponentials. Scores, softmax and sums in fp32. The work is divided over the
+ * cached length as the lengths on the device say. q and the cache of one dtype,
+ * or an e4m3 cache. workspace: rmsnorm_paged_attention_workspace_bytes(args)
+ * bytes of device memory, of its own for every call in flight. */
+typedef struct rmsnorm_paged_attention_args {
+  const rmsnorm_kv_cache* cache;
+  const void* q;              /* [batch, q_heads, head_dim] */
+  void* out;                  /* [batch, q_heads, head_dim] contiguous */
+  float* lse;                 /* [batch, q_heads], or NULL */
+  const int32_t* page_table;  /* [batch, max_pages], rows page_table_stride apart */
+  const int32_t* seq_lens;    /* [batch] */
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t q_strides[2];
+  int64_t page_table_stride;
+  int64_t batch;
+  int64_t max_pages;
+  int32_t q_heads;
+  int32_t dtype;
+  float scale;
+  int32_t device;
+} rmsnorm_paged_attention_args;
+
+size_t rmsnorm_paged_attention_workspace_bytes(const rmsnorm_paged_attention_args* args);
+int rmsnorm_paged_attention(const rmsnorm_paged_attention_args* args, void* stream);
+
 /* ---- failure detection and recovery (no reference counterpart) ---------- */
 
 /* Limit on each wait for a peer's partial sum, in nanoseconds (default
@@ -372,7 +531,9 @@ const char* rmsnorm_tp_last_error(void);
  * added rmsnorm_tp_forward_group_static_status, the batch kernel family
  * (rmsnorm_tp_set_kernel_family(3)), the push encodings and the fused
  * row-parallel linear entry points; 1.03 widened the profile counters of
- * rmsnorm_tp_set_profile from 5 to 20. */
+ * rmsnorm_tp_set_profile from 5 to 20. The rmsnorm_qk_*, rmsnorm_kv_* and
+ * rmsnorm_paged_attention entry points came after it; they change nothing that
+ * 1.03 has, and a caller finds them by their symbols. */
 int rmsnorm_tp_abi_version(void);
 
 #ifdef __cplusplus

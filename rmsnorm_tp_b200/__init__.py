@@ -32,6 +32,15 @@ from .api import (
     get_dependent_launch,
     tag_of,
 )
+from .heads import (
+    PagedKVCache,
+    paged_attention,
+    qk_norm_rope,
+    qk_norm_rope_backward,
+    qk_norm_rope_with_grad,
+    qk_norm_rope_write,
+    rope_table,
+)
 
 __all__ = [
     "FusedTPRMSNorm",
@@ -43,6 +52,13 @@ __all__ = [
     "exchange_handles",
     "local_rmsnorm",
     "local_rmsnorm_backward",
+    "qk_norm_rope",
+    "qk_norm_rope_backward",
+    "qk_norm_rope_with_grad",
+    "qk_norm_rope_write",
+    "rope_table",
+    "PagedKVCache",
+    "paged_attention",
     "RMSNormTPError",
     "RMSNormTPDeviceError",
     "plan",

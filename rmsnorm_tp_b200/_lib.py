@@ -15,6 +15,8 @@ LIB_PATH = os.path.join(_HERE, "_C", "librmsnorm_tp_b200.so")
 
 # enum rmsnorm_tp_dtype
 F32, BF16, F16 = 0, 1, 2
+# cache element type beside them (RMSNORM_KV_E4M3)
+KV_E4M3 = 3
 # enum rmsnorm_tp_error
 OK, ERR_INVALID, ERR_CUDA, ERR_STATE, ERR_ROWS, ERR_DEVICE, ERR_HANDLE = range(7)
 # enum rmsnorm_tp_device_status
@@ -145,6 +147,14 @@ SIGNATURES = {
             _i64, _i32, ctypes.c_float, ctypes.POINTER(_c_void_p), _sz, _c_void_p,
         ],
     ),
+    # packed argument structures: see heads.py
+    "rmsnorm_qk_rope_forward": (_i32, [ctypes.c_char_p, _c_void_p]),
+    "rmsnorm_qk_rope_write": (_i32, [ctypes.c_char_p, _c_void_p]),
+    "rmsnorm_qk_rope_backward_workspace_bytes": (_sz, [_i32]),
+    "rmsnorm_qk_rope_backward": (_i32, [ctypes.c_char_p, _c_void_p]),
+    "rmsnorm_kv_read": (_i32, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i32, _i32, _c_void_p]),
+    "rmsnorm_paged_attention_workspace_bytes": (_sz, [ctypes.c_char_p]),
+    "rmsnorm_paged_attention": (_i32, [ctypes.c_char_p, _c_void_p]),
     "rmsnorm_tp_forward_group_static": (
         _i32,
         [

@@ -3,8 +3,10 @@
 The library is plain CUDA C++ (no torch, no pybind11): kernels.cu holds the
 forward kernels and their launcher, backward.cu the backward kernels,
 noalloc.cu the allocation-free group entry point, linear.cu the fused row-parallel linear
-(tcgen05 GEMM) -> reduce-scatter -> TP RMSNorm kernel, comm.cpp the extern "C" entry points declared in
-include/rmsnorm_tp_b200.h. The CUDA runtime is linked statically, so the
+(tcgen05 GEMM) -> reduce-scatter -> TP RMSNorm kernel, qk_rope.cu the norms of query and key
+heads with the rotation (and the write into a paged cache), kv_cache.cu the cache's read-back,
+paged_attention.cu the attention of one new token, comm.cpp the extern "C" entry points declared
+in include/rmsnorm_tp_b200.h. The CUDA runtime is linked statically, so the
 library loads (and its symbols can be listed) on a machine without a GPU.
 
     python rmsnorm_tp_b200/build.py          # build if sources are newer
@@ -29,13 +31,15 @@ LIB_PATH = os.path.join(OUT_DIR, LIB_NAME)
 
 SOURCES = [os.path.join(CSRC, "kernels.cu"), os.path.join(CSRC, "backward.cu"),
            os.path.join(CSRC, "comm.cpp"), os.path.join(CSRC, "noalloc.cu"),
-           os.path.join(CSRC, "linear.cu")]
+           os.path.join(CSRC, "linear.cu"), os.path.join(CSRC, "qk_rope.cu"),
+           os.path.join(CSRC, "kv_cache.cu"), os.path.join(CSRC, "paged_attention.cu")]
 HEADERS = [
     os.path.join(CSRC, "device_common.cuh"),
     os.path.join(CSRC, "rtp_common.h"),
     os.path.join(CSRC, "internal.h"),
     os.path.join(CSRC, "ptx.cuh"),
     os.path.join(CSRC, "sm100.cuh"),
+    os.path.join(CSRC, "heads_common.cuh"),
     os.path.join(ROOT_DIR, "include", "rmsnorm_tp_b200.h"),
 ]
 

@@ -1,0 +1,124 @@
+// Shared by the operators on query / key heads, the paged cache and the
+// single-token attention (qk_rope.cu, kv_cache.cu, paged_attention.cu):
+// argument checks, launches, and the element conversions of the cache.
+#pragma once
+
+#include <cuda_fp8.h>
+#include <stdarg.h>
+#include <stdio.h>
+
+#include "../../include/rmsnorm_tp_b200.h"
+#include "device_common.cuh"
+#include "internal.h"
+
+namespace rtp {
+
+// Records a formatted message as the calling thread's last error, returns `code`.
+inline int refuse(int code, const char* fmt, ...) {
+  char buf[384];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  return record_error(code, buf);
+}
+
+// Makes `device` current for the scope (the tensors' device need not be the
+// caller's current one), restoring the caller's device after.
+struct OnDevice {
+  int prev = -1;
+  bool switched = false;
+  cudaError_t err;
+  explicit OnDevice(int device) {
+    err = cudaGetDevice(&prev);
+    if (err == cudaSuccess && prev != device) {
+      err = cudaSetDevice(device);
+      switched = err == cudaSuccess;
+    }
+  }
+  ~OnDevice() {
+    if (switched) cudaSetDevice(prev);
+  }
+};
+
+// SM count of `device` (cached), 0 on failure.
+int sm_count(int device);
+
+// Launch with programmatic stream serialization when dependent launch is on.
+// Every kernel launched through here starts with grid_dep_wait().
+cudaError_t launch_dependent(const void* fn, dim3 grid, dim3 block, size_t smem, void** args,
+                             cudaStream_t stream);
+
+inline int launch_failed(cudaError_t e, const char* who) {
+  cudaGetLastError();   // a refused launch leaves the error behind otherwise
+  return refuse(RMSNORM_TP_ERR_CUDA, "%s: kernel launch: %s (%s)", who, cudaGetErrorString(e),
+                cudaGetErrorName(e));
+}
+
+// Checks the cache a call is given; 0 or a recorded error.
+int check_cache(const char* who, const rmsnorm_kv_cache* c);
+
+// Extent of a [tokens, heads, dim] view whose last stride is 1.
+struct View {
+  uintptr_t base;
+  int64_t n0, n1, dim, s0, s1;   // elements
+  int eb;
+  uintptr_t bytes() const {      // from the first element to behind the last
+    if (n0 == 0 || n1 == 0) return 0;
+    return (uintptr_t)(((n0 - 1) * s0 + (n1 - 1) * s1 + dim) * eb);
+  }
+};
+inline View view_of(const void* p, int64_t tokens, int64_t heads, int64_t dim, const int64_t* st,
+                    int eb) {
+  // a stride of an axis of one entry says nothing: leave it out
+  return View{reinterpret_cast<uintptr_t>(p), tokens, heads, dim, tokens > 1 ? st[0] : heads * dim,
+              heads > 1 ? st[1] : dim, eb};
+}
+
+// Whether two views may share an element. Exact for column blocks of one matrix
+// (the same token stride), else by their extents.
+inline bool views_overlap(const View& a, const View& b) {
+  const uintptr_t an = a.bytes(), bn = b.bytes();
+  if (an == 0 || bn == 0) return false;
+  if (!(a.base < b.base + bn && b.base < a.base + an)) return false;
+  if (a.n0 > 1 && b.n0 > 1 && a.s0 == b.s0 && a.s0 > 0 && a.eb == b.eb) {
+    const int64_t step = a.s0 * a.eb;
+    const int64_t ra = ((a.n1 - 1) * a.s1 + a.dim) * a.eb, rb = ((b.n1 - 1) * b.s1 + b.dim) * b.eb;
+    int64_t d = ((int64_t)(b.base - a.base)) % step;
+    if (d < 0) d += step;
+    if (ra <= step && rb <= step && d >= ra && d + rb <= step) return false;
+  }
+  return true;
+}
+inline bool views_same(const View& a, const View& b) {
+  return a.base == b.base && a.s0 == b.s0 && a.s1 == b.s1 && a.eb == b.eb;
+}
+// Whether a written view's own rows are apart.
+inline bool view_apart(const View& a) {
+  const bool heads_inside = a.s1 >= a.dim && a.s0 >= (a.n1 - 1) * a.s1 + a.dim;
+  const bool tokens_inside = a.s0 >= a.dim && a.s1 >= (a.n0 - 1) * a.s0 + a.dim;
+  return heads_inside || tokens_inside;
+}
+
+// ---- cache elements -----------------------------------------------------------
+constexpr float kE4M3Max = 448.f;
+// Smallest row maximum a scale is made of (2^-100): keeps 448 / maximum finite
+// and the scale a normal number, also for a row of zeros.
+constexpr float kE4M3Floor = 7.8886090522101181e-31f;
+
+__device__ __forceinline__ unsigned short e4m3x2_of(float lo, float hi) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ unsigned char e4m3_of(float v) {
+  return __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ float2 e4m3x2_to(unsigned short c) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(c, __NV_E4M3);
+  return __half22float2(__half2(h));
+}
+__device__ __forceinline__ float e4m3_to(unsigned char c) {
+  const __half_raw h = __nv_cvt_fp8_to_halfraw(c, __NV_E4M3);
+  return __half2float(__half(h));
+}
+
+}  // namespace rtp

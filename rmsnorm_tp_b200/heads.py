@@ -1,0 +1,357 @@
+"""The operators between the two norms of a transformer block, on one rank's heads.
+
+``qk_norm_rope`` (and its backward) norms the query and key heads and turns them by
+their positions; ``qk_norm_rope_write`` does so and puts keys and values into a
+``PagedKVCache``, which holds them in q's type or as e4m3 codes; ``paged_attention``
+is the attention of one new token of each sequence over that cache. Its output is
+the input ``a`` of ``FusedTPLinearRMSNorm``. Heads are split over a tensor-parallel
+group as the projection's columns are, so none of these exchanges anything. No
+counterpart in the reference. As in ``api``: ``AssertionError`` for the contract's
+checks, ``RMSNormTPError`` for what the library refuses, no fallback.
+"""
+from __future__ import annotations
+
+import ctypes
+import functools
+import struct
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+from ._lib import LIB, check
+from .api import _DTYPES, _stream_of, dtype_code
+
+# layouts of rmsnorm_qk_rope_args, rmsnorm_qk_rope_backward_args, rmsnorm_kv_cache and
+# rmsnorm_paged_attention_args (include/rmsnorm_tp_b200.h)
+_ROPE_ARGS = struct.Struct("@9Q10q2q2Q6ifi")
+_BACK_ARGS = struct.Struct("@12Qq8q2q6ifi")
+_CACHE = struct.Struct("@4Qq4i")
+_ATTN_ARGS = struct.Struct("@7Qq3q2q2ifi")
+
+_CACHE_DTYPES = {**_DTYPES, torch.float8_e4m3fn: _lib.KV_E4M3}
+
+
+def rope_table(max_positions: int, rotary_dim: int, base: float = 10000.0,
+               device=None) -> torch.Tensor:
+    """fp32 [max_positions, rotary_dim]: the cosines, then the sines, of position *
+    base^(-2i / rotary_dim). The angles are computed in 64 bits; any other table of
+    this layout (scaled frequencies, say) serves as well."""
+    if max_positions < 1 or rotary_dim < 2 or rotary_dim % 2:
+        raise AssertionError(f"max_positions {max_positions} must be positive and rotary_dim "
+                             f"{rotary_dim} even and positive")
+    freq = float(base) ** (-torch.arange(0, rotary_dim, 2, device=device, dtype=torch.float64) / rotary_dim)
+    angle = torch.arange(max_positions, device=device, dtype=torch.float64)[:, None] * freq
+    return torch.cat([angle.cos(), angle.sin()], 1).to(torch.float32)
+
+
+def _check_head_rows(name: str, t: torch.Tensor, like: torch.Tensor, heads: int) -> None:
+    if t.dtype != like.dtype or t.device != like.device:
+        raise AssertionError(f"{name} must have q's dtype and device, got {t.dtype} on {t.device}")
+    if t.dim() != 3 or t.shape[0] != like.shape[0] or t.shape[2] != like.shape[2] or \
+            (heads and t.shape[1] != heads):
+        raise AssertionError(f"{name} must be [tokens={like.shape[0]}, {heads or 'heads'}, "
+                             f"head_dim={like.shape[2]}], got {tuple(t.shape)}")
+    if t.stride(2) != 1:
+        raise AssertionError(f"{name}'s last dimension must have stride 1")
+
+
+def _check_turn(q: torch.Tensor, k: torch.Tensor, q_weight, k_weight, rope: torch.Tensor,
+                positions: torch.Tensor) -> None:
+    device = q.device
+    if not q.is_cuda:
+        raise AssertionError("q must be a CUDA tensor")
+    if q.dtype not in _DTYPES:
+        raise AssertionError(f"unsupported dtype {q.dtype}; expected float32, bfloat16 or float16")
+    if q.dim() != 3 or q.stride(2) != 1:
+        raise AssertionError("q must be [tokens, q_heads, head_dim] with stride 1 in the last "
+                             f"dimension, got {tuple(q.shape)} with strides {q.stride()}")
+    _check_head_rows("k", k, q, 0)
+    if (q_weight is None) != (k_weight is None):
+        raise AssertionError("give both q_weight and k_weight, or neither (rotation without norm)")
+    if q_weight is not None:
+        for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+            if w.dtype != q.dtype or w.device != device or w.shape != q.shape[2:] or not w.is_contiguous():
+                raise AssertionError(f"{name} must be contiguous [{q.shape[2]}] with q's dtype and device")
+    if rope.dtype != torch.float32 or rope.device != device or rope.dim() != 2 or not rope.is_contiguous():
+        raise AssertionError("rope must be a contiguous float32 [max_positions, rotary_dim] on q's device")
+    _check_index("positions", positions, q, torch.int64)
+
+
+def _check_index(name: str, t: torch.Tensor, q: torch.Tensor, dtype: torch.dtype) -> None:
+    if t.dtype != dtype or t.device != q.device or t.shape != q.shape[:1] or not t.is_contiguous():
+        raise AssertionError(f"{name} must be contiguous {dtype} [{q.shape[0]}] on q's device")
+
+
+def _turn(fn, what, q, k, v, q_out, k_out, q_weight, k_weight, rope, positions, cache, slots, eps,
+          interleaved) -> None:
+    device = q.device.index
+    n = q_weight is not None
+    args = _ROPE_ARGS.pack(
+        q.data_ptr(), k.data_ptr(), 0 if v is None else v.data_ptr(), q_out.data_ptr(),
+        0 if k_out is None else k_out.data_ptr(), q_weight.data_ptr() if n else 0,
+        k_weight.data_ptr() if n else 0, rope.data_ptr(), positions.data_ptr(),
+        q.stride(0), q.stride(1), k.stride(0), k.stride(1),
+        *((0, 0) if v is None else v.stride()[:2]), q_out.stride(0), q_out.stride(1),
+        *((0, 0) if k_out is None else k_out.stride()[:2]),
+        q.shape[0], rope.shape[0], 0 if cache is None else cache._address,
+        0 if slots is None else slots.data_ptr(), q.shape[1], k.shape[1], q.shape[2], rope.shape[1],
+        _DTYPES[q.dtype], bool(interleaved), eps, device)
+    check(fn(args, _stream_of(device)), what)
+
+
+def _fresh(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor],
+                 k_weight: Optional[torch.Tensor], rope: torch.Tensor, positions: torch.Tensor,
+                 eps: float = 1e-6, interleaved: bool = False, q_out: Optional[torch.Tensor] = None,
+                 k_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """RMSNorm of every query and key head, then the rotation by the token's position.
+
+    ``q`` [tokens, q_heads, head_dim] and ``k`` [tokens, kv_heads, head_dim] may be views
+    (column blocks of the projection's output); the weights are [head_dim], shared by the
+    heads, or both None (rotation alone). ``rope``: see ``rope_table``; its width is the
+    rotary_dim, and elements behind it are not turned. Pairs are (i, i + rotary_dim / 2),
+    or with ``interleaved`` (2i, 2i + 1). ``positions`` int64 [tokens]; one outside the
+    table makes the token's turned elements NaN. ``q_out`` / ``k_out`` receive the results
+    instead of fresh tensors and may be q / k themselves. fp32 inside, rounded once."""
+    _check_turn(q, k, q_weight, k_weight, rope, positions)
+    if q_out is None:
+        q_out = _fresh(q)
+    else:
+        _check_head_rows("q_out", q_out, q, q.shape[1])
+    if k_out is None:
+        k_out = _fresh(k)
+    else:
+        _check_head_rows("k_out", k_out, q, k.shape[1])
+    _turn(LIB.rmsnorm_qk_rope_forward, "rmsnorm_qk_rope_forward", q, k, None, q_out, k_out, q_weight,
+          k_weight, rope, positions, None, None, eps, interleaved)
+    return q_out, k_out
+
+
+def qk_norm_rope_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
+                          q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
+                          rope: torch.Tensor, positions: torch.Tensor, eps: float = 1e-6,
+                          interleaved: bool = False):
+    """Gradients ``(dq, dk, dq_weight, dk_weight)`` of ``qk_norm_rope`` for the output
+    gradients (the last two None without weights). The weights' gradients are sums over
+    tokens and heads in a fixed order; over a tensor-parallel group they are this rank's
+    heads' share. Capturable in a CUDA graph."""
+    _check_turn(q, k, q_weight, k_weight, rope, positions)
+    _check_head_rows("dq_out", dq_out, q, q.shape[1])
+    _check_head_rows("dk_out", dk_out, q, k.shape[1])
+    dq, dk = _fresh(q), _fresh(k)
+    n, d, device = q_weight is not None, q.shape[2], q.device.index
+    dw = ws = None
+    nbytes = 0
+    if n:
+        dw = torch.empty(2 * d, dtype=q.dtype, device=q.device)
+        nbytes = LIB.rmsnorm_qk_rope_backward_workspace_bytes(d)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    args = _BACK_ARGS.pack(
+        dq_out.data_ptr(), dk_out.data_ptr(), q.data_ptr(), k.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+        dw.data_ptr() if n else 0, q_weight.data_ptr() if n else 0, k_weight.data_ptr() if n else 0,
+        rope.data_ptr(), positions.data_ptr(), ws.data_ptr() if n else 0, nbytes,
+        dq_out.stride(0), dq_out.stride(1), dk_out.stride(0), dk_out.stride(1), q.stride(0), q.stride(1),
+        k.stride(0), k.stride(1), q.shape[0], rope.shape[0], q.shape[1], k.shape[1], d, rope.shape[1],
+        _DTYPES[q.dtype], bool(interleaved), eps, device)
+    check(LIB.rmsnorm_qk_rope_backward(args, _stream_of(device)), "rmsnorm_qk_rope_backward")
+    return dq, dk, dw[:d] if n else None, dw[d:] if n else None
+
+
+class _QkNormRopeFunction(torch.autograd.Function):
+    """Autograd around qk_norm_rope: forward kernel, backward kernel."""
+
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, rope, positions, eps, interleaved):
+        ctx.save_for_backward(q, k, q_weight, k_weight, rope, positions)
+        ctx.eps, ctx.interleaved = eps, interleaved
+        return qk_norm_rope(q, k, q_weight, k_weight, rope, positions, eps, interleaved)
+
+    @staticmethod
+    def backward(ctx, dq_out, dk_out):
+        q, k, q_weight, k_weight, rope, positions = ctx.saved_tensors
+        dq_out = dq_out if dq_out.stride(2) == 1 else dq_out.contiguous()
+        dk_out = dk_out if dk_out.stride(2) == 1 else dk_out.contiguous()
+        return (*qk_norm_rope_backward(dq_out, dk_out, q, k, q_weight, k_weight, rope, positions, ctx.eps,
+                                       ctx.interleaved), None, None, None, None)
+
+
+def qk_norm_rope_with_grad(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor],
+                           k_weight: Optional[torch.Tensor], rope: torch.Tensor, positions: torch.Tensor,
+                           eps: float = 1e-6, interleaved: bool = False):
+    """``qk_norm_rope`` recorded for autograd; its backward runs the backward kernel."""
+    return _QkNormRopeFunction.apply(q, k, q_weight, k_weight, rope, positions, eps, interleaved)
+
+
+class PagedKVCache:
+    """Keys and values of many sequences in pages of ``page_size`` tokens.
+
+    ``k`` and ``v`` are [num_pages, kv_heads, page_size, head_dim], so a head's rows of a
+    page lie in one piece; ``dtype`` float32, bfloat16, float16 or float8_e4m3fn. The last
+    holds codes, with a scale for each (token, head) in ``k_scale`` and ``v_scale``
+    [num_pages, kv_heads, page_size] fp32: scale = max(amax, 2^-100) / 448 of the row, code =
+    e4m3(x / scale), and a row stands for code * scale. A row with an infinity reads back
+    as NaN. The token at ``offset`` of ``page`` has slot page * page_size + offset; which
+    pages belong to which sequence is the caller's ``page_table``. head_dim is a multiple
+    of 16, at most 256. A fresh cache holds zeros."""
+
+    def __init__(self, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int,
+                 dtype: torch.dtype = torch.bfloat16, device=None):
+        device = torch.device("cuda") if device is None else torch.device(device)
+        if min(num_pages, page_size, num_kv_heads) < 1:
+            raise AssertionError("num_pages, page_size and num_kv_heads must be positive")
+        if dtype not in _CACHE_DTYPES:
+            raise AssertionError(f"unsupported cache dtype {dtype}")
+        shape = (num_pages, num_kv_heads, page_size)
+        k, v = (torch.zeros(*shape, head_dim, dtype=dtype, device=device) for _ in range(2))
+        scales = (None, None)
+        if dtype == torch.float8_e4m3fn:
+            scales = tuple(torch.zeros(shape, dtype=torch.float32, device=device) for _ in range(2))
+        self._adopt(k, v, *scales)
+
+    @classmethod
+    def from_tensors(cls, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None,
+                     v_scale: Optional[torch.Tensor] = None) -> "PagedKVCache":
+        """A cache over tensors that the caller holds (no copy)."""
+        cache = cls.__new__(cls)
+        cache._adopt(k, v, k_scale, v_scale)
+        return cache
+
+    def _adopt(self, k, v, k_scale, v_scale) -> None:
+        if k.dtype not in _CACHE_DTYPES:
+            raise AssertionError(f"unsupported cache dtype {k.dtype}")
+        if not k.is_cuda or k.dim() != 4:
+            raise AssertionError("k must be a CUDA tensor [num_pages, kv_heads, page_size, head_dim]")
+        for name, t in (("k", k), ("v", v)):
+            if t.shape != k.shape or t.dtype != k.dtype or t.device != k.device or not t.is_contiguous():
+                raise AssertionError(f"{name} must be contiguous with k's shape, dtype and device")
+        e4m3 = k.dtype == torch.float8_e4m3fn
+        for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
+            if (t is not None) != e4m3:
+                raise AssertionError(f"{name} belongs to a float8_e4m3fn cache, and only to one")
+            if e4m3 and (t.shape != k.shape[:3] or t.dtype != torch.float32 or t.device != k.device
+                         or not t.is_contiguous()):
+                raise AssertionError(f"{name} must be contiguous float32 {tuple(k.shape[:3])} on k's device")
+        self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = k.shape
+        if self.head_dim % 16 or not 16 <= self.head_dim <= 256:
+            raise AssertionError(f"head_dim {self.head_dim} must be a multiple of 16, at most 256")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.dtype, self.device = k.dtype, k.device
+        self._struct = ctypes.create_string_buffer(_CACHE.pack(
+            k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if e4m3 else 0,
+            v_scale.data_ptr() if e4m3 else 0, self.num_pages, self.page_size, self.num_kv_heads,
+            self.head_dim, _CACHE_DTYPES[k.dtype]))
+        self._address = ctypes.addressof(self._struct)
+
+    def read(self, slots: torch.Tensor, dtype: Optional[torch.dtype] = None):
+        """(k, v) [count, kv_heads, head_dim] of ``dtype``: the rows at ``slots`` (int64
+        [count]), an e4m3 row as code * scale rounded once. A slot outside the cache gives
+        zeros. ``dtype`` is the cache's own unless given (bfloat16 for an e4m3 cache)."""
+        if dtype is None:
+            dtype = torch.bfloat16 if self.dtype == torch.float8_e4m3fn else self.dtype
+        code = dtype_code(dtype)
+        if slots.dtype != torch.int64 or slots.device != self.device or slots.dim() != 1 or \
+                not slots.is_contiguous():
+            raise AssertionError("slots must be contiguous int64 [count] on the cache's device")
+        count = slots.shape[0]
+        k, v = (torch.empty(count, self.num_kv_heads, self.head_dim, dtype=dtype, device=self.device)
+                for _ in range(2))
+        check(LIB.rmsnorm_kv_read(self._address, k.data_ptr(), v.data_ptr(), slots.data_ptr(), count, code,
+                                  self.device.index, _stream_of(self.device.index)), "rmsnorm_kv_read")
+        return k, v
+
+
+def qk_norm_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight: Optional[torch.Tensor],
+                       k_weight: Optional[torch.Tensor], rope: torch.Tensor, positions: torch.Tensor,
+                       cache: PagedKVCache, slots: torch.Tensor, eps: float = 1e-6,
+                       interleaved: bool = False, q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``qk_norm_rope`` whose keys go into ``cache`` with ``v`` beside them; returns the
+    queries. ``slots`` int64 [tokens] are distinct within a call; a token whose slot lies
+    outside the cache (-1: padding) leaves the cache as it is. The cache has q's dtype, or
+    float8_e4m3fn (quantised from the fp32 values)."""
+    _check_turn(q, k, q_weight, k_weight, rope, positions)
+    _check_head_rows("v", v, q, k.shape[1])
+    _check_index("slots", slots, q, torch.int64)
+    if cache.device != q.device or cache.num_kv_heads != k.shape[1] or cache.head_dim != q.shape[2]:
+        raise AssertionError(f"the cache holds {cache.num_kv_heads} heads of {cache.head_dim} on "
+                             f"{cache.device}, the call has {k.shape[1]} of {q.shape[2]} on {q.device}")
+    if cache.dtype != q.dtype and cache.dtype != torch.float8_e4m3fn:
+        raise AssertionError(f"a {cache.dtype} cache does not take {q.dtype}")
+    if q_out is None:
+        q_out = _fresh(q)
+    else:
+        _check_head_rows("q_out", q_out, q, q.shape[1])
+    _turn(LIB.rmsnorm_qk_rope_write, "rmsnorm_qk_rope_write", q, k, v, q_out, None, q_weight, k_weight,
+          rope, positions, cache, slots, eps, interleaved)
+    return q_out
+
+
+def _attention_args(q, out, lse, page_table, seq_lens, ws, ws_bytes, cache_address, strides, table_stride,
+                    batch, max_pages, q_heads, dtype, scale, device) -> bytes:
+    return _ATTN_ARGS.pack(cache_address, q, out, lse, page_table, seq_lens, ws, ws_bytes, *strides,
+                           table_stride, batch, max_pages, q_heads, dtype, scale, device)
+
+
+@functools.lru_cache(maxsize=4096)
+def _attention_workspace(num_pages, page_size, kv_heads, head_dim, cache_dtype, batch, max_pages, q_heads,
+                         dtype, device) -> int:
+    """Bytes for a call of these sizes (a function of sizes alone); raises what the
+    library refuses."""
+    some = 256   # an address that the size check takes and never follows
+    cache = ctypes.create_string_buffer(_CACHE.pack(some, some, some, some, num_pages, page_size, kv_heads,
+                                                    head_dim, cache_dtype))
+    nbytes = LIB.rmsnorm_paged_attention_workspace_bytes(_attention_args(
+        some, some, 0, some, some, 0, 0, ctypes.addressof(cache), (0, 0), 0, batch, max_pages, q_heads,
+        dtype, 1.0, device))
+    if nbytes == 0 and batch > 0:
+        raise _lib.RMSNormTPError(_lib.ERR_INVALID, f"rmsnorm_paged_attention: {_lib.last_error()}")
+    return nbytes
+
+
+def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tensor, seq_lens: torch.Tensor,
+                    scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                    return_lse: bool = False):
+    """Attention of one new token of each sequence over its cached tokens (that token's
+    own key among them: write it first).
+
+    ``q`` [batch, q_heads, head_dim], q_heads a multiple of the cache's heads, of the
+    cache's dtype or any for an e4m3 cache; ``page_table`` int32 [batch, max_pages];
+    ``seq_lens`` int32 [batch], on the device: the work is divided as they say when the
+    kernel runs, so a captured call follows them. Returns ``out`` [batch, q_heads,
+    head_dim], with ``return_lse`` also the fp32 logarithm of each head's sum of
+    exponentials [batch, q_heads]. A sequence without tokens gives zeros and -inf; pages
+    outside the cache are left out, lengths cut to max_pages * page_size. ``scale`` is
+    head_dim^-0.5 unless given."""
+    if not q.is_cuda or q.dim() != 3 or q.stride(2) != 1:
+        raise AssertionError("q must be a CUDA tensor [batch, q_heads, head_dim] with stride 1 in the last "
+                             f"dimension, got {tuple(q.shape)}")
+    if q.dtype not in _DTYPES:
+        raise AssertionError(f"unsupported dtype {q.dtype}; expected float32, bfloat16 or float16")
+    batch, heads, d = q.shape
+    if cache.device != q.device or d != cache.head_dim or heads % cache.num_kv_heads:
+        raise AssertionError(f"q has {heads} heads of {d} on {q.device}, the cache {cache.num_kv_heads} of "
+                             f"{cache.head_dim} on {cache.device}")
+    if cache.dtype != q.dtype and cache.dtype != torch.float8_e4m3fn:
+        raise AssertionError(f"a {cache.dtype} cache does not serve {q.dtype} queries")
+    if page_table.dtype != torch.int32 or page_table.device != q.device or page_table.dim() != 2 or \
+            page_table.shape[0] != batch or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        raise AssertionError(f"page_table must be int32 [{batch}, max_pages] on q's device, rows in one piece")
+    _check_index("seq_lens", seq_lens, q, torch.int32)
+    if out is None:
+        out = _fresh(q)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
+        raise AssertionError("out must be contiguous with q's shape, dtype and device")
+    lse = torch.empty(batch, heads, dtype=torch.float32, device=q.device) if return_lse else None
+    max_pages, device, dtype = page_table.shape[1], q.device.index, _DTYPES[q.dtype]
+    nbytes = _attention_workspace(cache.num_pages, cache.page_size, cache.num_kv_heads, d,
+                                  _CACHE_DTYPES[cache.dtype], batch, max_pages, heads, dtype, device)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    args = _attention_args(q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0,
+                           page_table.data_ptr(), seq_lens.data_ptr(), ws.data_ptr(), nbytes,
+                           cache._address, q.stride()[:2], page_table.stride(0), batch, max_pages, heads,
+                           dtype, d ** -0.5 if scale is None else scale, device)
+    check(LIB.rmsnorm_paged_attention(args, _stream_of(device)), "rmsnorm_paged_attention")
+    return (out, lse) if return_lse else out
