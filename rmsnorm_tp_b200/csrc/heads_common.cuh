@@ -100,6 +100,26 @@ inline bool view_apart(const View& a) {
   return heads_inside || tokens_inside;
 }
 
+// threadIdx.x as a value made after this point: addresses formed with it cannot be loaded
+// before a preceding grid_dep_wait, read-only loads among them.
+__device__ __forceinline__ int thread_here() {
+  int t = threadIdx.x;
+  asm volatile("" : "+r"(t));
+  return t;
+}
+
+// Page and offset of a slot; 32-bit division where the cache's slots allow it.
+__device__ __forceinline__ void page_of(int64_t slot, int page, int64_t num_slots, int64_t& pg, int& off) {
+  if (num_slots <= 0xFFFFFFFFll) {
+    const unsigned p = (unsigned)slot / (unsigned)page;
+    pg = p;
+    off = (int)((unsigned)slot - p * (unsigned)page);
+  } else {
+    pg = slot / page;
+    off = (int)(slot - pg * page);
+  }
+}
+
 // ---- cache elements -----------------------------------------------------------
 constexpr float kE4M3Max = 448.f;
 // Smallest row maximum a scale is made of (2^-100): keeps 448 / maximum finite

@@ -72,42 +72,72 @@ struct ReadArgs {
 
 constexpr int kBlock = 256;
 
-// One thread per 16 elements of an output row.
+// 8 elements from memory in fp32.
+template <typename TC>
+__device__ __forceinline__ void load8(const TC* p, float (&f)[8]) {
+  if constexpr (sizeof(TC) == 1) {
+    uint2 c;
+    asm("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(c.x), "=r"(c.y) : "l"(p));
+    const uint32_t w[2] = {c.x, c.y};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 v = e4m3x2_to((unsigned short)(w[i / 2] >> (16 * (i & 1))));
+      f[2 * i] = v.x;
+      f[2 * i + 1] = v.y;
+    }
+  } else if constexpr (sizeof(TC) == 2) {
+    Pack<TC>::unpack(ptx::ld_stream_v4(p), f);
+  } else {
+    const uint4 a = ptx::ld_stream_v4(p), b = ptx::ld_stream_v4(p + 4);
+    const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(w[e]);
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
+  if constexpr (sizeof(T) == 2) {
+    ptx::st_v4(p, Pack<T>::pack(f));
+  } else {
+    const float a[4] = {f[0], f[1], f[2], f[3]}, b[4] = {f[4], f[5], f[6], f[7]};
+    ptx::st_v4(p, Pack<T>::pack(a));
+    ptx::st_v4(p + 4, Pack<T>::pack(b));
+  }
+}
+
+// A thread brings 8 elements of K and of V of one row, so that a warp's 16-bit outputs
+// are 512 bytes in one piece. Bound by HBM: each row read once, written once.
 template <typename TC, typename T>
 __global__ void __launch_bounds__(kBlock) kv_read_kernel(const __grid_constant__ ReadArgs a) {
-  constexpr bool kE4M3 = sizeof(TC) == 1;
   ptx::grid_dep_wait();
-  const int per_row = a.d / 16;
-  const int64_t n = a.count * a.heads * per_row;
-  const int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x;
-  if (i >= 2 * n) return;
-  const bool is_v = i >= n;
-  const int64_t u = is_v ? i - n : i;
-  const int64_t row = u / per_row;
-  const int e0 = (int)(u - row * per_row) * 16;
-  const int64_t t = row / a.heads;
+  ptx::grid_dep_launch_dependents();
+  const unsigned tid = thread_here();
+  const unsigned per_row = a.d / 8, rows = kBlock / per_row;   // 2 to 32; rows of this CTA
+  const unsigned r = tid / per_row, e0 = (tid - r * per_row) * 8;
+  const int64_t row = (int64_t)blockIdx.x * rows + r;
+  if (r >= rows || row >= a.count * a.heads) return;
+  const int64_t t = (unsigned)row / (unsigned)a.heads;   // at most 2^31 rows
   const int h = (int)(row - t * a.heads);
   const int64_t slot = a.slots[t];
-  float f[16];
-  if (slot < 0 || slot >= a.num_slots) {
+  float k[8] = {}, v[8] = {};
+  if (slot >= 0 && slot < a.num_slots) {
+    int64_t pg;
+    int off;
+    page_of(slot, a.page, a.num_slots, pg, off);
+    const int64_t at = (pg * a.heads + h) * a.page + off;
+    load8(static_cast<const TC*>(a.k) + at * a.d + e0, k);
+    load8(static_cast<const TC*>(a.v) + at * a.d + e0, v);
+    if constexpr (sizeof(TC) == 1) {
+      const float ks = a.ks[at], vs = a.vs[at];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) f[e] = 0.f;
-  } else {
-    const int64_t pg = slot / a.page;
-    const int64_t at = (pg * a.heads + h) * a.page + (slot - pg * a.page);
-    const TC* x = static_cast<const TC*>(is_v ? a.v : a.k) + at * a.d + e0;
-    const float scale = kE4M3 ? (is_v ? a.vs : a.ks)[at] : 1.f;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      if constexpr (kE4M3)
-        f[e] = e4m3_to(reinterpret_cast<const unsigned char*>(x)[e]) * scale;
-      else
-        f[e] = Pack<TC>::to_f(x[e]);
+      for (int e = 0; e < 8; ++e) {
+        k[e] *= ks;
+        v[e] *= vs;
+      }
     }
   }
-  T* y = static_cast<T*>(is_v ? a.vo : a.ko) + row * a.d + e0;
-#pragma unroll
-  for (int e = 0; e < 16; ++e) y[e] = Pack<T>::from_f(f[e]);
+  store8(static_cast<T*>(a.ko) + row * a.d + e0, k);
+  store8(static_cast<T*>(a.vo) + row * a.d + e0, v);
 }
 
 template <typename T>
@@ -150,9 +180,9 @@ extern "C" int rmsnorm_kv_read(const rmsnorm_kv_cache* c, void* k_out, void* v_o
   const void* fn = dtype == RMSNORM_TP_F32    ? read_fn<float>(c->dtype)
                    : dtype == RMSNORM_TP_BF16 ? read_fn<__nv_bfloat16>(c->dtype)
                                               : read_fn<__half>(c->dtype);
-  const int64_t n = 2 * count * c->kv_heads * (c->head_dim / 16);
+  const int64_t per_block = kBlock / (c->head_dim / 8), rows = count * c->kv_heads;
   void* args[] = {&a};
-  const cudaError_t e = launch_dependent(fn, dim3((unsigned)((n + kBlock - 1) / kBlock)), dim3(kBlock), 0,
-                                         args, reinterpret_cast<cudaStream_t>(stream));
+  const cudaError_t e = launch_dependent(fn, dim3((unsigned)((rows + per_block - 1) / per_block)),
+                                         dim3(kBlock), 0, args, reinterpret_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? RMSNORM_TP_OK : launch_failed(e, who);
 }

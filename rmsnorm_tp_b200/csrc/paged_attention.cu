@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(kAnyBlock) attention_any_kernel(const __grid_c
   __shared__ int64_t at[kAnyBlock];
   __shared__ float red[kAnyBlock / 32];
   ptx::grid_dep_wait();
-  const int h = blockIdx.x, tid = threadIdx.x;
+  const int h = blockIdx.x, tid = thread_here();
   const int64_t b = blockIdx.y, split = blockIdx.z;
   const int kvh = h / (a.hq / a.hk);
   const TQ* qg = static_cast<const TQ*>(a.q) + b * a.qst + h * a.qsh;
@@ -130,19 +130,20 @@ __global__ void __launch_bounds__(kAnyBlock) attention_any_kernel(const __grid_c
 template <typename TQ>
 __global__ void __launch_bounds__(kAnyBlock) attention_join_any_kernel(const __grid_constant__ AttnArgs a) {
   ptx::grid_dep_wait();
+  const int tid = thread_here();
   const int64_t row = blockIdx.x;
   const float* w = a.part + row * a.splits * (a.d + 2);
   float m = -INFINITY, l = 0.f;
   for (int s = 0; s < a.splits; ++s) m = fmaxf(m, w[s * (a.d + 2)]);
   const float ref = m == -INFINITY ? 0.f : m;
   for (int s = 0; s < a.splits; ++s) l += exp2f(w[s * (a.d + 2)] - ref) * w[s * (a.d + 2) + 1];
-  for (int i = threadIdx.x; i < a.d; i += kAnyBlock) {
+  for (int i = tid; i < a.d; i += kAnyBlock) {
     float o = 0.f;
     for (int s = 0; s < a.splits; ++s)
       o = fmaf(exp2f(w[s * (a.d + 2)] - ref), w[s * (a.d + 2) + 2 + i], o);
     static_cast<TQ*>(a.out)[row * a.d + i] = Pack<TQ>::from_f(l == 0.f ? 0.f : o / l);
   }
-  if (a.lse && threadIdx.x == 0) a.lse[row] = kLn2 * (ref + log2f(l));
+  if (a.lse && tid == 0) a.lse[row] = kLn2 * (ref + log2f(l));
 }
 
 // ---- tensor cores: 16-bit queries, head_dim 64, 96, 128, 192 or 256 ----------------
@@ -314,7 +315,7 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
   __shared__ int s_b;
   ptx::grid_dep_wait();
   ptx::grid_dep_launch_dependents();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = thread_here(), lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, qd = lane & 3;
 
   // this CTA's run of tiles [t0, t1): every thread sums the tiles of a run of sequences
@@ -715,7 +716,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const _
   __shared__ float s_x[kJoinWarps];
   ptx::grid_dep_wait();
   ptx::grid_dep_launch_dependents();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = thread_here(), lane = tid & 31, warp = tid >> 5;
   // sequences without tokens have no tile: their zeros are written here
   const int64_t blocks = (int64_t)gridDim.x * gridDim.y;
   for (int64_t b = (int64_t)blockIdx.y * gridDim.x + blockIdx.x; b < a.batch; b += blocks) {

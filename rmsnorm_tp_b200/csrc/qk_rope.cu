@@ -69,9 +69,11 @@ __device__ __forceinline__ void pair_of(int u, int d, int r, int interleaved, in
 }
 
 // Element offset of a cache row.
-__device__ __forceinline__ int64_t cache_row(int64_t slot, int head, int heads, int page) {
-  const int64_t pg = slot / page;
-  return (pg * heads + head) * page + (slot - pg * page);
+__device__ __forceinline__ int64_t cache_row(int64_t slot, int head, const QkArgs& a) {
+  int64_t pg;
+  int off;
+  page_of(slot, a.page, a.num_slots, pg, off);
+  return (pg * a.hk + head) * a.page + off;
 }
 
 // ---- any head_dim, alignment and stride: one warp per row ----------------------
@@ -80,11 +82,11 @@ __device__ __forceinline__ int64_t cache_row(int64_t slot, int head, int heads, 
 template <typename T, bool kWrite>
 __global__ void __launch_bounds__(kBlock) qk_rope_any_kernel(const __grid_constant__ QkArgs a) {
   ptx::grid_dep_wait();
-  const int lane = threadIdx.x & 31;
+  const int tid = thread_here(), lane = tid & 31;
   const int heads = a.hq + a.hk + (kWrite ? a.hk : 0);
-  const int64_t row = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  const int64_t row = (int64_t)blockIdx.x * kWarps + (tid >> 5);
   if (row >= a.tokens * heads) return;
-  const int64_t t = row / heads;
+  const int64_t t = (unsigned)row / (unsigned)heads;   // at most 2^31 rows
   const int h = (int)(row - t * heads);
   const bool is_q = h < a.hq, is_v = kWrite && h >= a.hq + a.hk;
   const int hh = is_q ? h : is_v ? h - a.hq - a.hk : h - a.hq;
@@ -136,7 +138,7 @@ __global__ void __launch_bounds__(kBlock) qk_rope_any_kernel(const __grid_consta
   }
   const int64_t slot = a.slots[t];
   if (slot < 0 || slot >= a.num_slots) return;
-  const int64_t at = cache_row(slot, hh, a.hk, a.page);
+  const int64_t at = cache_row(slot, hh, a);
   void* cache = is_v ? a.vc : a.kc;
   if (!a.e4m3) {
     T* y = static_cast<T*>(cache) + at * a.d;
@@ -178,7 +180,7 @@ __global__ void __launch_bounds__(kBlock)
 qk_rope_backward_any_kernel(const __grid_constant__ QkBackArgs a) {
   extern __shared__ float dw[];     // [kWarps][d]
   ptx::grid_dep_wait();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int tid = thread_here(), lane = tid & 31, warp = tid >> 5;
   const int pairs = a.r / 2 + (a.d - a.r + 1) / 2;
   float* mine = dw + warp * a.d;
   for (int part = 0; part < 2; ++part) {
@@ -249,12 +251,385 @@ qk_rope_backward_any_kernel(const __grid_constant__ QkBackArgs a) {
     }
     if (!a.norm) continue;
     __syncthreads();
-    for (int i = threadIdx.x; i < a.d; i += kBlock) {
+    for (int i = tid; i < a.d; i += kBlock) {
       float s = 0.f;
       for (int v = 0; v < kWarps; ++v) s += dw[v * a.d + i];
       a.ws[((int64_t)blockIdx.x * 2 + part) * a.d + i] = s;
     }
     __syncthreads();
+  }
+}
+
+// ---- 16-byte vectors: a head's row in the registers of a group of lanes ------------
+//
+// A lane holds one unit, two 16-byte vectors of the row chosen so that the turn stays
+// inside the lane: elements [8 j, 8 j + 8) and their partners half a rotary_dim on
+// (neighbouring vectors where pairs are interleaved or not turned). head_dim 128 in
+// bf16 takes 8 lanes, so a warp works on 4 rows at once; cosines, sines and weights stay
+// in registers over the rows of a token. Bound by HBM: each row is read once and written
+// once; the next row's vectors are in flight while a row is computed.
+template <typename T>
+struct UnitOf {
+  int ea, eb;            // first elements of the two vectors
+  bool on, turned;
+  __device__ __forceinline__ UnitOf(int j, int d, int r, int interleaved) {
+    constexpr int E = Pack<T>::kE;
+    on = j * 2 * E < d;
+    turned = j * 2 * E < r;
+    if (interleaved || !turned) {
+      ea = j * 2 * E;
+      eb = ea + E;
+    } else {
+      ea = j * E;
+      eb = ea + r / 2;
+    }
+  }
+};
+
+// Cosines and sines of a unit: table columns [j E, j E + E) and rotary_dim / 2 on, in
+// either pairing.
+template <typename T>
+struct Turn {
+  static constexpr int E = Pack<T>::kE;
+  float c[E], s[E];
+  __device__ __forceinline__ void load(const float* rope, int64_t pos, int64_t max_pos, int r, int j) {
+    const bool known = pos >= 0 && pos < max_pos;
+    const float4* row = reinterpret_cast<const float4*>(rope + (known ? pos : 0) * r + j * E);
+    const float4* row2 = reinterpret_cast<const float4*>(rope + (known ? pos : 0) * r + r / 2 + j * E);
+#pragma unroll
+    for (int i = 0; i < E / 4; ++i) {
+      const float4 a = __ldg(row + i), b = __ldg(row2 + i);
+      c[4 * i] = a.x, c[4 * i + 1] = a.y, c[4 * i + 2] = a.z, c[4 * i + 3] = a.w;
+      s[4 * i] = b.x, s[4 * i + 1] = b.y, s[4 * i + 2] = b.z, s[4 * i + 3] = b.w;
+    }
+    if (!known)
+#pragma unroll
+      for (int i = 0; i < E; ++i) c[i] = s[i] = quiet_nan();
+  }
+  // (a, b) turned by the angle (back: by its negative).
+  template <bool kBack>
+  __device__ __forceinline__ void apply(float (&a)[E], float (&b)[E], int interleaved) const {
+    if (!interleaved) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) pair<kBack>(a[i], b[i], c[i], s[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < E / 2; ++i) {
+        pair<kBack>(a[2 * i], a[2 * i + 1], c[i], s[i]);
+        pair<kBack>(b[2 * i], b[2 * i + 1], c[E / 2 + i], s[E / 2 + i]);
+      }
+    }
+  }
+  template <bool kBack>
+  static __device__ __forceinline__ void pair(float& a, float& b, float c, float s) {
+    const float x = kBack ? a * c + b * s : a * c - b * s;
+    b = kBack ? b * c - a * s : a * s + b * c;
+    a = x;
+  }
+};
+
+template <int L>
+__device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+  return v;
+}
+template <int L>
+__device__ __forceinline__ float lanes_max(float v) {
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+  return v;
+}
+
+// Rows are numbered over tokens, then heads (q, k, v); a warp takes `run` groups of
+// 32 / L neighbouring rows.
+template <typename T, int L, bool kWrite>
+__global__ void __launch_bounds__(kBlock) qk_rope_kernel(const __grid_constant__ QkArgs a, int run) {
+  constexpr int E = Pack<T>::kE, kRows = 32 / L;
+  ptx::grid_dep_wait();
+  ptx::grid_dep_launch_dependents();
+  const int tid = thread_here(), lane = tid & 31, j = lane % L;
+  const UnitOf<T> u(j, a.d, a.r, a.interleaved);
+  const int heads = a.hq + a.hk + (kWrite ? a.hk : 0);
+  const int64_t rows = a.tokens * heads;
+  int64_t row = ((int64_t)blockIdx.x * kWarps + (tid >> 5)) * run * kRows + lane / L;
+  int64_t t = (unsigned)row / (unsigned)heads;   // at most 2^31 rows and a CTA's more
+  int h = (int)(row - t * heads);
+  uint4 wq[2] = {}, wk[2] = {};
+  if (a.norm && u.on) {
+    wq[0] = ptx::ld_cached_v4(static_cast<const T*>(a.qw) + u.ea);
+    wq[1] = ptx::ld_cached_v4(static_cast<const T*>(a.qw) + u.eb);
+    wk[0] = ptx::ld_cached_v4(static_cast<const T*>(a.kw) + u.ea);
+    wk[1] = ptx::ld_cached_v4(static_cast<const T*>(a.kw) + u.eb);
+  }
+  auto fetch = [&](int64_t t, int h, bool live, uint4 (&x)[2]) {
+    if (!live || !u.on) {
+      x[0] = x[1] = make_uint4(0u, 0u, 0u, 0u);
+      return;
+    }
+    const T* p;
+    if (h < a.hq) p = static_cast<const T*>(a.q.p) + t * a.q.st + h * a.q.sh;
+    else if (!kWrite || h < a.hq + a.hk) p = static_cast<const T*>(a.k.p) + t * a.k.st + (h - a.hq) * a.k.sh;
+    else p = static_cast<const T*>(a.v.p) + t * a.v.st + (h - a.hq - a.hk) * a.v.sh;
+    x[0] = ptx::ld_stream_v4(p + u.ea);
+    x[1] = ptx::ld_stream_v4(p + u.eb);
+  };
+  Turn<T> turn;
+  int64_t turn_of = -1, slot = -1;
+  uint4 next[2];
+  fetch(t, h, row < rows, next);
+#pragma unroll 1
+  for (int i = 0; i < run; ++i) {
+    const bool live = row < rows;
+    if (!__any_sync(0xFFFFFFFFu, live)) break;
+    if (live && t != turn_of) {
+      turn_of = t;
+      const int64_t pos = a.positions[t];
+      if (kWrite) slot = a.slots[t];
+      if (u.turned) turn.load(a.rope, pos, a.max_pos, a.r, j);
+    }
+    const uint4 x[2] = {next[0], next[1]};
+    const int64_t t_now = t;
+    const int h_now = h;
+    row += kRows;
+    h += kRows;
+    while (h >= heads) {
+      h -= heads;
+      ++t;
+    }
+    if (i + 1 < run) fetch(t, h, row < rows, next);
+
+    const bool is_q = h_now < a.hq, is_v = kWrite && h_now >= a.hq + a.hk;
+    float ya[E], yb[E];
+    Pack<T>::unpack(x[0], ya);
+    Pack<T>::unpack(x[1], yb);
+    if (a.norm) {
+      float sa = 0.f, sb = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        sa = fmaf(ya[e], ya[e], sa);
+        sb = fmaf(yb[e], yb[e], sb);
+      }
+      const float inv = rsqrtf(lanes_sum<L>(sa + sb) / (float)a.d + a.eps);
+      if (!is_v) {
+        float wa[E], wb[E];
+        Pack<T>::unpack(is_q ? wq[0] : wk[0], wa);
+        Pack<T>::unpack(is_q ? wq[1] : wk[1], wb);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          ya[e] = (ya[e] * inv) * wa[e];
+          yb[e] = (yb[e] * inv) * wb[e];
+        }
+      }
+    }
+    if (u.turned && !is_v) turn.template apply<false>(ya, yb, a.interleaved);
+    if (!kWrite || is_q) {
+      if (live && u.on) {
+        T* y = is_q ? static_cast<T*>(a.qo.p) + t_now * a.qo.st + h_now * a.qo.sh
+                    : static_cast<T*>(a.ko.p) + t_now * a.ko.st + (h_now - a.hq) * a.ko.sh;
+        ptx::st_v4(y + u.ea, Pack<T>::pack(ya));
+        ptx::st_v4(y + u.eb, Pack<T>::pack(yb));
+      }
+      if (!kWrite) continue;
+    }
+    if constexpr (kWrite) {
+      const bool keep = live && !is_q && slot >= 0 && slot < a.num_slots;
+      const int64_t at = keep ? cache_row(slot, is_v ? h_now - a.hq - a.hk : h_now - a.hq, a) : 0;
+      void* cache = is_v ? a.vc : a.kc;
+      if (!a.e4m3) {
+        if (keep && u.on) {
+          T* y = static_cast<T*>(cache) + at * a.d;
+          ptx::st_v4(y + u.ea, Pack<T>::pack(ya));
+          ptx::st_v4(y + u.eb, Pack<T>::pack(yb));
+        }
+        continue;
+      }
+      if (!__any_sync(0xFFFFFFFFu, keep)) continue;
+      float most = kE4M3Floor;
+#pragma unroll
+      for (int e = 0; e < E; ++e) most = fmaxf(most, fmaxf(fabsf(ya[e]), fabsf(yb[e])));
+      most = lanes_max<L>(most);
+      if (keep && u.on) {
+        const float to = kE4M3Max / most;
+        unsigned char* y = static_cast<unsigned char*>(cache) + at * a.d;
+        uint32_t ca[E / 4], cb[E / 4];
+#pragma unroll
+        for (int e = 0; e < E / 4; ++e) {
+          ca[e] = e4m3x2_of(ya[4 * e] * to, ya[4 * e + 1] * to) |
+                  (uint32_t)e4m3x2_of(ya[4 * e + 2] * to, ya[4 * e + 3] * to) << 16;
+          cb[e] = e4m3x2_of(yb[4 * e] * to, yb[4 * e + 1] * to) |
+                  (uint32_t)e4m3x2_of(yb[4 * e + 2] * to, yb[4 * e + 3] * to) << 16;
+        }
+        if constexpr (E == 8) {
+          *reinterpret_cast<uint2*>(y + u.ea) = make_uint2(ca[0], ca[1]);
+          *reinterpret_cast<uint2*>(y + u.eb) = make_uint2(cb[0], cb[1]);
+        } else {
+          *reinterpret_cast<uint32_t*>(y + u.ea) = ca[0];
+          *reinterpret_cast<uint32_t*>(y + u.eb) = cb[0];
+        }
+        if (j == 0) (is_v ? a.vs : a.ks)[at] = most / kE4M3Max;
+      }
+    }
+  }
+}
+
+// The backward: g and x in registers, dw summed per lane over the CTA's rows (a run of
+// each operand's rows for each warp), then over the warp's row groups and the warps in a
+// fixed order.
+template <typename T, int L>
+__global__ void __launch_bounds__(kBlock, 2)
+qk_rope_backward_kernel(const __grid_constant__ QkBackArgs a) {
+  constexpr int E = Pack<T>::kE, kRows = 32 / L;
+  extern __shared__ float dw[];     // [kWarps][d]
+  ptx::grid_dep_wait();
+  ptx::grid_dep_launch_dependents();
+  const int tid = thread_here(), lane = tid & 31, warp = tid >> 5, j = lane % L;
+  const UnitOf<T> u(j, a.d, a.r, a.interleaved);
+  const int64_t workers = (int64_t)gridDim.x * kWarps, me = (int64_t)blockIdx.x * kWarps + warp;
+  const float rd = 1.f / (float)a.d;
+#pragma unroll 1
+  for (int part = 0; part < 2; ++part) {
+    const int heads = part == 0 ? a.hq : a.hk;
+    const Rows xr = part == 0 ? a.q : a.k, gr = part == 0 ? a.dqo : a.dko;
+    T* dx = static_cast<T*>(part == 0 ? a.dq : a.dk);
+    float wa[E] = {}, wb[E] = {}, da[E] = {}, db[E] = {};
+    if (a.norm && u.on) {
+      const T* w = static_cast<const T*>(part == 0 ? a.qw : a.kw);
+      Pack<T>::unpack(ptx::ld_cached_v4(w + u.ea), wa);
+      Pack<T>::unpack(ptx::ld_cached_v4(w + u.eb), wb);
+    }
+    const int64_t rows = a.tokens * heads, groups = (rows + kRows - 1) / kRows;
+    const int64_t first = groups * me / workers, end = groups * (me + 1) / workers;
+    int64_t row = first * kRows + lane / L;
+    int64_t t = row / heads;
+    int h = (int)(row - t * heads);
+    Turn<T> turn;
+    int64_t turn_of = -1;
+    uint4 x[2], g[2];
+    auto fetch = [&]() {
+      x[0] = x[1] = g[0] = g[1] = make_uint4(0u, 0u, 0u, 0u);
+      if (row >= rows || !u.on) return;
+      const T* p = static_cast<const T*>(gr.p) + t * gr.st + h * gr.sh;
+      g[0] = ptx::ld_stream_v4(p + u.ea);
+      g[1] = ptx::ld_stream_v4(p + u.eb);
+      if (a.norm) {
+        p = static_cast<const T*>(xr.p) + t * xr.st + h * xr.sh;
+        x[0] = ptx::ld_stream_v4(p + u.ea);
+        x[1] = ptx::ld_stream_v4(p + u.eb);
+      }
+    };
+    if (first < end) fetch();
+#pragma unroll 1
+    for (int64_t i = first; i < end; ++i) {
+      const bool live = row < rows;
+      if (live && t != turn_of) {
+        turn_of = t;
+        if (u.turned) turn.load(a.rope, a.positions[t], a.max_pos, a.r, j);
+      }
+      float xa[E], xb[E], ga[E], gb[E];
+      Pack<T>::unpack(x[0], xa);
+      Pack<T>::unpack(x[1], xb);
+      Pack<T>::unpack(g[0], ga);
+      Pack<T>::unpack(g[1], gb);
+      T* y = dx + row * a.d;
+      row += kRows;
+      h += kRows;
+      while (h >= heads) {
+        h -= heads;
+        ++t;
+      }
+      if (i + 1 < end) fetch();
+      if (u.turned && live) turn.template apply<true>(ga, gb, a.interleaved);
+      if (a.norm) {
+        float ss = 0.f, sg = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          ss = fmaf(xa[e], xa[e], fmaf(xb[e], xb[e], ss));
+          sg = fmaf(ga[e] * wa[e], xa[e], fmaf(gb[e] * wb[e], xb[e], sg));
+        }
+        ss = lanes_sum<L>(ss);
+        sg = lanes_sum<L>(sg);
+        const float inv = rsqrtf(ss * rd + a.eps);
+        const float k = inv * inv * inv * (sg * rd);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float na = ga[e] * inv, nb = gb[e] * inv;
+          da[e] = fmaf(na, xa[e], da[e]);
+          db[e] = fmaf(nb, xb[e], db[e]);
+          ga[e] = na * wa[e] - xa[e] * k;
+          gb[e] = nb * wb[e] - xb[e] * k;
+        }
+      }
+      if (live && u.on) {
+        ptx::st_v4(y + u.ea, Pack<T>::pack(ga));
+        ptx::st_v4(y + u.eb, Pack<T>::pack(gb));
+      }
+    }
+    if (!a.norm) continue;
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+#pragma unroll
+      for (int o = L; o < 32; o <<= 1) {
+        da[e] += __shfl_xor_sync(0xFFFFFFFFu, da[e], o);
+        db[e] += __shfl_xor_sync(0xFFFFFFFFu, db[e], o);
+      }
+    if (lane < L && u.on) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        dw[warp * a.d + u.ea + e] = da[e];
+        dw[warp * a.d + u.eb + e] = db[e];
+      }
+    }
+    __syncthreads();
+    for (int i = tid; i < a.d; i += kBlock) {
+      float s = 0.f;
+      for (int v = 0; v < kWarps; ++v) s += dw[v * a.d + i];
+      a.ws[((int64_t)blockIdx.x * 2 + part) * a.d + i] = s;
+    }
+    __syncthreads();
+  }
+}
+
+// Lanes of a row where the vector kernels take it, else 0 (the kernels for any row):
+// units of two whole vectors on both sides of rotary_dim, at most 32 of them, and every
+// address a multiple of 16 bytes.
+int lanes_of(int d, int r, int eb, uintptr_t addresses, int64_t strides) {
+  const int unit = 32 / eb;   // elements
+  if (d % unit || r % unit || d / unit > 32) return 0;
+  if ((addresses & 15u) || (strides * eb) % 16) return 0;
+  const int n = d / unit;
+  return n <= 4 ? 4 : n <= 8 ? 8 : n <= 16 ? 16 : 32;
+}
+uintptr_t bits_of(const void* p) { return reinterpret_cast<uintptr_t>(p); }
+
+template <typename T, bool kWrite>
+const void* forward_fn(int lanes) {
+  switch (lanes) {
+    case 4:
+      return reinterpret_cast<const void*>(qk_rope_kernel<T, 4, kWrite>);
+    case 8:
+      return reinterpret_cast<const void*>(qk_rope_kernel<T, 8, kWrite>);
+    case 16:
+      return reinterpret_cast<const void*>(qk_rope_kernel<T, 16, kWrite>);
+    case 32:
+      return reinterpret_cast<const void*>(qk_rope_kernel<T, 32, kWrite>);
+    default:
+      return reinterpret_cast<const void*>(qk_rope_any_kernel<T, kWrite>);
+  }
+}
+template <typename T>
+const void* backward_fn(int lanes) {
+  switch (lanes) {
+    case 4:
+      return reinterpret_cast<const void*>(qk_rope_backward_kernel<T, 4>);
+    case 8:
+      return reinterpret_cast<const void*>(qk_rope_backward_kernel<T, 8>);
+    case 16:
+      return reinterpret_cast<const void*>(qk_rope_backward_kernel<T, 16>);
+    case 32:
+      return reinterpret_cast<const void*>(qk_rope_backward_kernel<T, 32>);
+    default:
+      return reinterpret_cast<const void*>(qk_rope_backward_any_kernel<T>);
   }
 }
 
@@ -361,14 +736,25 @@ int run_forward(const char* who, const rmsnorm_qk_rope_args* in, void* stream) {
   OnDevice on(in->device);
   if (on.err != cudaSuccess) return launch_failed(on.err, who);
   const int64_t rows = a.tokens * (a.hq + a.hk * (kWrite ? 2 : 1));
-  const void* fn = in->dtype == RMSNORM_TP_F32
-                       ? reinterpret_cast<const void*>(qk_rope_any_kernel<float, kWrite>)
-                   : in->dtype == RMSNORM_TP_BF16
-                       ? reinterpret_cast<const void*>(qk_rope_any_kernel<__nv_bfloat16, kWrite>)
-                       : reinterpret_cast<const void*>(qk_rope_any_kernel<__half, kWrite>);
-  void* args[] = {&a};
-  const cudaError_t e = launch_dependent(fn, dim3((unsigned)((rows + kWarps - 1) / kWarps)), dim3(kBlock),
-                                         0, args, reinterpret_cast<cudaStream_t>(stream));
+  uintptr_t bits = bits_of(a.q.p) | bits_of(a.k.p) | bits_of(a.v.p) | bits_of(a.qo.p) | bits_of(a.ko.p) |
+                   bits_of(a.qw) | bits_of(a.kw) | bits_of(a.rope);
+  int64_t strides = a.q.st | a.q.sh | a.k.st | a.k.sh | a.v.st | a.v.sh | a.qo.st | a.qo.sh | a.ko.st | a.ko.sh;
+  const int lanes = lanes_of(a.d, a.r, elem_bytes(in->dtype), bits, strides);
+  const void* fn = in->dtype == RMSNORM_TP_F32    ? forward_fn<float, kWrite>(lanes)
+                   : in->dtype == RMSNORM_TP_BF16 ? forward_fn<__nv_bfloat16, kWrite>(lanes)
+                                                  : forward_fn<__half, kWrite>(lanes);
+  // groups of rows for each warp: as many as leave every SM 32 warps, at most 8
+  const int64_t groups = lanes ? (rows * lanes + 31) / 32 : rows;
+  int run = 1;
+  if (lanes) {
+    const int64_t full = 32ll * sm_count(in->device);
+    run = (int)(groups / (full > 0 ? full : 1));
+    run = run < 1 ? 1 : run > 8 ? 8 : run;
+  }
+  const int64_t blocks = (groups + (int64_t)run * kWarps - 1) / ((int64_t)run * kWarps);
+  void* args[] = {&a, &run};
+  const cudaError_t e = launch_dependent(fn, dim3((unsigned)blocks), dim3(kBlock), 0, args,
+                                         reinterpret_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? RMSNORM_TP_OK : launch_failed(e, who);
 }
 
@@ -455,13 +841,17 @@ int rmsnorm_qk_rope_backward(const rmsnorm_qk_rope_backward_args* in, void* stre
     a.interleaved = in->interleaved != 0;
     a.norm = norm;
     a.eps = in->eps;
-    const int64_t want = (a.tokens * a.hq + kWarps - 1) / kWarps;
+    const uintptr_t bits = bits_of(a.dqo.p) | bits_of(a.dko.p) | (norm ? bits_of(a.q.p) | bits_of(a.k.p) : 0) |
+                           bits_of(a.dq) | bits_of(a.dk) | bits_of(a.qw) | bits_of(a.kw) | bits_of(a.rope);
+    const int64_t strides = a.dqo.st | a.dqo.sh | a.dko.st | a.dko.sh |
+                            (norm ? a.q.st | a.q.sh | a.k.st | a.k.sh : 0);
+    const int lanes = lanes_of(a.d, a.r, eb, bits, strides);
+    const int64_t groups = lanes ? (a.tokens * a.hq * lanes + 31) / 32 : a.tokens * a.hq;
+    const int64_t want = (groups + kWarps - 1) / kWarps;
     grid = (int)(want < kBackwardMaxGrid ? want : kBackwardMaxGrid);
-    const void* fn = in->dtype == RMSNORM_TP_F32
-                         ? reinterpret_cast<const void*>(qk_rope_backward_any_kernel<float>)
-                     : in->dtype == RMSNORM_TP_BF16
-                         ? reinterpret_cast<const void*>(qk_rope_backward_any_kernel<__nv_bfloat16>)
-                         : reinterpret_cast<const void*>(qk_rope_backward_any_kernel<__half>);
+    const void* fn = in->dtype == RMSNORM_TP_F32    ? backward_fn<float>(lanes)
+                     : in->dtype == RMSNORM_TP_BF16 ? backward_fn<__nv_bfloat16>(lanes)
+                                                    : backward_fn<__half>(lanes);
     void* args[] = {&a};
     const size_t smem = norm ? (size_t)kWarps * a.d * sizeof(float) : 0;
     const cudaError_t e = launch_dependent(fn, dim3((unsigned)grid), dim3(kBlock), smem, args, st);
