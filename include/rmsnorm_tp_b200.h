@@ -349,7 +349,7 @@ int rmsnorm_kv_read(const rmsnorm_kv_cache* cache, void* k_out, void* v_out, con
  * h' = h / (q_heads / kv_heads); token j of sequence b lies in page
  * page_table[b][j / page_size]. A length is cut to max_pages * page_size; tokens
  * in a page outside [0, num_pages) are left out; a sequence with no tokens gives
- * zeros and lse = -inf. lse (optional): the natural logarithm of the sum of the
+ * zeros and lse = -inf; max_pages * page_size is at most 2^31 - 128. lse (optional): the natural logarithm of the sum of the
  * exponentials. Scores, softmax and sums in fp32. The work is divided over the
  * cached length as the lengths on the device say. q and the cache of one dtype,
  * or an e4m3 cache. workspace: rmsnorm_paged_attention_workspace_bytes(args)

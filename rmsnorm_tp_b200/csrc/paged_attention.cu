@@ -25,12 +25,14 @@ struct AttnArgs {
   float* part;          // per (sequence, head, split): m, l, o[d]
   int64_t qst, qsh, table_stride, num_pages, max_tokens, batch;
   int hq, hk, page, d, splits;
-  int row_groups;       // groups of 16 query heads that share a kv head
+  int row_groups;       // groups of 8 (16) query heads that share a kv head
   int segments;         // kv heads * row_groups
   int q_pairs;          // the queries' elements can be read two at a time
+  int whole_pages;      // pages of 16 k tokens
   float scale_log2;     // scale * log2(e): scores in base 2
 };
 
+constexpr int64_t kMostTokens = (int64_t(1) << 31) - 128;   // a tile's last token is an int
 constexpr float kLn2 = 0.69314718055994531f;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -149,30 +151,38 @@ __global__ void __launch_bounds__(kAnyBlock) attention_join_any_kernel(const __g
 // ---- tensor cores: 16-bit queries, head_dim 64, 96, 128, 192 or 256 ----------------
 //
 // The bound is HBM: a token's K and V rows are read once for its whole group of query
-// heads, and the products need (at 16 padded heads) 4 * 16 * head_dim flops for them, a
-// tenth of what warp-level mma.sync gives at that rate of bytes; tcgen05's 128-row tiles
-// would be 1/16 used at a group of 8. A CTA of 4 warps takes tiles of 64 tokens, 16 for
-// each warp, which runs its own softmax and its own cp.async ring (no CTA barrier in
-// the loop; the loads run ahead over the borders of sequences), and the warps' results
-// are joined at a sequence's end.
+// heads. The products are K Q^T and V^T P with the tokens (then the elements) as the 16
+// rows of mma.sync and 8 query heads as its columns, so a group of up to 8 pads nothing
+// but itself; tcgen05's 128-row tiles would be 1/16 used, and warp-level mma.sync gives
+// ten times the rate that the bytes ask for. A CTA of 4 warps takes tiles of 64 tokens,
+// 16 for each warp, which runs its own softmax and its own cp.async ring (no CTA barrier
+// in the loop; the loads run ahead over the borders of sequences); the warps' results are
+// joined at a sequence's end.
 //
-// All (sequence, kv head, 16 query heads) are laid behind one another in tiles, and each
-// CTA takes an equal run of tiles, from the lengths on the device: ragged batches
+// All (sequence, kv head, 8 or 16 query heads) are laid behind one another in tiles, and
+// each CTA takes an equal run of tiles, from the lengths on the device: ragged batches
 // balance to a tile and nothing on the host knows a length. A run that ends inside a
-// sequence leaves m, l and o in the workspace (at most two for each CTA), and the join
-// kernel adds them in CTA order.
+// sequence leaves its reference, sum and o in the workspace (at most two such parts for
+// each CTA), and the join kernel adds them in CTA order.
+//
+// The softmax's reference is a score seen, not the maximum: it moves only when a score
+// passes it by more than 2^8, so most tiles need no maximum over the warp and no
+// rescaling; exponentials are then at most 2^8.
 constexpr int kWarps = 4;
 constexpr int kBlock = 32 * kWarps;
 constexpr int kTile = 16 * kWarps;      // tokens of a CTA's tile
-constexpr int kRows = 16;               // query heads of a tile
+constexpr float kSlack = 8.f;           // log2 of the largest exponential
 
-struct alignas(16) Meta {               // what a CTA's last segment leaves to the join
-  int32_t open, b, hs, last;            // open: it goes on in the CTAs up to `last`
+// A segment (query heads of one kv head of one sequence) whose tiles several CTAs have:
+// `owner` to `last`; owner < 0: none.
+struct alignas(16) Seg {
+  int32_t b, hs, owner, last;
 };
 
-template <int D, bool kE4M3>
+template <int D, bool kE4M3, int NG>
 struct Shape {
-  static constexpr int kChunks = D * (kE4M3 ? 1 : 2) / 16;   // 16-byte chunks of a row
+  static constexpr int kRowBytes = D * (kE4M3 ? 1 : 2);
+  static constexpr int kChunks = kRowBytes / 16;             // 16-byte chunks of a row
   // rows of 8 k chunks are swizzled (chunk ^ (row & 7)), others padded to an odd number:
   // either way 8 rows of one chunk fall into 8 different bank groups
   static constexpr bool kSwizzle = kChunks % 8 == 0;
@@ -180,7 +190,11 @@ struct Shape {
   static constexpr int kOperand = 16 * kPitch;               // one warp's K (or V) tile
   static constexpr int kSide = kE4M3 ? 128 + 16 : 16;        // its scales and its mask
   static constexpr int kStage = 2 * kOperand + kSide;
-  static constexpr int kJoin = kWarps * 8 * (D / 2 + 8) * 4;
+  // lanes that load one row, and rows of one load instruction
+  static constexpr int kLanes = kChunks % 8 == 0 ? 8 : kChunks % 4 == 0 ? 4 : 2;
+  static constexpr int kRowsAtOnce = 32 / kLanes;
+  static constexpr int kJoinPitch = D / 2 + 4;
+  static constexpr int kJoin = kWarps * 8 * kJoinPitch * 4;
   // two CTAs of at most 110 KB on an SM where at least three stages fit, else one
   static constexpr int kTwo = (110 * 1024 - kJoin) / (kWarps * kStage);
   static constexpr int kOne = (220 * 1024 - kJoin) / (kWarps * kStage);
@@ -210,6 +224,12 @@ __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
 __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t a) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+// 8 x 8 matrix of 16-bit elements transposed over the warp.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 template <bool kBf16>
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -262,21 +282,23 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
   unpack2<kBf16>(hi, hx, hy);
   lo = pack2<kBf16>(fmaxf(x - hx, kLeast), fmaxf(y - hy, kLeast));
 }
-__device__ __forceinline__ float quad_max(float v) {
-  v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 1));
-  return fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, 2));
+// Over the lanes that hold one head (lane / 4 differs).
+__device__ __forceinline__ float head_max(float v) {
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+  return v;
 }
-__device__ __forceinline__ float quad_sum(float v) {
-  v += __shfl_xor_sync(0xFFFFFFFFu, v, 1);
-  return v + __shfl_xor_sync(0xFFFFFFFFu, v, 2);
+__device__ __forceinline__ float head_sum(float v) {
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+  return v;
 }
 // The reference of exponentials: 0 where nothing has been seen (their value is 0 then).
 __device__ __forceinline__ float ref_of(float m) { return m == -INFINITY ? 0.f : m; }
 
 // Place in the row of tiles: tile `tile` of the `tiles` of segment (b, hs).
 struct Place {
-  int b, hs, tile, tiles;
-  int64_t len;
+  int b, hs, tile, tiles, len;
 };
 
 __device__ __forceinline__ int tiles_of(int64_t len) { return (int)((len + kTile - 1) / kTile); }
@@ -289,25 +311,26 @@ __device__ __forceinline__ void advance(const AttnArgs& a, Place& p) {
   p.hs = 0;
   do {
     ++p.b;
-    p.len = length_of(a, p.b);
+    p.len = (int)length_of(a, p.b);
   } while (p.len == 0);
   p.tiles = tiles_of(p.len);
 }
 
-template <typename TQ, bool kE4M3, int D>
-__global__ void __launch_bounds__(kBlock, Shape<D, kE4M3>::kCtas)
+// NG: groups of 8 query heads that one CTA holds.
+template <typename TQ, bool kE4M3, int D, int NG>
+__global__ void __launch_bounds__(kBlock, Shape<D, kE4M3, NG>::kCtas)
 attention_kernel(const __grid_constant__ AttnArgs a) {
-  using S = Shape<D, kE4M3>;
-  constexpr bool kBf16 = !kE4M3 && sizeof(TQ) == 2 && !__is_same(TQ, __half);   // of the products
+  using S = Shape<D, kE4M3, NG>;
+  constexpr bool kQBf16 = __is_same(TQ, __nv_bfloat16);
+  constexpr bool kBf16 = !kE4M3 && kQBf16;   // of the products: e4m3 codes become fp16
   // the numerators as two 16-bit parts where their rounding to one would be of the output's
   // own size; one fp16 part (2^-11) beside a bf16 output (2^-8)
-  constexpr bool kTwoParts = !kE4M3 || __is_same(TQ, __half);
-  // fp16 numerators run up to 2^15 instead of 1, so that fp16's smallest number, 2^-24, is
-  // 2^-39 of the largest
-  constexpr float kLift = kBf16 || kE4M3 ? 1.f : 32768.f;
-  constexpr float kLiftLog2 = kBf16 || kE4M3 ? 0.f : 15.f;
-  constexpr int kEb = kE4M3 ? 1 : 2;
-  constexpr int NT = D / 8, KS = D / 16;
+  constexpr bool kTwoParts = !kE4M3 || !kQBf16;
+  // fp16 numerators run up to 2^15, so that fp16's smallest number is 2^-39 of the largest
+  constexpr float kLiftLog2 = kBf16 || kE4M3 ? 0.f : 15.f - kSlack;
+  constexpr float kLift = kBf16 || kE4M3 ? 1.f : 128.f;
+  constexpr int KS = D / 16;
+  constexpr int kRows = 8 * NG;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows], s_v[kWarps][kRows];
   __shared__ int64_t s_scan[kWarps];
@@ -338,12 +361,12 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
   }
   const int64_t workers = total < gridDim.x ? total : gridDim.x;
   const int64_t me = blockIdx.x;
-  Meta* meta = reinterpret_cast<Meta*>(a.part);
-  if (me >= workers) {
-    if (tid == 0) meta[me] = Meta{0, 0, 0, 0};
-    return;
-  }
+  Seg* meta = reinterpret_cast<Seg*>(a.part) + 2 * me;   // the segment that began before, and one left open
+  if (tid < 2) meta[tid] = Seg{0, 0, -1, -1};
+  if (me >= workers) return;
   const int64_t t0 = total * me / workers, t1 = total * (me + 1) / workers;
+  // the CTA that has a tile of the row
+  auto worker_of = [&](int64_t tile) { return (int)(((tile + 1) * workers - 1) / total); };
   if (upto - mine <= t0 && t0 < upto) {
     int64_t rest = t0 - (upto - mine);
     int64_t b = tid * per;
@@ -358,52 +381,68 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
   __syncthreads();
   Place at;
   at.b = s_b;
-  at.len = length_of(a, at.b);
+  at.len = (int)length_of(a, at.b);
   at.tiles = tiles_of(at.len);
   at.hs = (int)(s_rest / at.tiles);
   at.tile = (int)(s_rest - (int64_t)at.hs * at.tiles);
   const int n = (int)(t1 - t0);
+  if (tid == 0 && at.tile > 0)
+    meta[0] = Seg{at.b, at.hs, worker_of(t0 - at.tile), worker_of(t0 - at.tile + at.tiles - 1)};
 
   float* join = reinterpret_cast<float*>(smem);
-  const uint32_t ring = ptx::smem_addr(smem) + S::kJoin + warp * S::kStages * S::kStage;
   unsigned char* ring_p = smem + S::kJoin + warp * S::kStages * S::kStage;
+  const uint32_t ring = ptx::smem_addr(ring_p);
 
-  // ---- loads: lane l < 16 knows the row of token l of the warp's next tile ----
+  // ---- loads ----
+  const int lr = lane / S::kLanes, lc = lane % S::kLanes;
+  const unsigned char* kp = static_cast<const unsigned char*>(a.k) + lc * 16;
+  const unsigned char* vp = static_cast<const unsigned char*>(a.v) + lc * 16;
+  const uint32_t side_off = 2 * S::kOperand;
   Place ahead = at;
-  int sent = 0;
-  int32_t page_id = -1;               // of this lane's token, read one tile early
+  int sent = 0, into = 0;
+  int32_t page_id = -1;               // read one tile early
+  // pages of 16 k tokens: the warp's 16 tokens lie in one page, one row behind another;
+  // else lane l (and l + 16) knows the row of token l
   auto look_up = [&]() {
-    const int64_t t = (int64_t)ahead.tile * kTile + warp * 16 + (lane & 15);
+    const int t = ahead.tile * kTile + warp * 16 + (a.whole_pages ? 0 : lane & 15);
     page_id = t < ahead.len ? a.table[ahead.b * a.table_stride + (unsigned)t / (unsigned)a.page] : -1;
   };
   look_up();
   auto send = [&]() {
     if (sent < n) {
-      const int stage = sent % S::kStages;
-      const uint32_t dst = ring + stage * S::kStage;
-      const int64_t t = (int64_t)ahead.tile * kTile + warp * 16 + (lane & 15);
-      const bool live = page_id >= 0 && page_id < a.num_pages;
-      const unsigned mask = __ballot_sync(0xFFFFFFFFu, live) & 0xFFFFu;
+      const uint32_t dst = ring + into * S::kStage;
+      const int t = ahead.tile * kTile + warp * 16 + (a.whole_pages ? 0 : lane & 15);
       const int kvh = ahead.hs / a.row_groups;
+      const bool live = page_id >= 0 && page_id < a.num_pages;
       const int64_t row = live ? ((int64_t)page_id * a.hk + kvh) * a.page + (unsigned)t % (unsigned)a.page : 0;
-      if (lane == 0)
-        *reinterpret_cast<unsigned*>(ring_p + stage * S::kStage + 2 * S::kOperand + (kE4M3 ? 128 : 0)) = mask;
-      if constexpr (kE4M3)            // lanes 0-15 K's scales, 16-31 V's
-        cp_async4(dst + 2 * S::kOperand + lane * 4, (lane < 16 ? a.ks : a.vs) + row, live);
-      const unsigned char* kp = static_cast<const unsigned char*>(a.k);
-      const unsigned char* vp = static_cast<const unsigned char*>(a.v);
+      unsigned mask;
+      if (a.whole_pages) {
+        const int left = ahead.len - t;
+        mask = !live ? 0u : left >= 16 ? 0xFFFFu : (1u << left) - 1u;
+      } else {
+        mask = __ballot_sync(0xFFFFFFFFu, live) & 0xFFFFu;
+      }
+      if constexpr (kE4M3) {          // lanes 0-15 K's scales, 16-31 V's
+        const int64_t r = a.whole_pages ? row + (lane & 15) : row;
+        const bool on = (mask >> (lane & 15)) & 1u;
+        cp_async4(dst + side_off + lane * 4, (lane < 16 ? a.ks : a.vs) + (on ? r : 0), on);
+      }
 #pragma unroll
-      for (int i = 0; i < (16 * S::kChunks + 31) / 32; ++i) {
-        const int u = i * 32 + lane;
-        const int r = u / S::kChunks, c = u - r * S::kChunks;
-        const int64_t from = __shfl_sync(0xFFFFFFFFu, row, r & 15) * (D * kEb) + c * 16;
-        const bool on = (mask >> (r & 15)) & 1u;
-        if (16 * S::kChunks % 32 == 0 || u < 16 * S::kChunks) {
-          const uint32_t to = dst + r * S::kPitch + (S::kSwizzle ? c ^ (r & 7) : c) * 16;
-          cp_async16(to, kp + from, on);
-          cp_async16(to + S::kOperand, vp + from, on);
+      for (int i = 0; i < 16 / S::kRowsAtOnce; ++i) {
+        const int r = i * S::kRowsAtOnce + lr;
+        const int64_t from = (a.whole_pages ? row + r : __shfl_sync(0xFFFFFFFFu, row, r)) * S::kRowBytes;
+        const bool on = (mask >> r) & 1u;
+        const int64_t safe = on ? from : 0;
+        const uint32_t to = dst + r * S::kPitch + (S::kSwizzle ? lc ^ (r & 7) : lc) * 16;
+#pragma unroll
+        for (int k = 0; k < S::kChunks / S::kLanes; ++k) {
+          cp_async16(to + k * S::kLanes * 16, kp + safe + k * S::kLanes * 16, on);
+          cp_async16(to + S::kOperand + k * S::kLanes * 16, vp + safe + k * S::kLanes * 16, on);
         }
       }
+      if (lane == 0)
+        *reinterpret_cast<unsigned*>(ring_p + into * S::kStage + side_off + (kE4M3 ? 128 : 0)) = mask;
+      into = into + 1 == S::kStages ? 0 : into + 1;
       if (++sent < n) {
         advance(a, ahead);
         look_up();
@@ -414,283 +453,293 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
 #pragma unroll 1
   for (int i = 0; i < S::kStages - 1; ++i) send();
 
-  uint32_t q[KS][4];
-  float o[NT][4];
-  float m[2], l[2], mv[2];            // rows g and g + 8; mv: maximum of the V-weighted scores
-  float unit[2];                      // factor of the raw scores
-  int rows = 0;
+  uint32_t q[NG][KS][2];
+  float o[NG][KS][4];                 // [16 elements][head 2 qd, 2 qd + 1] of each group of 8
+  float m[NG][2], l[NG][2], mv[NG][2];   // references of the scores and (e4m3) of the V-weighted ones
+  float unit[NG][2];                  // factor of the raw scores
+  int rows = 0, stage = 0;
 
-  const uint32_t k_lane = kE4M3 ? ((lane >> 3) & 1) * 8 + (lane & 7) : (lane >> 4) * 8 + (lane & 7);
-  const uint32_t k_chunk = kE4M3 ? lane >> 4 : (lane >> 3) & 1;
-  const uint32_t v_lane = ((lane >> 3) & 1) * 8 + (lane & 7);
-  const uint32_t v_chunk = lane >> 4;
-  const uint32_t k_row = k_lane * S::kPitch, v_row = S::kOperand + v_lane * S::kPitch;
+  // K as 16 tokens x 16 elements: matrices (tokens 0-7, 8-15) x (chunk, next chunk)
+  const uint32_t k_tok = ((lane >> 3) & 1) * 8 + (lane & 7), k_chunk = lane >> 4;
+  // V^T: 16-bit (chunk, next chunk) x (tokens 0-7, 8-15), e4m3 as K
+  const uint32_t v_tok = kE4M3 ? k_tok : (lane >> 4) * 8 + (lane & 7);
+  const uint32_t v_chunk = kE4M3 ? k_chunk : (lane >> 3) & 1;
+  const uint32_t k_row = k_tok * S::kPitch, v_row = S::kOperand + v_tok * S::kPitch;
 
-  bool fresh = true, whole = false;
+  bool fresh = true, whole = false, began = false;
 #pragma unroll 1
   for (int i = 0; i < n; ++i) {
     if (fresh) {
       fresh = false;
-      whole = at.tile == 0;
+      began = whole = at.tile == 0;
       const int group = a.hq / a.hk;
       const int kvh = at.hs / a.row_groups, first = (at.hs - kvh * a.row_groups) * kRows;
       rows = min(kRows, group - first);
-      const TQ* qg = static_cast<const TQ*>(a.q) + at.b * a.qst + (int64_t)(kvh * group + first) * a.qsh;
-      const unsigned short* qu = reinterpret_cast<const unsigned short*>(qg);
+      const unsigned short* qu = static_cast<const unsigned short*>(a.q) + at.b * a.qst +
+                                 (int64_t)(kvh * group + first) * a.qsh;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int r = g + (j & 1) * 8;
-          // e4m3: a thread's four K codes are neighbours, so its k index runs 4 qd .. 4 qd + 3
-          const int e = ks * 16 + (kE4M3 ? 4 * qd + (j >> 1) * 2 : 2 * qd + (j >> 1) * 8);
-          uint32_t v = 0;
-          if (r < rows) {
-            const unsigned short* p = qu + r * a.qsh + e;
-            v = a.q_pairs ? *reinterpret_cast<const uint32_t*>(p) : p[0] | (uint32_t)p[1] << 16;
-          }
-          q[ks][j] = v;
-        }
-      unit[0] = unit[1] = a.scale_log2;
-      if constexpr (kE4M3) {
-        // fp16 beside the fp16 that the codes become: each head scaled by a power of two so
-        // that its largest element lies in [2^14, 2^15), exact down to 2^-28 of it
-        float most[2] = {0.f, 0.f};
+      for (int x = 0; x < NG; ++x) {
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            float x, y;
-            unpack2<__is_same(TQ, __nv_bfloat16)>(q[ks][j], x, y);
-            most[j & 1] = fmaxf(most[j & 1], fmaxf(fabsf(x), fabsf(y)));
+          for (int j = 0; j < 2; ++j) {
+            const int r = 8 * x + g;
+            // e4m3: a thread's four K codes are neighbours, so its k index runs 4 qd .. 4 qd + 3
+            const int e = ks * 16 + (kE4M3 ? 4 * qd + 2 * j : 2 * qd + 8 * j);
+            uint32_t v = 0;
+            if (r < rows) {
+              const unsigned short* p = qu + r * a.qsh + e;
+              v = a.q_pairs ? *reinterpret_cast<const uint32_t*>(p) : p[0] | (uint32_t)p[1] << 16;
+            }
+            q[x][ks][j] = v;
           }
-        float up[2];
+        unit[x][0] = unit[x][1] = a.scale_log2;
+        if constexpr (kE4M3) {
+          // fp16 beside the fp16 that the codes become: each head scaled by a power of two so
+          // that its largest element lies in [2^14, 2^15), exact down to 2^-28 of it
+          float most = 0.f;
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          int e = (int)(__float_as_uint(quad_max(most[r])) >> 23);   // biased exponent
+          for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              float lo, hi;
+              unpack2<kQBf16>(q[x][ks][j], lo, hi);
+              most = fmaxf(most, fmaxf(fabsf(lo), fabsf(hi)));
+            }
+          most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
+          most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
+          int e = (int)(__float_as_uint(most) >> 23);   // biased exponent
           e = e < 40 ? 40 : e == 255 ? 141 : e;
-          up[r] = __uint_as_float((unsigned)(127 + 141 - e) << 23);
-          unit[r] *= __uint_as_float((unsigned)(127 - 141 + e) << 23);
+          const float up = __uint_as_float((unsigned)(127 + 141 - e) << 23);
+          const float down = __uint_as_float((unsigned)(127 - 141 + e) << 23);
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              float lo, hi;
+              unpack2<kQBf16>(q[x][ks][j], lo, hi);
+              q[x][ks][j] = f16x2_pack(lo * up, hi * up);
+            }
+          // lane 4 g' holds head g's factor; this lane's scores are those of heads 2 qd, 2 qd + 1
+          unit[x][0] *= __shfl_sync(0xFFFFFFFFu, down, 8 * qd);
+          unit[x][1] *= __shfl_sync(0xFFFFFFFFu, down, 8 * qd + 4);
         }
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            float x, y;
-            unpack2<__is_same(TQ, __nv_bfloat16)>(q[ks][j], x, y);
-            q[ks][j] = f16x2_pack(x * up[j & 1], y * up[j & 1]);
-          }
+        for (int j = 0; j < KS; ++j) o[x][j][0] = o[x][j][1] = o[x][j][2] = o[x][j][3] = 0.f;
+        m[x][0] = m[x][1] = mv[x][0] = mv[x][1] = -INFINITY;
+        l[x][0] = l[x][1] = 0.f;
       }
-#pragma unroll
-      for (int j = 0; j < NT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-      m[0] = m[1] = mv[0] = mv[1] = -INFINITY;
-      l[0] = l[1] = 0.f;
     }
     cp_wait<S::kStages - 2>();
     __syncwarp();
     send();                           // into the stage that every lane left in the last turn
-    const int stage = i % S::kStages;
     const uint32_t base = ring + stage * S::kStage;
-    const unsigned char* side = ring_p + stage * S::kStage + 2 * S::kOperand;
+    const unsigned char* side = ring_p + stage * S::kStage + side_off;
+    stage = stage + 1 == S::kStages ? 0 : stage + 1;
     const unsigned mask = *reinterpret_cast<const unsigned*>(side + (kE4M3 ? 128 : 0));
     if (mask != 0u) {
-      float s[2][4] = {};
+      float s[NG][4];                 // (token g, heads 2 qd, 2 qd + 1), (token g + 8, the same)
+      {
+        float s2[NG][4];              // the odd steps' sums: two chains instead of one
 #pragma unroll
-      for (int ks = 0; ks < KS; ks += kE4M3 ? 2 : 1) {
-        uint32_t r[4];
-        const uint32_t c = (kE4M3 ? ks : 2 * ks) + k_chunk;
-        ldsm4(r, base + k_row + (S::kSwizzle ? c ^ (k_lane & 7) : c) * 16);
-        if constexpr (kE4M3) {
+        for (int x = 0; x < NG; ++x)
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
+          for (int j = 0; j < 4; ++j) s[x][j] = s2[x][j] = 0.f;
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
-              mma<false>(s[t], q[ks + h], e4m3x2_f16x2(r[2 * h + t]), e4m3x2_f16x2(r[2 * h + t] >> 16));
-        } else {
-          mma<kBf16>(s[0], q[ks], r[0], r[1]);
-          mma<kBf16>(s[1], q[ks], r[2], r[3]);
-        }
-      }
-      float w[2][4];                  // numerators as V meets them
-      float grow = 0.f;               // > 0: a maximum rose
-      float top[2] = {-INFINITY, -INFINITY}, topv[2] = {-INFINITY, -INFINITY};
-      float lv[2][2];
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int tok = t * 8 + 2 * qd + j;
-          float f = 1.f;
+        for (int ks = 0; ks < KS; ks += 2) {
+          uint32_t r[4], r2[4];
           if constexpr (kE4M3) {
-            f = reinterpret_cast<const float*>(side)[tok];
-            lv[t][j] = lg2(reinterpret_cast<const float*>(side)[16 + tok]);
+            const uint32_t c = ks + k_chunk;
+            uint32_t w[4];
+            ldsm4(w, base + k_row + (S::kSwizzle ? c ^ (k_tok & 7) : c) * 16);
+            r[0] = e4m3x2_f16x2(w[0]), r[2] = e4m3x2_f16x2(w[0] >> 16);
+            r[1] = e4m3x2_f16x2(w[1]), r[3] = e4m3x2_f16x2(w[1] >> 16);
+            r2[0] = e4m3x2_f16x2(w[2]), r2[2] = e4m3x2_f16x2(w[2] >> 16);
+            r2[1] = e4m3x2_f16x2(w[3]), r2[3] = e4m3x2_f16x2(w[3] >> 16);
+          } else {
+            const uint32_t c = 2 * ks + k_chunk;
+            ldsm4(r, base + k_row + (S::kSwizzle ? c ^ (k_tok & 7) : c) * 16);
+            ldsm4(r2, base + k_row + (S::kSwizzle ? (c + 2) ^ (k_tok & 7) : c + 2) * 16);
           }
-          const bool on = (mask >> tok) & 1u;
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            float& x = s[t][2 * r + j];
-            x = on ? x * (kE4M3 ? unit[r] * f : unit[r]) : -INFINITY;
-            top[r] = fmaxf(top[r], x);
-            if constexpr (kE4M3) topv[r] = fmaxf(topv[r], on ? x + lv[t][j] : -INFINITY);
+          for (int x = 0; x < NG; ++x) {
+            mma<kBf16>(s[x], r, q[x][ks][0], q[x][ks][1]);
+            mma<kBf16>(s2[x], r2, q[x][ks + 1][0], q[x][ks + 1][1]);
           }
         }
-      float ref[2], refv[2], keep[2];
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float now = fmaxf(m[r], quad_max(top[r]));
-        ref[r] = ref_of(now);
-        const float fade = ex2(m[r] - ref[r]);
-        if (now > m[r]) grow = 1.f;
-        m[r] = now;
-        l[r] *= fade;
-        keep[r] = fade;
-        if constexpr (kE4M3) {
-          const float nowv = fmaxf(mv[r], quad_max(topv[r]));
-          refv[r] = ref_of(nowv);
-          keep[r] = ex2(mv[r] - refv[r]);
-          if (nowv > mv[r]) grow = 1.f;
-          mv[r] = nowv;
+        for (int x = 0; x < NG; ++x)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) s[x][j] += s2[x][j];
+      }
+      const bool on[2] = {(bool)((mask >> g) & 1u), (bool)((mask >> (g + 8)) & 1u)};
+      float ksc[2] = {1.f, 1.f}, lv[2] = {0.f, 0.f};
+      if constexpr (kE4M3) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          ksc[t] = reinterpret_cast<const float*>(side)[8 * t + g];
+          lv[t] = lg2(reinterpret_cast<const float*>(side)[16 + 8 * t + g]);
         }
       }
+      bool rise = false;
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int x = 0; x < NG; ++x)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            const float x = s[t][2 * r + j];
-            const float p = ex2(x - ref[r]);
-            l[r] += p;
-            if constexpr (kE4M3) {
-              const bool on = (mask >> (t * 8 + 2 * qd + j)) & 1u;
-              w[t][2 * r + j] = on ? ex2(x + lv[t][j] - refv[r]) : 0.f;
-            } else {
-              w[t][2 * r + j] = p * kLift;
-            }
-          }
-      if (__any_sync(0xFFFFFFFFu, grow > 0.f)) {
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          o[j][0] *= keep[0];
-          o[j][1] *= keep[0];
-          o[j][2] *= keep[1];
-          o[j][3] *= keep[1];
+        for (int j = 0; j < 4; ++j) {
+          const int t = j >> 1, h = j & 1;
+          s[x][j] = on[t] ? s[x][j] * (kE4M3 ? unit[x][h] * ksc[t] : unit[x][h]) : -INFINITY;
+          rise |= s[x][j] > m[x][h] + kSlack;
+          if constexpr (kE4M3) rise |= on[t] && s[x][j] + lv[t] > mv[x][h] + kSlack;
         }
-      }
-      uint32_t hi[4], lo[4];
+      if (__any_sync(0xFFFFFFFFu, rise)) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float x = w[j >> 1][(j & 1) * 2], y = w[j >> 1][(j & 1) * 2 + 1];
-        if constexpr (kTwoParts) split2<kBf16>(x, y, hi[j], lo[j]);
-        else hi[j] = pack2<kBf16>(x, y);
-      }
-#pragma unroll
-      for (int j = 0; j < NT / 2; j += kE4M3 ? 2 : 1) {
-        uint32_t r[4];
-        const uint32_t c = (kE4M3 ? j : 2 * j) + v_chunk;
-        ldsm4t(r, base + v_row + (S::kSwizzle ? c ^ (v_lane & 7) : c) * 16);
-        if constexpr (kE4M3) {
-          // r[2 h], r[2 h + 1]: tokens 0-7 and 8-15 of chunk j + h; its bytes are
-          // (token 2 qd: elements 2 g, 2 g + 1), (token 2 qd + 1: the same)
+        for (int x = 0; x < NG; ++x)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const uint32_t x = __byte_perm(r[2 * h], 0, 0x3120), y = __byte_perm(r[2 * h + 1], 0, 0x3120);
-            float (&even)[4] = o[2 * (j + h)];
-            float (&odd)[4] = o[2 * (j + h) + 1];
-            const uint32_t e0 = e4m3x2_f16x2(x), e1 = e4m3x2_f16x2(y);
-            const uint32_t d0 = e4m3x2_f16x2(x >> 16), d1 = e4m3x2_f16x2(y >> 16);
-            mma<false>(even, hi, e0, e1);
-            mma<false>(odd, hi, d0, d1);
-            if constexpr (kTwoParts) {
-              mma<false>(even, lo, e0, e1);
-              mma<false>(odd, lo, d0, d1);
+            const float now = fmaxf(m[x][h], head_max(fmaxf(s[x][h], s[x][2 + h])));
+            float keep = ex2(m[x][h] - ref_of(now));
+            l[x][h] *= keep;
+            m[x][h] = now;
+            if constexpr (kE4M3) {
+              const float nowv = fmaxf(mv[x][h], head_max(fmaxf(on[0] ? s[x][h] + lv[0] : -INFINITY,
+                                                               on[1] ? s[x][2 + h] + lv[1] : -INFINITY)));
+              keep = ex2(mv[x][h] - ref_of(nowv));
+              mv[x][h] = nowv;
+            }
+#pragma unroll
+            for (int j = 0; j < KS; ++j) {
+              o[x][j][h] *= keep;
+              o[x][j][2 + h] *= keep;
             }
           }
+      }
+      uint32_t hi[NG][2], lo[NG][2];  // P as 16 tokens x 8 heads
+#pragma unroll
+      for (int x = 0; x < NG; ++x) {
+        const float ref[2] = {ref_of(m[x][0]), ref_of(m[x][1])};
+        const float refv[2] = {ref_of(mv[x][0]), ref_of(mv[x][1])};
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          float w[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float v = s[x][2 * t + h], p = ex2(v - ref[h]);
+            l[x][h] += p;
+            w[h] = kE4M3 ? (on[t] ? ex2(v + lv[t] - refv[h]) : 0.f) : p * kLift;
+          }
+          if constexpr (kTwoParts) {
+            split2<kBf16>(w[0], w[1], hi[x][t], lo[x][t]);
+            lo[x][t] = transposed(lo[x][t]);
+          } else {
+            hi[x][t] = pack2<kBf16>(w[0], w[1]);
+          }
+          hi[x][t] = transposed(hi[x][t]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < KS; j += kE4M3 ? 2 : 1) {
+        uint32_t r[4], r2[4];
+        const uint32_t c = (kE4M3 ? j : 2 * j) + v_chunk;
+        const uint32_t from = base + v_row + (S::kSwizzle ? c ^ (v_tok & 7) : c) * 16;
+        if constexpr (kE4M3) {
+          // bytes of w: (token 2 qd: elements 2 g, 2 g + 1), (token 2 qd + 1: the same), so row g
+          // of the product is element 2 g and row g + 8 element 2 g + 1
+          uint32_t w[4];
+          ldsm4t(w, from);
+#pragma unroll
+          for (int t = 0; t < 4; ++t) w[t] = __byte_perm(w[t], 0, 0x3120);
+          r[0] = e4m3x2_f16x2(w[0]), r[1] = e4m3x2_f16x2(w[0] >> 16);
+          r[2] = e4m3x2_f16x2(w[1]), r[3] = e4m3x2_f16x2(w[1] >> 16);
+          r2[0] = e4m3x2_f16x2(w[2]), r2[1] = e4m3x2_f16x2(w[2] >> 16);
+          r2[2] = e4m3x2_f16x2(w[3]), r2[3] = e4m3x2_f16x2(w[3] >> 16);
         } else {
-          mma<kBf16>(o[2 * j], hi, r[0], r[1]);
-          mma<kBf16>(o[2 * j + 1], hi, r[2], r[3]);
-          mma<kBf16>(o[2 * j], lo, r[0], r[1]);
-          mma<kBf16>(o[2 * j + 1], lo, r[2], r[3]);
+          ldsm4t(r, from);
+        }
+#pragma unroll
+        for (int x = 0; x < NG; ++x) {
+          mma<kBf16>(o[x][j], r, hi[x][0], hi[x][1]);
+          if constexpr (kTwoParts) mma<kBf16>(o[x][j], r, lo[x][0], lo[x][1]);
+          if constexpr (kE4M3) {
+            mma<kBf16>(o[x][j + 1], r2, hi[x][0], hi[x][1]);
+            if constexpr (kTwoParts) mma<kBf16>(o[x][j + 1], r2, lo[x][0], lo[x][1]);
+          }
         }
       }
     }
 
     const bool last = at.tile + 1 == at.tiles;
     if (last || i + 1 == n) {
-      // ---- the warps' results of the segment, joined: half a head's elements of 8 rows at a time
-      if constexpr (!kE4M3) {
-        mv[0] = m[0] - kLiftLog2;
-        mv[1] = m[1] - kLiftLog2;
-      }
+      // ---- the warps' results of the segment, joined: half of 8 heads' elements at a time
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float sum = quad_sum(l[r]);
-        if (qd == 0) {
-          s_m[warp][g + 8 * r] = m[r];
-          s_v[warp][g + 8 * r] = mv[r];
-          s_l[warp][g + 8 * r] = sum;
+      for (int x = 0; x < NG; ++x)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float sum = head_sum(l[x][h]);
+          if (g == 0) {
+            s_m[warp][8 * x + 2 * qd + h] = m[x][h];
+            s_v[warp][8 * x + 2 * qd + h] = kE4M3 ? mv[x][h] : m[x][h] - kLiftLog2;
+            s_l[warp][8 * x + 2 * qd + h] = sum;
+          }
         }
-      }
       whole = whole && last;
       const int kvh = at.hs / a.row_groups, first = (at.hs - kvh * a.row_groups) * kRows;
       const int64_t out_row = (int64_t)at.b * a.hq + kvh * (a.hq / a.hk) + first;
-      // the slot of a segment that began here, or of one that began before
-      const bool began = i + 1 - (at.tile + 1) >= 0;
+      // the part of a segment that began before, or of one left open
       const int64_t slot = 2 * me + (began ? 1 : 0);
-      float* pm = reinterpret_cast<float*>(meta + gridDim.x) + slot * kRows * 2;
-      float* po = reinterpret_cast<float*>(meta + gridDim.x) + 2ll * gridDim.x * kRows * 2 + slot * kRows * D;
-      if (i + 1 == n && tid == 0) {
-        // tile of the whole row where the segment ends -> the CTA that has it
-        const int64_t end = t1 + (at.tiles - at.tile - 1) - 1;
-        const bool open = began && !last;
-        meta[me] = Meta{open ? 1 : 0, at.b, at.hs, open ? (int)(((end + 1) * workers - 1) / total) : 0};
-      }
-      constexpr int kHalf = D / 2, kStride = kHalf + 8;
-      for (int rh = 0; rh * 8 < rows; ++rh)
+      float* pm = reinterpret_cast<float*>(reinterpret_cast<Seg*>(a.part) + 2 * gridDim.x) + slot * kRows * 2;
+      float* po = reinterpret_cast<float*>(reinterpret_cast<Seg*>(a.part) + 2 * gridDim.x) +
+                  2ll * gridDim.x * kRows * 2 + slot * kRows * D;
+      if (tid == 0 && began && !last)
+        meta[1] = Seg{at.b, at.hs, (int)me, worker_of(t1 - 1 + (at.tiles - 1 - at.tile))};
+      constexpr int kHalf = D / 2;
+#pragma unroll
+      for (int x = 0; x < NG; ++x) {
+        if (8 * x >= rows) break;
 #pragma unroll
         for (int dh = 0; dh < 2; ++dh) {
-          float* to = join + (warp * 8 + g) * kStride;
+          float* to = join + (warp * 8 + 2 * qd) * S::kJoinPitch;
 #pragma unroll
-          for (int j = 0; j < NT / 2; j += kE4M3 ? 2 : 1) {
-            const int k = dh * (NT / 2) + j;
-            const float x0 = rh ? o[k][2] : o[k][0], x1 = rh ? o[k][3] : o[k][1];
-            if constexpr (kE4M3) {
-              const float y0 = rh ? o[k + 1][2] : o[k + 1][0], y1 = rh ? o[k + 1][3] : o[k + 1][1];
-              *reinterpret_cast<float4*>(to + j * 8 + 4 * qd) = make_float4(x0, y0, x1, y1);
-            } else {
-              *reinterpret_cast<float2*>(to + j * 8 + 2 * qd) = make_float2(x0, x1);
+          for (int j = 0; j < KS / 2; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float (&v)[4] = o[x][dh * (KS / 2) + j];
+              float* p = to + h * S::kJoinPitch + 16 * j;
+              if constexpr (kE4M3) {
+                *reinterpret_cast<float2*>(p + 2 * g) = make_float2(v[h], v[2 + h]);
+              } else {
+                p[g] = v[h];
+                p[g + 8] = v[2 + h];
+              }
             }
-          }
           __syncthreads();
           for (int u = tid; u < 8 * (kHalf / 4); u += kBlock) {
-            const int r8 = u / (kHalf / 4), e = (u - r8 * (kHalf / 4)) * 4, r = rh * 8 + r8;
+            const int r8 = u / (kHalf / 4), e = (u - r8 * (kHalf / 4)) * 4, r = 8 * x + r8;
             if (r >= rows) continue;
             float mm = -INFINITY, ll = 0.f;
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, s_m[w][r]);
-            const float base2 = ref_of(mm);
-            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+            const float ref = ref_of(mm);
+            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
-              ll += s_l[w][r] * ex2(s_m[w][r] - base2);
-              const float f = s_v[w][r] == -INFINITY ? 0.f : ex2(s_v[w][r] - base2);
-              const float4 y = *reinterpret_cast<const float4*>(join + (w * 8 + r8) * kStride + e);
-              x.x = fmaf(f, y.x, x.x);
-              x.y = fmaf(f, y.y, x.y);
-              x.z = fmaf(f, y.z, x.z);
-              x.w = fmaf(f, y.w, x.w);
+              ll += s_l[w][r] * ex2(s_m[w][r] - ref);
+              const float f = s_v[w][r] == -INFINITY ? 0.f : ex2(s_v[w][r] - ref);
+              const float4 z = *reinterpret_cast<const float4*>(join + (w * 8 + r8) * S::kJoinPitch + e);
+              y.x = fmaf(f, z.x, y.x);
+              y.y = fmaf(f, z.y, y.y);
+              y.z = fmaf(f, z.z, y.z);
+              y.w = fmaf(f, z.w, y.w);
             }
             const int at_e = dh * kHalf + e;
             if (whole) {
-              if (ll == 0.f) x = make_float4(0.f, 0.f, 0.f, 0.f);
-              const float d = ll == 0.f ? 1.f : ll;
-              uint2 y;
-              y.x = pack2<__is_same(TQ, __nv_bfloat16)>(x.x / d, x.y / d);
-              y.y = pack2<__is_same(TQ, __nv_bfloat16)>(x.z / d, x.w / d);
-              *reinterpret_cast<uint2*>(static_cast<TQ*>(a.out) + (out_row + r) * D + at_e) = y;
-              if (a.lse && at_e == 0) a.lse[out_row + r] = kLn2 * (base2 + log2f(ll));
+              const float d = ll == 0.f ? 1.f : ll;   // no weight at all: o is 0
+              uint2 out;
+              out.x = pack2<kQBf16>(y.x / d, y.y / d);
+              out.y = pack2<kQBf16>(y.z / d, y.w / d);
+              *reinterpret_cast<uint2*>(static_cast<TQ*>(a.out) + (out_row + r) * D + at_e) = out;
+              if (a.lse && at_e == 0) a.lse[out_row + r] = kLn2 * (ref + log2f(ll));
             } else {
-              *reinterpret_cast<float4*>(po + r * D + at_e) = x;
+              *reinterpret_cast<float4*>(po + r * D + at_e) = y;
               if (at_e == 0) {
                 pm[2 * r] = mm;
                 pm[2 * r + 1] = ll;
@@ -699,6 +748,7 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
           }
           __syncthreads();
         }
+      }
       fresh = true;
     }
     if (i + 1 < n) advance(a, at);
@@ -706,123 +756,161 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
   cp_wait<0>();
 }
 
-// Joins what the CTAs left of one segment: block (CTA, row) with the parts
-// of that row, the CTA's own and those behind it, warp w every eighth part.
-constexpr int kJoinWarps = 8;
+// Joins what the CTAs left of a segment. Every CTA that had a part of it takes an equal
+// share of its elements over all parts: 4 elements of a head for a thread, the
+// parts divided over the threads that are left, and added in a fixed tree.
+constexpr int kJoinBlock = 256;
 
-template <typename TQ, int D>
-__global__ void __launch_bounds__(kJoinWarps * 32) attention_join_kernel(const __grid_constant__ AttnArgs a) {
-  __shared__ float s_o[kJoinWarps][D];
-  __shared__ float s_x[kJoinWarps];
+template <typename TQ, int D, int NG>
+__global__ void __launch_bounds__(kJoinBlock) attention_join_kernel(const __grid_constant__ AttnArgs a) {
+  constexpr int kRows = 8 * NG, kUnits = D / 4;
+  __shared__ float s_top[kRows], s_sum[kRows];
+  __shared__ float4 s_red[kJoinBlock];
   ptx::grid_dep_wait();
   ptx::grid_dep_launch_dependents();
   const int tid = thread_here(), lane = tid & 31, warp = tid >> 5;
   // sequences without tokens have no tile: their zeros are written here
-  const int64_t blocks = (int64_t)gridDim.x * gridDim.y;
-  for (int64_t b = (int64_t)blockIdx.y * gridDim.x + blockIdx.x; b < a.batch; b += blocks) {
+  for (int64_t b = blockIdx.x; b < a.batch; b += gridDim.x) {
     if (length_of(a, b) != 0) continue;
-    for (int i = tid; i < a.hq * D; i += kJoinWarps * 32)
+    for (int i = tid; i < a.hq * D; i += kJoinBlock)
       static_cast<TQ*>(a.out)[b * a.hq * D + i] = Pack<TQ>::from_f(0.f);
     if (a.lse)
-      for (int i = tid; i < a.hq; i += kJoinWarps * 32) a.lse[b * a.hq + i] = -INFINITY;
+      for (int i = tid; i < a.hq; i += kJoinBlock) a.lse[b * a.hq + i] = -INFINITY;
   }
   const int64_t workers = gridDim.x, me = blockIdx.x;
-  const Meta* meta = reinterpret_cast<const Meta*>(a.part);
-  const Meta seg = meta[me];
-  if (!seg.open) return;
-  const int group = a.hq / a.hk;
-  const int kvh = seg.hs / a.row_groups, first = (seg.hs - kvh * a.row_groups) * kRows;
-  const int r = blockIdx.y;
-  if (r >= min(kRows, group - first)) return;
-  const float* pm = reinterpret_cast<const float*>(meta + workers);
+  const Seg* meta = reinterpret_cast<const Seg*>(a.part);
+  const float* pm = reinterpret_cast<const float*>(meta + 2 * workers);
   const float* po = pm + 2 * workers * kRows * 2;
-  const int parts = seg.last - (int)me + 1;
-  auto slot = [&](int i) { return i == 0 ? 2 * me + 1 : 2 * (me + i); };
-  float top = -INFINITY;
-  for (int i = tid; i < parts; i += kJoinWarps * 32) top = fmaxf(top, pm[(slot(i) * kRows + r) * 2]);
+  const Seg both[2] = {meta[2 * me], meta[2 * me + 1]};
+  const int group = a.hq / a.hk;
+#pragma unroll 1
+  for (int which = 0; which < 2; ++which) {
+    const Seg seg = both[which];
+    if (seg.owner < 0) continue;
+    const int kvh = seg.hs / a.row_groups, first = (seg.hs - kvh * a.row_groups) * kRows;
+    const int rows = min(kRows, group - first), parts = seg.last - seg.owner + 1, p = (int)me - seg.owner;
+    const int u0 = rows * kUnits * p / parts, u1 = rows * kUnits * (p + 1) / parts;
+    if (u0 == u1) continue;
+    auto slot = [&](int i) { return 2ll * (seg.owner + i) + (i == 0 ? 1 : 0); };
+    const int r0 = u0 / kUnits, r1 = (u1 - 1) / kUnits;
+    __syncthreads();
+    for (int r = r0 + warp; r <= r1; r += kJoinBlock / 32) {
+      float top = -INFINITY, sum = 0.f;
+      for (int i = lane; i < parts; i += 32) top = fmaxf(top, pm[(slot(i) * kRows + r) * 2]);
 #pragma unroll
-  for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
-  if (lane == 0) s_x[warp] = top;
-  __syncthreads();
-  for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, s_x[w]);
-  const float ref = ref_of(top);
-  float o[D / 32], l = 0.f;
-#pragma unroll
-  for (int j = 0; j < D / 32; ++j) o[j] = 0.f;
+      for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
+      for (int i = lane; i < parts; i += 32) {
+        const float2 ml = *reinterpret_cast<const float2*>(pm + (slot(i) * kRows + r) * 2);
+        sum = fmaf(ex2(ml.x - ref_of(top)), ml.y, sum);
+      }
+      sum = warp_allreduce_sum(sum);
+      if (lane == 0) {
+        s_top[r] = top;
+        s_sum[r] = sum;
+      }
+    }
+    __syncthreads();
+    const int nu = min(u1 - u0, kJoinBlock);
+    int slices = kJoinBlock / nu;
+    if (slices > parts) slices = parts;
+    for (int ub = u0; ub < u1; ub += nu) {
+      const int slice = tid / nu, u = ub + tid - slice * nu, r = u / kUnits, e = (u - r * kUnits) * 4;
+      const bool on = slice < slices && u < u1;
+      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (on) {
+        const float ref = ref_of(s_top[r]);
 #pragma unroll 4
-  for (int i = warp; i < parts; i += kJoinWarps) {
-    const float2 ml = *reinterpret_cast<const float2*>(pm + (slot(i) * kRows + r) * 2);
-    const float f = ex2(ml.x - ref);
-    l = fmaf(f, ml.y, l);
-    const float* p = po + (slot(i) * kRows + r) * D;
-#pragma unroll
-    for (int j = 0; j < D / 32; ++j) o[j] = fmaf(f, p[j * 32 + lane], o[j]);
+        for (int i = slice; i < parts; i += slices) {
+          const float f = ex2(pm[(slot(i) * kRows + r) * 2] - ref);
+          const float4 z = *reinterpret_cast<const float4*>(po + (slot(i) * kRows + r) * D + e);
+          y.x = fmaf(f, z.x, y.x);
+          y.y = fmaf(f, z.y, y.y);
+          y.z = fmaf(f, z.z, y.z);
+          y.w = fmaf(f, z.w, y.w);
+        }
+      }
+      for (int left = slices; left > 1;) {
+        const int half = (left + 1) / 2;
+        __syncthreads();
+        s_red[tid] = y;
+        __syncthreads();
+        if (slice + half < left) {
+          const float4 z = s_red[tid + half * nu];
+          y.x += z.x;
+          y.y += z.y;
+          y.z += z.z;
+          y.w += z.w;
+        }
+        left = half;
+      }
+      if (on && slice == 0) {
+        const int64_t row = (int64_t)seg.b * a.hq + kvh * group + first + r;
+        const float l = s_sum[r], d = l == 0.f ? 1.f : l;
+        constexpr bool kQBf16 = __is_same(TQ, __nv_bfloat16);
+        uint2 out;
+        out.x = pack2<kQBf16>(y.x / d, y.y / d);
+        out.y = pack2<kQBf16>(y.z / d, y.w / d);
+        *reinterpret_cast<uint2*>(static_cast<TQ*>(a.out) + row * D + e) = out;
+        if (a.lse && e == 0) a.lse[row] = kLn2 * (ref_of(s_top[r]) + log2f(l));
+      }
+    }
   }
-#pragma unroll
-  for (int j = 0; j < D / 32; ++j) s_o[warp][j * 32 + lane] = o[j];
-  __syncthreads();
-  if (lane == 0) s_x[warp] = l;
-  __syncthreads();
-  l = 0.f;
-  for (int w = 0; w < kJoinWarps; ++w) l += s_x[w];
-  const int64_t row = (int64_t)seg.b * a.hq + kvh * group + first + r;
-  for (int e = tid; e < D; e += kJoinWarps * 32) {
-    float x = 0.f;
-    for (int w = 0; w < kJoinWarps; ++w) x += s_o[w][e];
-    static_cast<TQ*>(a.out)[row * D + e] = Pack<TQ>::from_f(l == 0.f ? 0.f : x / l);
-  }
-  if (a.lse && tid == 0) a.lse[row] = kLn2 * (ref + log2f(l));
 }
 
 // ---- which kernel, and its launch ---------------------------------------------------
 struct Kernels {
   const void* main;
   const void* join;
-  int smem, ctas;
-  std::atomic<bool>* ready;      // per device: the shared-memory limit has been raised
+  int smem, ctas, rows;
+  std::atomic<bool>* ready;   // per device: the shared-memory limit has been raised
 };
 constexpr int kMaxDevices = 64;
 
-template <typename TQ, bool kE4M3, int D>
+template <typename TQ, bool kE4M3, int D, int NG>
 Kernels kernels() {
   static std::atomic<bool> ready[kMaxDevices];
-  return Kernels{reinterpret_cast<const void*>(attention_kernel<TQ, kE4M3, D>),
-                 reinterpret_cast<const void*>(attention_join_kernel<TQ, D>), Shape<D, kE4M3>::kSmem,
-                 Shape<D, kE4M3>::kCtas, ready};
+  return Kernels{reinterpret_cast<const void*>(attention_kernel<TQ, kE4M3, D, NG>),
+                 reinterpret_cast<const void*>(attention_join_kernel<TQ, D, NG>),
+                 Shape<D, kE4M3, NG>::kSmem, Shape<D, kE4M3, NG>::kCtas, 8 * NG, ready};
 }
-template <typename TQ, bool kE4M3>
+template <typename TQ, bool kE4M3, int NG>
 Kernels kernels_of(int d) {
   switch (d) {
     case 64:
-      return kernels<TQ, kE4M3, 64>();
+      return kernels<TQ, kE4M3, 64, NG>();
     case 96:
-      return kernels<TQ, kE4M3, 96>();
+      return kernels<TQ, kE4M3, 96, NG>();
     case 128:
-      return kernels<TQ, kE4M3, 128>();
+      return kernels<TQ, kE4M3, 128, NG>();
     case 192:
-      return kernels<TQ, kE4M3, 192>();
+      return kernels<TQ, kE4M3, 192, NG>();
     case 256:
-      return kernels<TQ, kE4M3, 256>();
+      return kernels<TQ, kE4M3, 256, NG>();
     default:
-      return Kernels{nullptr, nullptr, 0, 0, nullptr};
+      return Kernels{};
   }
 }
-// main == nullptr: the sizes or the type take the plain kernel.
-Kernels find_kernels(int dtype, int cache_dtype, int d) {
-  const bool e4m3 = cache_dtype == RMSNORM_KV_E4M3;
-  if (dtype == RMSNORM_TP_BF16)
-    return e4m3 ? kernels_of<__nv_bfloat16, true>(d) : kernels_of<__nv_bfloat16, false>(d);
-  if (dtype == RMSNORM_TP_F16) return e4m3 ? kernels_of<__half, true>(d) : kernels_of<__half, false>(d);
-  return Kernels{nullptr, nullptr, 0, 0, nullptr};
+// main == nullptr: the sizes or the type take the plain kernel. Groups of more than 8 query
+// heads take two of mma's 8 columns at once, so that K and V leave shared memory once.
+Kernels find_kernels(const rmsnorm_paged_attention_args* a) {
+  const bool e4m3 = a->cache->dtype == RMSNORM_KV_E4M3, bf16 = a->dtype == RMSNORM_TP_BF16;
+  if (!bf16 && a->dtype != RMSNORM_TP_F16) return Kernels{};
+  const int d = a->cache->head_dim;
+  if (a->q_heads / a->cache->kv_heads <= 8) {
+    if (bf16) return e4m3 ? kernels_of<__nv_bfloat16, true, 1>(d) : kernels_of<__nv_bfloat16, false, 1>(d);
+    return e4m3 ? kernels_of<__half, true, 1>(d) : kernels_of<__half, false, 1>(d);
+  }
+  if (bf16) return e4m3 ? kernels_of<__nv_bfloat16, true, 2>(d) : kernels_of<__nv_bfloat16, false, 2>(d);
+  return e4m3 ? kernels_of<__half, true, 2>(d) : kernels_of<__half, false, 2>(d);
 }
 
-int row_groups_of(const rmsnorm_paged_attention_args* a) {
-  return (a->q_heads / a->cache->kv_heads + kRows - 1) / kRows;
+int row_groups_of(const rmsnorm_paged_attention_args* a, const Kernels& k) {
+  return (a->q_heads / a->cache->kv_heads + k.rows - 1) / k.rows;
 }
 // CTAs of the main kernel: one resident wave, or a tile each of the longest lengths.
 int64_t worker_count(const rmsnorm_paged_attention_args* a, const Kernels& k, int sms) {
   const int64_t tiles = (a->max_pages * a->cache->page_size + kTile - 1) / kTile;
-  const int64_t most = tiles * a->batch * a->cache->kv_heads * row_groups_of(a);
+  const int64_t most = tiles * a->batch * a->cache->kv_heads * row_groups_of(a, k);
   const int64_t wave = (int64_t)sms * k.ctas;
   return most < 1 ? 1 : most < wave ? most : wave;
 }
@@ -857,8 +945,8 @@ int check_attention(const char* who, const rmsnorm_paged_attention_args* a) {
                   a->q_heads, c->kv_heads);
   if (a->batch < 0 || a->batch > 65535)
     return refuse(RMSNORM_TP_ERR_INVALID, "%s: batch %lld outside [0, 65535]", who, (long long)a->batch);
-  if (a->max_pages < 0 || a->max_pages * (int64_t)c->page_size > (int64_t(1) << 31) - 1)
-    return refuse(RMSNORM_TP_ERR_INVALID, "%s: %lld pages of %d tokens: a sequence holds under 2^31 tokens",
+  if (a->max_pages < 0 || a->max_pages * (int64_t)c->page_size > kMostTokens)
+    return refuse(RMSNORM_TP_ERR_INVALID, "%s: %lld pages of %d tokens: a sequence holds at most 2^31 - 128",
                   who, (long long)a->max_pages, c->page_size);
   if (a->device < 0) return refuse(RMSNORM_TP_ERR_INVALID, "%s: device %d", who, a->device);
   return RMSNORM_TP_OK;
@@ -877,10 +965,10 @@ size_t rmsnorm_paged_attention_workspace_bytes(const rmsnorm_paged_attention_arg
     refuse(RMSNORM_TP_ERR_CUDA, "paged_attention_workspace_bytes: no device %d", a->device);
     return 0;
   }
-  const Kernels k = find_kernels(a->dtype, a->cache->dtype, a->cache->head_dim);
+  const Kernels k = find_kernels(a);
   if (k.main != nullptr)
-    return (size_t)worker_count(a, k, sms) *
-           (sizeof(Meta) + 2 * kRows * (size_t)(a->cache->head_dim + 2) * sizeof(float));
+    return (size_t)worker_count(a, k, sms) * 2 *
+           (sizeof(Seg) + k.rows * (size_t)(a->cache->head_dim + 2) * sizeof(float));
   return (size_t)a->batch * a->q_heads * any_splits(a, sms) * (a->cache->head_dim + 2) * sizeof(float);
 }
 
@@ -926,15 +1014,16 @@ int rmsnorm_paged_attention(const rmsnorm_paged_attention_args* in, void* stream
   a.page = c->page_size;
   a.d = c->head_dim;
   a.scale_log2 = in->scale * kLog2e;
-  a.row_groups = row_groups_of(in);
-  a.segments = a.hk * a.row_groups;
   a.q_pairs = ((reinterpret_cast<uintptr_t>(in->q) & 3u) | (uintptr_t)((a.qst | a.qsh) & 1)) == 0;
   OnDevice on(in->device);
   if (on.err != cudaSuccess) return launch_failed(on.err, who);
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   void* args[] = {&a};
-  const Kernels k = find_kernels(in->dtype, c->dtype, a.d);
+  const Kernels k = find_kernels(in);
   if (k.main != nullptr) {
+    a.row_groups = row_groups_of(in, k);
+    a.segments = a.hk * a.row_groups;
+    a.whole_pages = a.page % 16 == 0;
     if (in->device >= kMaxDevices || !k.ready[in->device]) {
       const cudaError_t e =
           cudaFuncSetAttribute(k.main, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem);
@@ -943,9 +1032,7 @@ int rmsnorm_paged_attention(const rmsnorm_paged_attention_args* in, void* stream
     }
     const unsigned n = (unsigned)worker_count(in, k, sms);
     cudaError_t e = launch_dependent(k.main, dim3(n), dim3(kBlock), k.smem, args, st);
-    const int group = a.hq / a.hk;
-    if (e == cudaSuccess)
-      e = launch_dependent(k.join, dim3(n, group < kRows ? group : kRows), dim3(kJoinWarps * 32), 0, args, st);
+    if (e == cudaSuccess) e = launch_dependent(k.join, dim3(n), dim3(kJoinBlock), 0, args, st);
     return e == cudaSuccess ? RMSNORM_TP_OK : launch_failed(e, who);
   }
   a.splits = any_splits(in, sms);
