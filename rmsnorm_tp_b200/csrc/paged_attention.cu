@@ -29,6 +29,7 @@ struct AttnArgs {
   int segments;         // kv heads * row_groups
   int q_pairs;          // the queries' elements can be read two at a time
   int whole_pages;      // pages of 16 k tokens
+  unsigned page_mul, page_shift;   // t / page = (umulhi(t, mul) + t) >> shift for t < 2^31
   float scale_log2;     // scale * log2(e): scores in base 2
 };
 
@@ -204,7 +205,10 @@ struct Shape {
   static_assert(kStages >= 3, "the ring needs three stages");
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async16_if(uint32_t dst, const void* src, bool live) {
   const int n = live ? 16 : 0;          // 0: zeros, nothing is read
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
 }
@@ -296,9 +300,10 @@ __device__ __forceinline__ float head_sum(float v) {
 // The reference of exponentials: 0 where nothing has been seen (their value is 0 then).
 __device__ __forceinline__ float ref_of(float m) { return m == -INFINITY ? 0.f : m; }
 
-// Place in the row of tiles: tile `tile` of the `tiles` of segment (b, hs).
+// Place in the row of tiles: tile `tile` of the `tiles` of segment (sequence b, kv head,
+// group of its query heads).
 struct Place {
-  int b, hs, tile, tiles, len;
+  int b, kvh, rg, tile, tiles, len;
 };
 
 __device__ __forceinline__ int tiles_of(int64_t len) { return (int)((len + kTile - 1) / kTile); }
@@ -307,8 +312,10 @@ __device__ __forceinline__ int tiles_of(int64_t len) { return (int)((len + kTile
 __device__ __forceinline__ void advance(const AttnArgs& a, Place& p) {
   if (++p.tile < p.tiles) return;
   p.tile = 0;
-  if (++p.hs < a.segments) return;
-  p.hs = 0;
+  if (++p.rg < a.row_groups) return;
+  p.rg = 0;
+  if (++p.kvh < a.hk) return;
+  p.kvh = 0;
   do {
     ++p.b;
     p.len = (int)length_of(a, p.b);
@@ -383,11 +390,13 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
   at.b = s_b;
   at.len = (int)length_of(a, at.b);
   at.tiles = tiles_of(at.len);
-  at.hs = (int)(s_rest / at.tiles);
-  at.tile = (int)(s_rest - (int64_t)at.hs * at.tiles);
+  const int hs = (int)(s_rest / at.tiles);
+  at.tile = (int)(s_rest - (int64_t)hs * at.tiles);
+  at.kvh = hs / a.row_groups;
+  at.rg = hs - at.kvh * a.row_groups;
   const int n = (int)(t1 - t0);
   if (tid == 0 && at.tile > 0)
-    meta[0] = Seg{at.b, at.hs, worker_of(t0 - at.tile), worker_of(t0 - at.tile + at.tiles - 1)};
+    meta[0] = Seg{at.b, hs, worker_of(t0 - at.tile), worker_of(t0 - at.tile + at.tiles - 1)};
 
   float* join = reinterpret_cast<float*>(smem);
   unsigned char* ring_p = smem + S::kJoin + warp * S::kStages * S::kStage;
@@ -397,53 +406,69 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
   const int lr = lane / S::kLanes, lc = lane % S::kLanes;
   const unsigned char* kp = static_cast<const unsigned char*>(a.k) + lc * 16;
   const unsigned char* vp = static_cast<const unsigned char*>(a.v) + lc * 16;
-  const uint32_t side_off = 2 * S::kOperand;
+  constexpr uint32_t kSideOff = 2 * S::kOperand, kMaskOff = kSideOff + (kE4M3 ? 128 : 0);
+  // this lane's chunk of its row in the tile, for rows lr and lr + 4 of 8
+  const uint32_t to0 = lr * S::kPitch + (S::kSwizzle ? lc ^ (lr & 7) : lc) * 16;
+  const uint32_t to1 = lr * S::kPitch + (S::kSwizzle ? lc ^ ((lr + S::kRowsAtOnce) & 7) : lc) * 16;
+  const int lane_tok = warp * 16 + (a.whole_pages ? 0 : lane & 15);
   Place ahead = at;
-  int sent = 0, into = 0;
-  int32_t page_id = -1;               // read one tile early
+  int left = n;                       // tiles not yet asked for
+  uint32_t into = 0;                  // stage that the next tile goes to
+  int32_t page_id = -1, page_off = 0; // read one tile early
   // pages of 16 k tokens: the warp's 16 tokens lie in one page, one row behind another;
   // else lane l (and l + 16) knows the row of token l
   auto look_up = [&]() {
-    const int t = ahead.tile * kTile + warp * 16 + (a.whole_pages ? 0 : lane & 15);
-    page_id = t < ahead.len ? a.table[ahead.b * a.table_stride + (unsigned)t / (unsigned)a.page] : -1;
+    const int t = ahead.tile * kTile + lane_tok;
+    const unsigned pg = (__umulhi((unsigned)t, a.page_mul) + (unsigned)t) >> a.page_shift;
+    page_off = t - (int)pg * a.page;
+    page_id = t < ahead.len ? a.table[ahead.b * a.table_stride + pg] : -1;
   };
   look_up();
   auto send = [&]() {
-    if (sent < n) {
+    if (left > 0) {
       const uint32_t dst = ring + into * S::kStage;
-      const int t = ahead.tile * kTile + warp * 16 + (a.whole_pages ? 0 : lane & 15);
-      const int kvh = ahead.hs / a.row_groups;
-      const bool live = page_id >= 0 && page_id < a.num_pages;
-      const int64_t row = live ? ((int64_t)page_id * a.hk + kvh) * a.page + (unsigned)t % (unsigned)a.page : 0;
+      const bool live = (unsigned)page_id < (unsigned)a.num_pages;
+      const int64_t row = live ? ((int64_t)page_id * a.hk + ahead.kvh) * a.page + page_off : 0;
+      const int rest = ahead.len - (ahead.tile * kTile + lane_tok);
       unsigned mask;
-      if (a.whole_pages) {
-        const int left = ahead.len - t;
-        mask = !live ? 0u : left >= 16 ? 0xFFFFu : (1u << left) - 1u;
-      } else {
-        mask = __ballot_sync(0xFFFFFFFFu, live) & 0xFFFFu;
-      }
+      if (a.whole_pages) mask = !live ? 0u : rest >= 16 ? 0xFFFFu : (1u << rest) - 1u;
+      else mask = __ballot_sync(0xFFFFFFFFu, live) & 0xFFFFu;
+      if (lane == 0) *reinterpret_cast<unsigned*>(ring_p + into * S::kStage + kMaskOff) = mask;
       if constexpr (kE4M3) {          // lanes 0-15 K's scales, 16-31 V's
         const int64_t r = a.whole_pages ? row + (lane & 15) : row;
         const bool on = (mask >> (lane & 15)) & 1u;
-        cp_async4(dst + side_off + lane * 4, (lane < 16 ? a.ks : a.vs) + (on ? r : 0), on);
+        cp_async4(dst + kSideOff + lane * 4, (lane < 16 ? a.ks : a.vs) + (on ? r : 0), on);
       }
+      if (a.whole_pages && mask == 0xFFFFu) {
+        const int64_t from = (row + lr) * S::kRowBytes;
+        const unsigned char* kf = kp + from;
+        const unsigned char* vf = vp + from;
 #pragma unroll
-      for (int i = 0; i < 16 / S::kRowsAtOnce; ++i) {
-        const int r = i * S::kRowsAtOnce + lr;
-        const int64_t from = (a.whole_pages ? row + r : __shfl_sync(0xFFFFFFFFu, row, r)) * S::kRowBytes;
-        const bool on = (mask >> r) & 1u;
-        const int64_t safe = on ? from : 0;
-        const uint32_t to = dst + r * S::kPitch + (S::kSwizzle ? lc ^ (r & 7) : lc) * 16;
+        for (int i = 0; i < 16 / S::kRowsAtOnce; ++i)
 #pragma unroll
-        for (int k = 0; k < S::kChunks / S::kLanes; ++k) {
-          cp_async16(to + k * S::kLanes * 16, kp + safe + k * S::kLanes * 16, on);
-          cp_async16(to + S::kOperand + k * S::kLanes * 16, vp + safe + k * S::kLanes * 16, on);
+          for (int k = 0; k < S::kChunks / S::kLanes; ++k) {
+            const uint32_t to = dst + (i & 1 ? to1 : to0) + i * S::kRowsAtOnce * S::kPitch + k * S::kLanes * 16;
+            const int at = i * S::kRowsAtOnce * S::kRowBytes + k * S::kLanes * 16;
+            cp_async16(to, kf + at);
+            cp_async16(to + S::kOperand, vf + at);
+          }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16 / S::kRowsAtOnce; ++i) {
+          const int r = i * S::kRowsAtOnce + lr;
+          const int64_t from = (a.whole_pages ? row + r : __shfl_sync(0xFFFFFFFFu, row, r)) * S::kRowBytes;
+          const bool on = (mask >> r) & 1u;
+          const int64_t safe = on ? from : 0;
+          const uint32_t to = dst + (i & 1 ? to1 : to0) + i * S::kRowsAtOnce * S::kPitch;
+#pragma unroll
+          for (int k = 0; k < S::kChunks / S::kLanes; ++k) {
+            cp_async16_if(to + k * S::kLanes * 16, kp + safe + k * S::kLanes * 16, on);
+            cp_async16_if(to + S::kOperand + k * S::kLanes * 16, vp + safe + k * S::kLanes * 16, on);
+          }
         }
       }
-      if (lane == 0)
-        *reinterpret_cast<unsigned*>(ring_p + into * S::kStage + side_off + (kE4M3 ? 128 : 0)) = mask;
       into = into + 1 == S::kStages ? 0 : into + 1;
-      if (++sent < n) {
+      if (--left > 0) {
         advance(a, ahead);
         look_up();
       }
@@ -457,7 +482,7 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
   float o[NG][KS][4];                 // [16 elements][head 2 qd, 2 qd + 1] of each group of 8
   float m[NG][2], l[NG][2], mv[NG][2];   // references of the scores and (e4m3) of the V-weighted ones
   float unit[NG][2];                  // factor of the raw scores
-  int rows = 0, stage = 0;
+  uint32_t stage = 0;
 
   // K as 16 tokens x 16 elements: matrices (tokens 0-7, 8-15) x (chunk, next chunk)
   const uint32_t k_tok = ((lane >> 3) & 1) * 8 + (lane & 7), k_chunk = lane >> 4;
@@ -466,17 +491,15 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
   const uint32_t v_chunk = kE4M3 ? k_chunk : (lane >> 3) & 1;
   const uint32_t k_row = k_tok * S::kPitch, v_row = S::kOperand + v_tok * S::kPitch;
 
-  bool fresh = true, whole = false, began = false;
 #pragma unroll 1
-  for (int i = 0; i < n; ++i) {
-    if (fresh) {
-      fresh = false;
-      began = whole = at.tile == 0;
-      const int group = a.hq / a.hk;
-      const int kvh = at.hs / a.row_groups, first = (at.hs - kvh * a.row_groups) * kRows;
-      rows = min(kRows, group - first);
+  for (int i = 0; i < n;) {
+    // ---- a segment, or what this CTA has of it ----
+    const bool began = at.tile == 0;
+    const int group = a.hq / a.hk, first = at.rg * kRows, rows = min(kRows, group - first);
+    const int end = min(at.tiles, at.tile + (n - i));
+    {
       const unsigned short* qu = static_cast<const unsigned short*>(a.q) + at.b * a.qst +
-                                 (int64_t)(kvh * group + first) * a.qsh;
+                                 (int64_t)(at.kvh * group + first) * a.qsh;
 #pragma unroll
       for (int x = 0; x < NG; ++x) {
 #pragma unroll
@@ -530,145 +553,149 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
         l[x][0] = l[x][1] = 0.f;
       }
     }
-    cp_wait<S::kStages - 2>();
-    __syncwarp();
-    send();                           // into the stage that every lane left in the last turn
-    const uint32_t base = ring + stage * S::kStage;
-    const unsigned char* side = ring_p + stage * S::kStage + side_off;
-    stage = stage + 1 == S::kStages ? 0 : stage + 1;
-    const unsigned mask = *reinterpret_cast<const unsigned*>(side + (kE4M3 ? 128 : 0));
-    if (mask != 0u) {
-      float s[NG][4];                 // (token g, heads 2 qd, 2 qd + 1), (token g + 8, the same)
-      {
-        float s2[NG][4];              // the odd steps' sums: two chains instead of one
+#pragma unroll 1
+    for (int tile = at.tile; tile < end; ++tile) {
+      cp_wait<S::kStages - 2>();
+      __syncwarp();
+      send();                           // into the stage that every lane left in the last turn
+      const uint32_t base = ring + stage * S::kStage;
+      const unsigned char* side = ring_p + stage * S::kStage + kSideOff;
+      stage = stage + 1 == S::kStages ? 0 : stage + 1;
+      const unsigned mask = *reinterpret_cast<const unsigned*>(side + (kE4M3 ? 128 : 0));
+      if (mask != 0u) {
+        float s[NG][4];                 // (token g, heads 2 qd, 2 qd + 1), (token g + 8, the same)
+        {
+          float s2[NG][4];              // the odd steps' sums: two chains instead of one
+#pragma unroll
+          for (int x = 0; x < NG; ++x)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[x][j] = s2[x][j] = 0.f;
+#pragma unroll
+          for (int ks = 0; ks < KS; ks += 2) {
+            uint32_t r[4], r2[4];
+            if constexpr (kE4M3) {
+              const uint32_t c = ks + k_chunk;
+              uint32_t w[4];
+              ldsm4(w, base + k_row + (S::kSwizzle ? c ^ (k_tok & 7) : c) * 16);
+              r[0] = e4m3x2_f16x2(w[0]), r[2] = e4m3x2_f16x2(w[0] >> 16);
+              r[1] = e4m3x2_f16x2(w[1]), r[3] = e4m3x2_f16x2(w[1] >> 16);
+              r2[0] = e4m3x2_f16x2(w[2]), r2[2] = e4m3x2_f16x2(w[2] >> 16);
+              r2[1] = e4m3x2_f16x2(w[3]), r2[3] = e4m3x2_f16x2(w[3] >> 16);
+            } else {
+              const uint32_t c = 2 * ks + k_chunk;
+              ldsm4(r, base + k_row + (S::kSwizzle ? c ^ (k_tok & 7) : c) * 16);
+              ldsm4(r2, base + k_row + (S::kSwizzle ? (c + 2) ^ (k_tok & 7) : c + 2) * 16);
+            }
+#pragma unroll
+            for (int x = 0; x < NG; ++x) {
+              mma<kBf16>(s[x], r, q[x][ks][0], q[x][ks][1]);
+              mma<kBf16>(s2[x], r2, q[x][ks + 1][0], q[x][ks + 1][1]);
+            }
+          }
+#pragma unroll
+          for (int x = 0; x < NG; ++x)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[x][j] += s2[x][j];
+        }
+        const bool on[2] = {(bool)((mask >> g) & 1u), (bool)((mask >> (g + 8)) & 1u)};
+        float ksc[2] = {1.f, 1.f}, lv[2] = {0.f, 0.f};
+        if constexpr (kE4M3) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            ksc[t] = reinterpret_cast<const float*>(side)[8 * t + g];
+            lv[t] = lg2(reinterpret_cast<const float*>(side)[16 + 8 * t + g]);
+          }
+        }
+        bool rise = false;
 #pragma unroll
         for (int x = 0; x < NG; ++x)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) s[x][j] = s2[x][j] = 0.f;
+          for (int j = 0; j < 4; ++j) {
+            const int t = j >> 1, h = j & 1;
+            s[x][j] = on[t] ? s[x][j] * (kE4M3 ? unit[x][h] * ksc[t] : unit[x][h]) : -INFINITY;
+            rise |= s[x][j] > m[x][h] + kSlack;
+            if constexpr (kE4M3) rise |= on[t] && s[x][j] + lv[t] > mv[x][h] + kSlack;
+          }
+        if (__any_sync(0xFFFFFFFFu, rise)) {
 #pragma unroll
-        for (int ks = 0; ks < KS; ks += 2) {
+          for (int x = 0; x < NG; ++x)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float now = fmaxf(m[x][h], head_max(fmaxf(s[x][h], s[x][2 + h])));
+              float keep = ex2(m[x][h] - ref_of(now));
+              l[x][h] *= keep;
+              m[x][h] = now;
+              if constexpr (kE4M3) {
+                const float nowv = fmaxf(mv[x][h], head_max(fmaxf(on[0] ? s[x][h] + lv[0] : -INFINITY,
+                                                                 on[1] ? s[x][2 + h] + lv[1] : -INFINITY)));
+                keep = ex2(mv[x][h] - ref_of(nowv));
+                mv[x][h] = nowv;
+              }
+#pragma unroll
+              for (int j = 0; j < KS; ++j) {
+                o[x][j][h] *= keep;
+                o[x][j][2 + h] *= keep;
+              }
+            }
+        }
+        uint32_t hi[NG][2], lo[NG][2];  // P as 16 tokens x 8 heads
+#pragma unroll
+        for (int x = 0; x < NG; ++x) {
+          const float ref[2] = {ref_of(m[x][0]), ref_of(m[x][1])};
+          const float refv[2] = {ref_of(mv[x][0]), ref_of(mv[x][1])};
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            float w[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float v = s[x][2 * t + h], p = ex2(v - ref[h]);
+              l[x][h] += p;
+              w[h] = kE4M3 ? (on[t] ? ex2(v + lv[t] - refv[h]) : 0.f) : p * kLift;
+            }
+            if constexpr (kTwoParts) {
+              split2<kBf16>(w[0], w[1], hi[x][t], lo[x][t]);
+              lo[x][t] = transposed(lo[x][t]);
+            } else {
+              hi[x][t] = pack2<kBf16>(w[0], w[1]);
+            }
+            hi[x][t] = transposed(hi[x][t]);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < KS; j += kE4M3 ? 2 : 1) {
           uint32_t r[4], r2[4];
+          const uint32_t c = (kE4M3 ? j : 2 * j) + v_chunk;
+          const uint32_t from = base + v_row + (S::kSwizzle ? c ^ (v_tok & 7) : c) * 16;
           if constexpr (kE4M3) {
-            const uint32_t c = ks + k_chunk;
+            // bytes of w: (token 2 qd: elements 2 g, 2 g + 1), (token 2 qd + 1: the same), so row g
+            // of the product is element 2 g and row g + 8 element 2 g + 1
             uint32_t w[4];
-            ldsm4(w, base + k_row + (S::kSwizzle ? c ^ (k_tok & 7) : c) * 16);
-            r[0] = e4m3x2_f16x2(w[0]), r[2] = e4m3x2_f16x2(w[0] >> 16);
-            r[1] = e4m3x2_f16x2(w[1]), r[3] = e4m3x2_f16x2(w[1] >> 16);
-            r2[0] = e4m3x2_f16x2(w[2]), r2[2] = e4m3x2_f16x2(w[2] >> 16);
-            r2[1] = e4m3x2_f16x2(w[3]), r2[3] = e4m3x2_f16x2(w[3] >> 16);
+            ldsm4t(w, from);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) w[t] = __byte_perm(w[t], 0, 0x3120);
+            r[0] = e4m3x2_f16x2(w[0]), r[1] = e4m3x2_f16x2(w[0] >> 16);
+            r[2] = e4m3x2_f16x2(w[1]), r[3] = e4m3x2_f16x2(w[1] >> 16);
+            r2[0] = e4m3x2_f16x2(w[2]), r2[1] = e4m3x2_f16x2(w[2] >> 16);
+            r2[2] = e4m3x2_f16x2(w[3]), r2[3] = e4m3x2_f16x2(w[3] >> 16);
           } else {
-            const uint32_t c = 2 * ks + k_chunk;
-            ldsm4(r, base + k_row + (S::kSwizzle ? c ^ (k_tok & 7) : c) * 16);
-            ldsm4(r2, base + k_row + (S::kSwizzle ? (c + 2) ^ (k_tok & 7) : c + 2) * 16);
+            ldsm4t(r, from);
           }
 #pragma unroll
           for (int x = 0; x < NG; ++x) {
-            mma<kBf16>(s[x], r, q[x][ks][0], q[x][ks][1]);
-            mma<kBf16>(s2[x], r2, q[x][ks + 1][0], q[x][ks + 1][1]);
-          }
-        }
-#pragma unroll
-        for (int x = 0; x < NG; ++x)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) s[x][j] += s2[x][j];
-      }
-      const bool on[2] = {(bool)((mask >> g) & 1u), (bool)((mask >> (g + 8)) & 1u)};
-      float ksc[2] = {1.f, 1.f}, lv[2] = {0.f, 0.f};
-      if constexpr (kE4M3) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          ksc[t] = reinterpret_cast<const float*>(side)[8 * t + g];
-          lv[t] = lg2(reinterpret_cast<const float*>(side)[16 + 8 * t + g]);
-        }
-      }
-      bool rise = false;
-#pragma unroll
-      for (int x = 0; x < NG; ++x)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int t = j >> 1, h = j & 1;
-          s[x][j] = on[t] ? s[x][j] * (kE4M3 ? unit[x][h] * ksc[t] : unit[x][h]) : -INFINITY;
-          rise |= s[x][j] > m[x][h] + kSlack;
-          if constexpr (kE4M3) rise |= on[t] && s[x][j] + lv[t] > mv[x][h] + kSlack;
-        }
-      if (__any_sync(0xFFFFFFFFu, rise)) {
-#pragma unroll
-        for (int x = 0; x < NG; ++x)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float now = fmaxf(m[x][h], head_max(fmaxf(s[x][h], s[x][2 + h])));
-            float keep = ex2(m[x][h] - ref_of(now));
-            l[x][h] *= keep;
-            m[x][h] = now;
+            mma<kBf16>(o[x][j], r, hi[x][0], hi[x][1]);
+            if constexpr (kTwoParts) mma<kBf16>(o[x][j], r, lo[x][0], lo[x][1]);
             if constexpr (kE4M3) {
-              const float nowv = fmaxf(mv[x][h], head_max(fmaxf(on[0] ? s[x][h] + lv[0] : -INFINITY,
-                                                               on[1] ? s[x][2 + h] + lv[1] : -INFINITY)));
-              keep = ex2(mv[x][h] - ref_of(nowv));
-              mv[x][h] = nowv;
+              mma<kBf16>(o[x][j + 1], r2, hi[x][0], hi[x][1]);
+              if constexpr (kTwoParts) mma<kBf16>(o[x][j + 1], r2, lo[x][0], lo[x][1]);
             }
-#pragma unroll
-            for (int j = 0; j < KS; ++j) {
-              o[x][j][h] *= keep;
-              o[x][j][2 + h] *= keep;
-            }
-          }
-      }
-      uint32_t hi[NG][2], lo[NG][2];  // P as 16 tokens x 8 heads
-#pragma unroll
-      for (int x = 0; x < NG; ++x) {
-        const float ref[2] = {ref_of(m[x][0]), ref_of(m[x][1])};
-        const float refv[2] = {ref_of(mv[x][0]), ref_of(mv[x][1])};
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          float w[2];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float v = s[x][2 * t + h], p = ex2(v - ref[h]);
-            l[x][h] += p;
-            w[h] = kE4M3 ? (on[t] ? ex2(v + lv[t] - refv[h]) : 0.f) : p * kLift;
-          }
-          if constexpr (kTwoParts) {
-            split2<kBf16>(w[0], w[1], hi[x][t], lo[x][t]);
-            lo[x][t] = transposed(lo[x][t]);
-          } else {
-            hi[x][t] = pack2<kBf16>(w[0], w[1]);
-          }
-          hi[x][t] = transposed(hi[x][t]);
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < KS; j += kE4M3 ? 2 : 1) {
-        uint32_t r[4], r2[4];
-        const uint32_t c = (kE4M3 ? j : 2 * j) + v_chunk;
-        const uint32_t from = base + v_row + (S::kSwizzle ? c ^ (v_tok & 7) : c) * 16;
-        if constexpr (kE4M3) {
-          // bytes of w: (token 2 qd: elements 2 g, 2 g + 1), (token 2 qd + 1: the same), so row g
-          // of the product is element 2 g and row g + 8 element 2 g + 1
-          uint32_t w[4];
-          ldsm4t(w, from);
-#pragma unroll
-          for (int t = 0; t < 4; ++t) w[t] = __byte_perm(w[t], 0, 0x3120);
-          r[0] = e4m3x2_f16x2(w[0]), r[1] = e4m3x2_f16x2(w[0] >> 16);
-          r[2] = e4m3x2_f16x2(w[1]), r[3] = e4m3x2_f16x2(w[1] >> 16);
-          r2[0] = e4m3x2_f16x2(w[2]), r2[1] = e4m3x2_f16x2(w[2] >> 16);
-          r2[2] = e4m3x2_f16x2(w[3]), r2[3] = e4m3x2_f16x2(w[3] >> 16);
-        } else {
-          ldsm4t(r, from);
-        }
-#pragma unroll
-        for (int x = 0; x < NG; ++x) {
-          mma<kBf16>(o[x][j], r, hi[x][0], hi[x][1]);
-          if constexpr (kTwoParts) mma<kBf16>(o[x][j], r, lo[x][0], lo[x][1]);
-          if constexpr (kE4M3) {
-            mma<kBf16>(o[x][j + 1], r2, hi[x][0], hi[x][1]);
-            if constexpr (kTwoParts) mma<kBf16>(o[x][j + 1], r2, lo[x][0], lo[x][1]);
           }
         }
       }
     }
 
-    const bool last = at.tile + 1 == at.tiles;
-    if (last || i + 1 == n) {
+    const bool last = end == at.tiles, whole = began && last;
+    i += end - at.tile;
+    {
       // ---- the warps' results of the segment, joined: half of 8 heads' elements at a time
 #pragma unroll
       for (int x = 0; x < NG; ++x)
@@ -681,16 +708,14 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
             s_l[warp][8 * x + 2 * qd + h] = sum;
           }
         }
-      whole = whole && last;
-      const int kvh = at.hs / a.row_groups, first = (at.hs - kvh * a.row_groups) * kRows;
-      const int64_t out_row = (int64_t)at.b * a.hq + kvh * (a.hq / a.hk) + first;
+      const int64_t out_row = (int64_t)at.b * a.hq + at.kvh * group + first;
       // the part of a segment that began before, or of one left open
       const int64_t slot = 2 * me + (began ? 1 : 0);
       float* pm = reinterpret_cast<float*>(reinterpret_cast<Seg*>(a.part) + 2 * gridDim.x) + slot * kRows * 2;
       float* po = reinterpret_cast<float*>(reinterpret_cast<Seg*>(a.part) + 2 * gridDim.x) +
                   2ll * gridDim.x * kRows * 2 + slot * kRows * D;
       if (tid == 0 && began && !last)
-        meta[1] = Seg{at.b, at.hs, (int)me, worker_of(t1 - 1 + (at.tiles - 1 - at.tile))};
+        meta[1] = Seg{at.b, at.kvh * a.row_groups + at.rg, (int)me, worker_of(t1 + (at.tiles - end) - 1)};
       constexpr int kHalf = D / 2;
 #pragma unroll
       for (int x = 0; x < NG; ++x) {
@@ -749,111 +774,111 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
           __syncthreads();
         }
       }
-      fresh = true;
     }
-    if (i + 1 < n) advance(a, at);
+    if (i < n) {
+      at.tile = at.tiles - 1;
+      advance(a, at);
+    }
   }
   cp_wait<0>();
 }
 
 // Joins what the CTAs left of a segment. Every CTA that had a part of it takes an equal
-// share of its elements over all parts: 4 elements of a head for a thread, the
-// parts divided over the threads that are left, and added in a fixed tree.
+// share of its elements over all parts: 4 elements of a head for a thread, the parts
+// divided over neighbouring threads. A thread's (reference, sum, elements) and its
+// neighbours' are joined as a softmax's halves are, in a fixed tree.
 constexpr int kJoinBlock = 256;
+
+struct Part {
+  float m, l;
+  float4 y;
+  __device__ __forceinline__ void add(float m2, float l2, const float4& y2) {
+    const float top = fmaxf(m, m2), ref = ref_of(top);
+    const float f = ex2(m - ref), f2 = ex2(m2 - ref);
+    m = top;
+    l = l * f + l2 * f2;
+    y.x = y.x * f + y2.x * f2;
+    y.y = y.y * f + y2.y * f2;
+    y.z = y.z * f + y2.z * f2;
+    y.w = y.w * f + y2.w * f2;
+  }
+};
 
 template <typename TQ, int D, int NG>
 __global__ void __launch_bounds__(kJoinBlock) attention_join_kernel(const __grid_constant__ AttnArgs a) {
   constexpr int kRows = 8 * NG, kUnits = D / 4;
-  __shared__ float s_top[kRows], s_sum[kRows];
-  __shared__ float4 s_red[kJoinBlock];
+  __shared__ float s_m[kJoinBlock / 32], s_l[kJoinBlock / 32];
+  __shared__ float4 s_y[kJoinBlock / 32];
   ptx::grid_dep_wait();
   ptx::grid_dep_launch_dependents();
-  const int tid = thread_here(), lane = tid & 31, warp = tid >> 5;
+  const int tid = thread_here();
+  const int64_t workers = gridDim.x, me = blockIdx.x;
+  const Seg* meta = reinterpret_cast<const Seg*>(a.part);
+  const float* pm = reinterpret_cast<const float*>(meta + 2 * workers);
+  const float* po = pm + 2 * workers * kRows * 2;
+  const int4 both[2] = {*reinterpret_cast<const int4*>(meta + 2 * me), *reinterpret_cast<const int4*>(meta + 2 * me + 1)};
+  const int group = a.hq / a.hk;
+#pragma unroll 1
+  for (int which = 0; which < 2; ++which) {
+    const Seg seg{both[which].x, both[which].y, both[which].z, both[which].w};
+    if (seg.owner < 0) continue;
+    const int kvh = seg.hs / a.row_groups, first = (seg.hs - kvh * a.row_groups) * kRows;
+    const int rows = min(kRows, group - first), parts = seg.last - seg.owner + 1, p = (int)me - seg.owner;
+    const int u0 = rows * kUnits * p / parts, u1 = rows * kUnits * (p + 1) / parts;
+    // threads of one unit: a power of two, no more than half of them idle
+    int lg = 0;
+    while ((2 << lg) * (u1 - u0) <= kJoinBlock && (1 << lg) < parts) ++lg;
+    const int slices = 1 << lg, at_once = kJoinBlock >> lg;
+    for (int ub = u0; ub < u1; ub += at_once) {
+      const int u = ub + (tid >> lg), r = u / kUnits, e = (u - r * kUnits) * 4;
+      Part mine{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+      if (u < u1) {
+#pragma unroll 4
+        for (int i = tid & (slices - 1); i < parts; i += slices) {
+          const int64_t at = (2ll * (seg.owner + i) + (i == 0 ? 1 : 0)) * kRows + r;
+          const float2 ml = *reinterpret_cast<const float2*>(pm + at * 2);
+          mine.add(ml.x, ml.y, *reinterpret_cast<const float4*>(po + at * D + e));
+        }
+      }
+      for (int o = min(slices, 32) >> 1; o > 0; o >>= 1) {
+        const float m2 = __shfl_xor_sync(0xFFFFFFFFu, mine.m, o), l2 = __shfl_xor_sync(0xFFFFFFFFu, mine.l, o);
+        const float4 y2 = make_float4(__shfl_xor_sync(0xFFFFFFFFu, mine.y.x, o), __shfl_xor_sync(0xFFFFFFFFu, mine.y.y, o),
+                                      __shfl_xor_sync(0xFFFFFFFFu, mine.y.z, o), __shfl_xor_sync(0xFFFFFFFFu, mine.y.w, o));
+        mine.add(m2, l2, y2);
+      }
+      if (slices > 32) {              // several warps for one unit
+        __syncthreads();
+        if ((tid & 31) == 0) {
+          s_m[tid >> 5] = mine.m;
+          s_l[tid >> 5] = mine.l;
+          s_y[tid >> 5] = mine.y;
+        }
+        __syncthreads();
+        if ((tid & (slices - 1)) == 0)
+          for (int w = 1; w < slices / 32; ++w) {
+            const int v = (tid >> 5) + w;
+            mine.add(s_m[v], s_l[v], s_y[v]);
+          }
+      }
+      if (u < u1 && (tid & (slices - 1)) == 0) {
+        const int64_t row = (int64_t)seg.b * a.hq + kvh * group + first + r;
+        const float d = mine.l == 0.f ? 1.f : mine.l;
+        constexpr bool kQBf16 = __is_same(TQ, __nv_bfloat16);
+        uint2 out;
+        out.x = pack2<kQBf16>(mine.y.x / d, mine.y.y / d);
+        out.y = pack2<kQBf16>(mine.y.z / d, mine.y.w / d);
+        *reinterpret_cast<uint2*>(static_cast<TQ*>(a.out) + row * D + e) = out;
+        if (a.lse && e == 0) a.lse[row] = kLn2 * (ref_of(mine.m) + log2f(mine.l));
+      }
+    }
+  }
   // sequences without tokens have no tile: their zeros are written here
-  for (int64_t b = blockIdx.x; b < a.batch; b += gridDim.x) {
+  for (int64_t b = me; b < a.batch; b += workers) {
     if (length_of(a, b) != 0) continue;
     for (int i = tid; i < a.hq * D; i += kJoinBlock)
       static_cast<TQ*>(a.out)[b * a.hq * D + i] = Pack<TQ>::from_f(0.f);
     if (a.lse)
       for (int i = tid; i < a.hq; i += kJoinBlock) a.lse[b * a.hq + i] = -INFINITY;
-  }
-  const int64_t workers = gridDim.x, me = blockIdx.x;
-  const Seg* meta = reinterpret_cast<const Seg*>(a.part);
-  const float* pm = reinterpret_cast<const float*>(meta + 2 * workers);
-  const float* po = pm + 2 * workers * kRows * 2;
-  const Seg both[2] = {meta[2 * me], meta[2 * me + 1]};
-  const int group = a.hq / a.hk;
-#pragma unroll 1
-  for (int which = 0; which < 2; ++which) {
-    const Seg seg = both[which];
-    if (seg.owner < 0) continue;
-    const int kvh = seg.hs / a.row_groups, first = (seg.hs - kvh * a.row_groups) * kRows;
-    const int rows = min(kRows, group - first), parts = seg.last - seg.owner + 1, p = (int)me - seg.owner;
-    const int u0 = rows * kUnits * p / parts, u1 = rows * kUnits * (p + 1) / parts;
-    if (u0 == u1) continue;
-    auto slot = [&](int i) { return 2ll * (seg.owner + i) + (i == 0 ? 1 : 0); };
-    const int r0 = u0 / kUnits, r1 = (u1 - 1) / kUnits;
-    __syncthreads();
-    for (int r = r0 + warp; r <= r1; r += kJoinBlock / 32) {
-      float top = -INFINITY, sum = 0.f;
-      for (int i = lane; i < parts; i += 32) top = fmaxf(top, pm[(slot(i) * kRows + r) * 2]);
-#pragma unroll
-      for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
-      for (int i = lane; i < parts; i += 32) {
-        const float2 ml = *reinterpret_cast<const float2*>(pm + (slot(i) * kRows + r) * 2);
-        sum = fmaf(ex2(ml.x - ref_of(top)), ml.y, sum);
-      }
-      sum = warp_allreduce_sum(sum);
-      if (lane == 0) {
-        s_top[r] = top;
-        s_sum[r] = sum;
-      }
-    }
-    __syncthreads();
-    const int nu = min(u1 - u0, kJoinBlock);
-    int slices = kJoinBlock / nu;
-    if (slices > parts) slices = parts;
-    for (int ub = u0; ub < u1; ub += nu) {
-      const int slice = tid / nu, u = ub + tid - slice * nu, r = u / kUnits, e = (u - r * kUnits) * 4;
-      const bool on = slice < slices && u < u1;
-      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (on) {
-        const float ref = ref_of(s_top[r]);
-#pragma unroll 4
-        for (int i = slice; i < parts; i += slices) {
-          const float f = ex2(pm[(slot(i) * kRows + r) * 2] - ref);
-          const float4 z = *reinterpret_cast<const float4*>(po + (slot(i) * kRows + r) * D + e);
-          y.x = fmaf(f, z.x, y.x);
-          y.y = fmaf(f, z.y, y.y);
-          y.z = fmaf(f, z.z, y.z);
-          y.w = fmaf(f, z.w, y.w);
-        }
-      }
-      for (int left = slices; left > 1;) {
-        const int half = (left + 1) / 2;
-        __syncthreads();
-        s_red[tid] = y;
-        __syncthreads();
-        if (slice + half < left) {
-          const float4 z = s_red[tid + half * nu];
-          y.x += z.x;
-          y.y += z.y;
-          y.z += z.z;
-          y.w += z.w;
-        }
-        left = half;
-      }
-      if (on && slice == 0) {
-        const int64_t row = (int64_t)seg.b * a.hq + kvh * group + first + r;
-        const float l = s_sum[r], d = l == 0.f ? 1.f : l;
-        constexpr bool kQBf16 = __is_same(TQ, __nv_bfloat16);
-        uint2 out;
-        out.x = pack2<kQBf16>(y.x / d, y.y / d);
-        out.y = pack2<kQBf16>(y.z / d, y.w / d);
-        *reinterpret_cast<uint2*>(static_cast<TQ*>(a.out) + row * D + e) = out;
-        if (a.lse && e == 0) a.lse[row] = kLn2 * (ref_of(s_top[r]) + log2f(l));
-      }
-    }
   }
 }
 
@@ -1024,6 +1049,10 @@ int rmsnorm_paged_attention(const rmsnorm_paged_attention_args* in, void* stream
     a.row_groups = row_groups_of(in, k);
     a.segments = a.hk * a.row_groups;
     a.whole_pages = a.page % 16 == 0;
+    unsigned shift = 0;   // ceil(log2(page))
+    while ((1ull << shift) < (unsigned)a.page) ++shift;
+    a.page_shift = shift;
+    a.page_mul = (unsigned)(((1ull << 32) * ((1ull << shift) - (unsigned)a.page)) / (unsigned)a.page + 1);
     if (in->device >= kMaxDevices || !k.ready[in->device]) {
       const cudaError_t e =
           cudaFuncSetAttribute(k.main, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem);
