@@ -306,6 +306,13 @@ struct Place {
   int b, kvh, rg, tile, tiles, len;
 };
 
+// a / b of non-negative numbers, in 32 bits where they fit (a 64-bit division takes some
+// hundred instructions, and a CTA cannot load before its first).
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  if (((a | b) >> 32) == 0) return (unsigned)a / (unsigned)b;
+  return a / b;
+}
+
 __device__ __forceinline__ int tiles_of(int64_t len) { return (int)((len + kTile - 1) / kTile); }
 
 // To the next tile; the caller knows that there is one.
@@ -371,9 +378,13 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
   Seg* meta = reinterpret_cast<Seg*>(a.part) + 2 * me;   // the segment that began before, and one left open
   if (tid < 2) meta[tid] = Seg{0, 0, -1, -1};
   if (me >= workers) return;
-  const int64_t t0 = total * me / workers, t1 = total * (me + 1) / workers;
-  // the CTA that has a tile of the row
-  auto worker_of = [&](int64_t tile) { return (int)(((tile + 1) * workers - 1) / total); };
+  // the first `more` CTAs have one tile more than the others
+  const int64_t each = quotient(total, workers), more = total - each * workers;
+  const int64_t t0 = me * each + (me < more ? me : more), t1 = t0 + each + (me < more ? 1 : 0);
+  auto worker_of = [&](int64_t tile) {
+    const int64_t line = more * (each + 1);
+    return (int)(tile < line ? quotient(tile, each + 1) : more + quotient(tile - line, each));
+  };
   if (upto - mine <= t0 && t0 < upto) {
     int64_t rest = t0 - (upto - mine);
     int64_t b = tid * per;
@@ -390,7 +401,7 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
   at.b = s_b;
   at.len = (int)length_of(a, at.b);
   at.tiles = tiles_of(at.len);
-  const int hs = (int)(s_rest / at.tiles);
+  const int hs = (int)quotient(s_rest, at.tiles);
   at.tile = (int)(s_rest - (int64_t)hs * at.tiles);
   at.kvh = hs / a.row_groups;
   at.rg = hs - at.kvh * a.row_groups;
