@@ -301,10 +301,9 @@ int rmsnorm_qk_rope_write(const rmsnorm_qk_rope_args* args, void* stream);
 /* Gradients of rmsnorm_qk_rope_forward, with g = R^T dy and inv the forward's
  * factor: dx = inv g w - x inv^3 mean(g w x), dw = sum over tokens and heads of
  * g x inv (without weights dx = g, and q, k may be NULL). dq and dk are
- * contiguous [tokens, heads, head_dim] and overlap no input; dweight holds the
- * query weight's gradient, then the key weight's ([2 * head_dim]). workspace:
- * rmsnorm_qk_rope_backward_workspace_bytes(head_dim) bytes of device memory
- * (fp32 partials of dweight, summed in a fixed order: deterministic). */
+ * contiguous [tokens, heads, head_dim] and overlap no input. workspace:
+ * rmsnorm_qk_rope_backward_workspace_bytes(head_dim) bytes of device memory, 16-byte
+ * aligned (fp32 partials of dw, summed in a fixed order: deterministic). */
 typedef struct rmsnorm_qk_rope_backward_args {
   const void* dq_out;         /* [tokens, q_heads, head_dim] */
   const void* dk_out;         /* [tokens, kv_heads, head_dim] */
@@ -312,7 +311,8 @@ typedef struct rmsnorm_qk_rope_backward_args {
   const void* k;
   void* dq;
   void* dk;
-  void* dweight;              /* NULL without weights */
+  void* dq_weight;            /* [head_dim], NULL without weights */
+  void* dk_weight;
   const void* q_weight;
   const void* k_weight;
   const float* rope;

@@ -590,6 +590,32 @@ qk_rope_backward_kernel(const __grid_constant__ QkBackArgs a) {
   }
 }
 
+// dw of both weights from the CTAs' partials ([parts][2 d]): a CTA has 32 columns, its warps
+// the parts w, w + 32, ..., added in that order and then in warp order.
+constexpr int kDwWarps = 32;
+
+template <typename T>
+__global__ void __launch_bounds__(kDwWarps * 32)
+qk_rope_dw_kernel(const float* ws, int parts, int d, T* dqw, T* dkw) {
+  __shared__ float s_sum[kDwWarps][32];
+  ptx::grid_dep_wait();
+  ptx::grid_dep_launch_dependents();
+  const int tid = thread_here(), lane = tid & 31, warp = tid >> 5;
+  const int col = blockIdx.x * 32 + lane;
+  float s = 0.f;
+  if (col < 2 * d) {
+#pragma unroll 10
+    for (int i = warp; i < parts; i += kDwWarps) s += ws[(int64_t)i * 2 * d + col];
+  }
+  s_sum[warp][lane] = s;
+  __syncthreads();
+  if (warp != 0 || col >= 2 * d) return;
+  s = 0.f;
+#pragma unroll
+  for (int w = 0; w < kDwWarps; ++w) s += s_sum[w][lane];
+  (col < d ? dqw + col : dkw + (col - d))[0] = Pack<T>::from_f(s);
+}
+
 // Lanes of a row where the vector kernels take it, else 0 (the kernels for any row):
 // units of two whole vectors on both sides of rotary_dim, at most 32 of them, and every
 // address a multiple of 16 bytes.
@@ -786,9 +812,9 @@ int rmsnorm_qk_rope_backward(const rmsnorm_qk_rope_backward_args* in, void* stre
   const bool norm = in->q_weight != nullptr;
   if (norm != (in->k_weight != nullptr))
     return refuse(RMSNORM_TP_ERR_INVALID, "%s: one of q_weight and k_weight is NULL", who);
-  if (norm && (!in->dweight || !in->workspace ||
+  if (norm && (!in->dq_weight || !in->dk_weight || !in->workspace ||
                in->workspace_bytes < (int64_t)rmsnorm_qk_rope_backward_workspace_bytes(in->head_dim)))
-    return refuse(RMSNORM_TP_ERR_INVALID, "%s: NULL dweight or a workspace of %lld bytes < %zu", who,
+    return refuse(RMSNORM_TP_ERR_INVALID, "%s: NULL dq_weight or dk_weight, or a workspace of %lld bytes < %zu", who,
                   (long long)in->workspace_bytes,
                   rmsnorm_qk_rope_backward_workspace_bytes(in->head_dim));
   const int eb = elem_bytes(in->dtype);
@@ -858,8 +884,15 @@ int rmsnorm_qk_rope_backward(const rmsnorm_qk_rope_backward_args* in, void* stre
     if (e != cudaSuccess) return launch_failed(e, who);
   }
   if (norm) {   // no tokens: zeros
-    const cudaError_t e = launch_dw_reduce(static_cast<const float*>(in->workspace), grid,
-                                           2 * (int64_t)in->head_dim, in->dweight, in->dtype, st);
+    const float* ws = static_cast<const float*>(in->workspace);
+    int d = in->head_dim;
+    void* dqw = in->dq_weight;
+    void* dkw = in->dk_weight;
+    void* args[] = {&ws, &grid, &d, &dqw, &dkw};
+    const void* fn = in->dtype == RMSNORM_TP_F32    ? reinterpret_cast<const void*>(qk_rope_dw_kernel<float>)
+                     : in->dtype == RMSNORM_TP_BF16 ? reinterpret_cast<const void*>(qk_rope_dw_kernel<__nv_bfloat16>)
+                                                    : reinterpret_cast<const void*>(qk_rope_dw_kernel<__half>);
+    const cudaError_t e = launch_dependent(fn, dim3((2 * d + 31) / 32), dim3(kDwWarps * 32), 0, args, st);
     if (e != cudaSuccess) return launch_failed(e, who);
   }
   return RMSNORM_TP_OK;

@@ -25,7 +25,7 @@ from .api import _DTYPES, _stream_of, dtype_code
 # layouts of rmsnorm_qk_rope_args, rmsnorm_qk_rope_backward_args, rmsnorm_kv_cache and
 # rmsnorm_paged_attention_args (include/rmsnorm_tp_b200.h)
 _ROPE_ARGS = struct.Struct("@9Q10q2q2Q6ifi")
-_BACK_ARGS = struct.Struct("@12Qq8q2q6ifi")
+_BACK_ARGS = struct.Struct("@13Qq8q2q6ifi")
 _CACHE = struct.Struct("@4Qq4i")
 _ATTN_ARGS = struct.Struct("@7Qq3q2q2ifi")
 
@@ -45,20 +45,54 @@ def rope_table(max_positions: int, rotary_dim: int, base: float = 10000.0,
     return torch.cat([angle.cos(), angle.sin()], 1).to(torch.float32)
 
 
-def _check_head_rows(name: str, t: torch.Tensor, like: torch.Tensor, heads: int) -> None:
-    if t.dtype != like.dtype or t.device != like.device:
+_F32, _I32, _I64 = torch.float32, torch.int32, torch.int64
+
+
+# A call's tensors are looked at attribute by attribute once, in one condition (a few
+# microseconds of host time are most of a decode-sized call); only where it fails does
+# _explain_* look again for the words.
+
+def _rows_fit(t: torch.Tensor, tokens: int, heads: int, d: int, dtype: torch.dtype, device: int) -> bool:
+    return t.dtype is dtype and t.get_device() == device and t.shape == (tokens, heads, d) and t.stride(2) == 1
+
+
+def _index_fits(t: torch.Tensor, n: int, dtype: torch.dtype, device: int) -> bool:
+    return t.dtype is dtype and t.get_device() == device and t.shape == (n,) and t.is_contiguous()
+
+
+def _weight_fits(t: torch.Tensor, d: int, dtype: torch.dtype, device: int) -> bool:
+    return t.dtype is dtype and t.get_device() == device and t.shape == (d,) and t.is_contiguous()
+
+
+def _turn_sizes(q, k, q_weight, k_weight, rope, positions):
+    """(device, dtype, tokens, q heads, kv heads, head_dim, table rows, rotary_dim) of
+    operands that fit together; AssertionError for others."""
+    qs, ks, rs = q.shape, k.shape, rope.shape
+    if len(qs) == 3 and len(ks) == 3 and len(rs) == 2:
+        tokens, hq, d = qs
+        device, dtype = q.get_device(), q.dtype
+        if (device >= 0 and dtype in _DTYPES and q.stride(2) == 1 and _rows_fit(k, tokens, ks[1], d, dtype, device)
+                and rope.dtype is _F32 and rope.get_device() == device and rope.is_contiguous()
+                and _index_fits(positions, tokens, _I64, device)
+                and (q_weight is None and k_weight is None
+                     or q_weight is not None and k_weight is not None
+                     and _weight_fits(q_weight, d, dtype, device) and _weight_fits(k_weight, d, dtype, device))):
+            return device, dtype, tokens, hq, ks[1], d, rs[0], rs[1]
+    _explain_turn(q, k, q_weight, k_weight, rope, positions)
+
+
+def _explain_rows(name: str, t: torch.Tensor, q: torch.Tensor, heads: int) -> None:
+    if t.dtype != q.dtype or t.device != q.device:
         raise AssertionError(f"{name} must have q's dtype and device, got {t.dtype} on {t.device}")
-    if t.dim() != 3 or t.shape[0] != like.shape[0] or t.shape[2] != like.shape[2] or \
-            (heads and t.shape[1] != heads):
-        raise AssertionError(f"{name} must be [tokens={like.shape[0]}, {heads or 'heads'}, "
-                             f"head_dim={like.shape[2]}], got {tuple(t.shape)}")
-    if t.stride(2) != 1:
-        raise AssertionError(f"{name}'s last dimension must have stride 1")
+    raise AssertionError(f"{name} must be [tokens={q.shape[0]}, {heads or 'heads'}, head_dim={q.shape[2]}] with "
+                         f"stride 1 in the last dimension, got {tuple(t.shape)} with strides {t.stride()}")
 
 
-def _check_turn(q: torch.Tensor, k: torch.Tensor, q_weight, k_weight, rope: torch.Tensor,
-                positions: torch.Tensor) -> None:
-    device = q.device
+def _explain_index(name: str, n: int, dtype: torch.dtype) -> None:
+    raise AssertionError(f"{name} must be contiguous {dtype} [{n}] on q's device")
+
+
+def _explain_turn(q, k, q_weight, k_weight, rope, positions) -> None:
     if not q.is_cuda:
         raise AssertionError("q must be a CUDA tensor")
     if q.dtype not in _DTYPES:
@@ -66,42 +100,18 @@ def _check_turn(q: torch.Tensor, k: torch.Tensor, q_weight, k_weight, rope: torc
     if q.dim() != 3 or q.stride(2) != 1:
         raise AssertionError("q must be [tokens, q_heads, head_dim] with stride 1 in the last "
                              f"dimension, got {tuple(q.shape)} with strides {q.stride()}")
-    _check_head_rows("k", k, q, 0)
+    tokens, _, d = q.shape
+    device = q.get_device()
+    if k.dim() != 3 or not _rows_fit(k, tokens, k.shape[1], d, q.dtype, device):
+        _explain_rows("k", k, q, 0)
     if (q_weight is None) != (k_weight is None):
         raise AssertionError("give both q_weight and k_weight, or neither (rotation without norm)")
-    if q_weight is not None:
-        for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-            if w.dtype != q.dtype or w.device != device or w.shape != q.shape[2:] or not w.is_contiguous():
-                raise AssertionError(f"{name} must be contiguous [{q.shape[2]}] with q's dtype and device")
-    if rope.dtype != torch.float32 or rope.device != device or rope.dim() != 2 or not rope.is_contiguous():
-        raise AssertionError("rope must be a contiguous float32 [max_positions, rotary_dim] on q's device")
-    _check_index("positions", positions, q, torch.int64)
-
-
-def _check_index(name: str, t: torch.Tensor, q: torch.Tensor, dtype: torch.dtype) -> None:
-    if t.dtype != dtype or t.device != q.device or t.shape != q.shape[:1] or not t.is_contiguous():
-        raise AssertionError(f"{name} must be contiguous {dtype} [{q.shape[0]}] on q's device")
-
-
-def _turn(fn, what, q, k, v, q_out, k_out, q_weight, k_weight, rope, positions, cache, slots, eps,
-          interleaved) -> None:
-    device = q.device.index
-    n = q_weight is not None
-    args = _ROPE_ARGS.pack(
-        q.data_ptr(), k.data_ptr(), 0 if v is None else v.data_ptr(), q_out.data_ptr(),
-        0 if k_out is None else k_out.data_ptr(), q_weight.data_ptr() if n else 0,
-        k_weight.data_ptr() if n else 0, rope.data_ptr(), positions.data_ptr(),
-        q.stride(0), q.stride(1), k.stride(0), k.stride(1),
-        *((0, 0) if v is None else v.stride()[:2]), q_out.stride(0), q_out.stride(1),
-        *((0, 0) if k_out is None else k_out.stride()[:2]),
-        q.shape[0], rope.shape[0], 0 if cache is None else cache._address,
-        0 if slots is None else slots.data_ptr(), q.shape[1], k.shape[1], q.shape[2], rope.shape[1],
-        _DTYPES[q.dtype], bool(interleaved), eps, device)
-    check(fn(args, _stream_of(device)), what)
-
-
-def _fresh(t: torch.Tensor) -> torch.Tensor:
-    return torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None and not _weight_fits(w, d, q.dtype, device):
+            raise AssertionError(f"{name} must be contiguous [{d}] with q's dtype and device")
+    if not _index_fits(positions, tokens, _I64, device):
+        _explain_index("positions", tokens, _I64)
+    raise AssertionError("rope must be a contiguous float32 [max_positions, rotary_dim] on q's device")
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor],
@@ -117,17 +127,25 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
     or with ``interleaved`` (2i, 2i + 1). ``positions`` int64 [tokens]; one outside the
     table makes the token's turned elements NaN. ``q_out`` / ``k_out`` receive the results
     instead of fresh tensors and may be q / k themselves. fp32 inside, rounded once."""
-    _check_turn(q, k, q_weight, k_weight, rope, positions)
+    device, dtype, tokens, hq, hk, d, most, r = _turn_sizes(q, k, q_weight, k_weight, rope, positions)
     if q_out is None:
-        q_out = _fresh(q)
-    else:
-        _check_head_rows("q_out", q_out, q, q.shape[1])
+        q_out = torch.empty_like(q)
+    elif not _rows_fit(q_out, tokens, hq, d, dtype, device):
+        _explain_rows("q_out", q_out, q, hq)
     if k_out is None:
-        k_out = _fresh(k)
-    else:
-        _check_head_rows("k_out", k_out, q, k.shape[1])
-    _turn(LIB.rmsnorm_qk_rope_forward, "rmsnorm_qk_rope_forward", q, k, None, q_out, k_out, q_weight,
-          k_weight, rope, positions, None, None, eps, interleaved)
+        k_out = torch.empty_like(k)
+    elif not _rows_fit(k_out, tokens, hk, d, dtype, device):
+        _explain_rows("k_out", k_out, q, hk)
+    a, b, _ = q.stride()
+    c, e, _ = k.stride()
+    f, g, _ = q_out.stride()
+    h, i, _ = k_out.stride()
+    args = _ROPE_ARGS.pack(
+        q.data_ptr(), k.data_ptr(), 0, q_out.data_ptr(), k_out.data_ptr(),
+        0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(),
+        rope.data_ptr(), positions.data_ptr(), a, b, c, e, 0, 0, f, g, h, i, tokens, most, 0, 0, hq, hk, d, r,
+        _DTYPES[dtype], bool(interleaved), eps, device)
+    check(LIB.rmsnorm_qk_rope_forward(args, _stream_of(device)), "rmsnorm_qk_rope_forward")
     return q_out, k_out
 
 
@@ -139,26 +157,38 @@ def qk_norm_rope_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.T
     gradients (the last two None without weights). The weights' gradients are sums over
     tokens and heads in a fixed order; over a tensor-parallel group they are this rank's
     heads' share. Capturable in a CUDA graph."""
-    _check_turn(q, k, q_weight, k_weight, rope, positions)
-    _check_head_rows("dq_out", dq_out, q, q.shape[1])
-    _check_head_rows("dk_out", dk_out, q, k.shape[1])
-    dq, dk = _fresh(q), _fresh(k)
-    n, d, device = q_weight is not None, q.shape[2], q.device.index
-    dw = ws = None
-    nbytes = 0
-    if n:
-        dw = torch.empty(2 * d, dtype=q.dtype, device=q.device)
-        nbytes = LIB.rmsnorm_qk_rope_backward_workspace_bytes(d)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    device, dtype, tokens, hq, hk, d, most, r = _turn_sizes(q, k, q_weight, k_weight, rope, positions)
+    if not _rows_fit(dq_out, tokens, hq, d, dtype, device):
+        _explain_rows("dq_out", dq_out, q, hq)
+    if not _rows_fit(dk_out, tokens, hk, d, dtype, device):
+        _explain_rows("dk_out", dk_out, q, hk)
+    dq, dk = q.new_empty(tokens, hq, d), k.new_empty(tokens, hk, d)
+    if q_weight is None:
+        dqw = dkw = None
+        weights = (0, 0, 0, 0)
+        ws_ptr = nbytes = 0
+    else:
+        dqw, dkw = torch.empty_like(q_weight), torch.empty_like(k_weight)
+        weights = (dqw.data_ptr(), dkw.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr())
+        nbytes = _backward_workspace(d)
+        ws = rope.new_empty(nbytes // 4)
+        ws_ptr = ws.data_ptr()
+    a, b, _ = dq_out.stride()
+    c, e, _ = dk_out.stride()
+    f, g, _ = q.stride()
+    h, i, _ = k.stride()
     args = _BACK_ARGS.pack(
-        dq_out.data_ptr(), dk_out.data_ptr(), q.data_ptr(), k.data_ptr(), dq.data_ptr(), dk.data_ptr(),
-        dw.data_ptr() if n else 0, q_weight.data_ptr() if n else 0, k_weight.data_ptr() if n else 0,
-        rope.data_ptr(), positions.data_ptr(), ws.data_ptr() if n else 0, nbytes,
-        dq_out.stride(0), dq_out.stride(1), dk_out.stride(0), dk_out.stride(1), q.stride(0), q.stride(1),
-        k.stride(0), k.stride(1), q.shape[0], rope.shape[0], q.shape[1], k.shape[1], d, rope.shape[1],
-        _DTYPES[q.dtype], bool(interleaved), eps, device)
+        dq_out.data_ptr(), dk_out.data_ptr(), q.data_ptr(), k.data_ptr(), dq.data_ptr(), dk.data_ptr(), *weights,
+        rope.data_ptr(), positions.data_ptr(), ws_ptr, nbytes, a, b, c, e, f, g, h, i, tokens, most, hq, hk, d, r,
+        _DTYPES[dtype], bool(interleaved), eps, device)
     check(LIB.rmsnorm_qk_rope_backward(args, _stream_of(device)), "rmsnorm_qk_rope_backward")
-    return dq, dk, dw[:d] if n else None, dw[d:] if n else None
+    return dq, dk, dqw, dkw
+
+
+@functools.lru_cache(maxsize=None)
+def _backward_workspace(head_dim: int) -> int:
+    """Bytes of the workspace (a function of the size alone)."""
+    return LIB.rmsnorm_qk_rope_backward_workspace_bytes(head_dim)
 
 
 class _QkNormRopeFunction(torch.autograd.Function):
@@ -239,11 +269,12 @@ class PagedKVCache:
         if self.head_dim % 16 or not 16 <= self.head_dim <= 256:
             raise AssertionError(f"head_dim {self.head_dim} must be a multiple of 16, at most 256")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.dtype, self.device = k.dtype, k.device
+        self.dtype, self.device, self._index = k.dtype, k.device, k.get_device()
+        self._code = _CACHE_DTYPES[k.dtype]
         self._struct = ctypes.create_string_buffer(_CACHE.pack(
             k.data_ptr(), v.data_ptr(), k_scale.data_ptr() if e4m3 else 0,
             v_scale.data_ptr() if e4m3 else 0, self.num_pages, self.page_size, self.num_kv_heads,
-            self.head_dim, _CACHE_DTYPES[k.dtype]))
+            self.head_dim, self._code))
         self._address = ctypes.addressof(self._struct)
 
     def read(self, slots: torch.Tensor, dtype: Optional[torch.dtype] = None):
@@ -252,15 +283,15 @@ class PagedKVCache:
         zeros. ``dtype`` is the cache's own unless given (bfloat16 for an e4m3 cache)."""
         if dtype is None:
             dtype = torch.bfloat16 if self.dtype == torch.float8_e4m3fn else self.dtype
-        code = dtype_code(dtype)
-        if slots.dtype != torch.int64 or slots.device != self.device or slots.dim() != 1 or \
+        code, device = dtype_code(dtype), self._index
+        if slots.dtype is not _I64 or slots.get_device() != device or slots.dim() != 1 or \
                 not slots.is_contiguous():
             raise AssertionError("slots must be contiguous int64 [count] on the cache's device")
         count = slots.shape[0]
-        k, v = (torch.empty(count, self.num_kv_heads, self.head_dim, dtype=dtype, device=self.device)
-                for _ in range(2))
+        k = torch.empty(count, self.num_kv_heads, self.head_dim, dtype=dtype, device=self.device)
+        v = torch.empty_like(k)
         check(LIB.rmsnorm_kv_read(self._address, k.data_ptr(), v.data_ptr(), slots.data_ptr(), count, code,
-                                  self.device.index, _stream_of(self.device.index)), "rmsnorm_kv_read")
+                                  device, _stream_of(device)), "rmsnorm_kv_read")
         return k, v
 
 
@@ -272,20 +303,30 @@ def qk_norm_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weig
     queries. ``slots`` int64 [tokens] are distinct within a call; a token whose slot lies
     outside the cache (-1: padding) leaves the cache as it is. The cache has q's dtype, or
     float8_e4m3fn (quantised from the fp32 values)."""
-    _check_turn(q, k, q_weight, k_weight, rope, positions)
-    _check_head_rows("v", v, q, k.shape[1])
-    _check_index("slots", slots, q, torch.int64)
-    if cache.device != q.device or cache.num_kv_heads != k.shape[1] or cache.head_dim != q.shape[2]:
+    device, dtype, tokens, hq, hk, d, most, r = _turn_sizes(q, k, q_weight, k_weight, rope, positions)
+    if not _rows_fit(v, tokens, hk, d, dtype, device):
+        _explain_rows("v", v, q, hk)
+    if not _index_fits(slots, tokens, _I64, device):
+        _explain_index("slots", tokens, _I64)
+    if cache._index != device or cache.num_kv_heads != hk or cache.head_dim != d:
         raise AssertionError(f"the cache holds {cache.num_kv_heads} heads of {cache.head_dim} on "
-                             f"{cache.device}, the call has {k.shape[1]} of {q.shape[2]} on {q.device}")
-    if cache.dtype != q.dtype and cache.dtype != torch.float8_e4m3fn:
-        raise AssertionError(f"a {cache.dtype} cache does not take {q.dtype}")
+                             f"{cache.device}, the call has {hk} of {d} on {q.device}")
+    if cache.dtype is not dtype and cache._code != _lib.KV_E4M3:
+        raise AssertionError(f"a {cache.dtype} cache does not take {dtype}")
     if q_out is None:
-        q_out = _fresh(q)
-    else:
-        _check_head_rows("q_out", q_out, q, q.shape[1])
-    _turn(LIB.rmsnorm_qk_rope_write, "rmsnorm_qk_rope_write", q, k, v, q_out, None, q_weight, k_weight,
-          rope, positions, cache, slots, eps, interleaved)
+        q_out = torch.empty_like(q)
+    elif not _rows_fit(q_out, tokens, hq, d, dtype, device):
+        _explain_rows("q_out", q_out, q, hq)
+    a, b, _ = q.stride()
+    c, e, _ = k.stride()
+    f, g, _ = v.stride()
+    h, i, _ = q_out.stride()
+    args = _ROPE_ARGS.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), 0,
+        0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(),
+        rope.data_ptr(), positions.data_ptr(), a, b, c, e, f, g, h, i, 0, 0, tokens, most, cache._address,
+        slots.data_ptr(), hq, hk, d, r, _DTYPES[dtype], bool(interleaved), eps, device)
+    check(LIB.rmsnorm_qk_rope_write(args, _stream_of(device)), "rmsnorm_qk_rope_write")
     return q_out
 
 
@@ -325,33 +366,36 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tens
     exponentials [batch, q_heads]. A sequence without tokens gives zeros and -inf; pages
     outside the cache are left out, lengths cut to max_pages * page_size. ``scale`` is
     head_dim^-0.5 unless given."""
-    if not q.is_cuda or q.dim() != 3 or q.stride(2) != 1:
+    qs, device, q_dtype = q.shape, q.get_device(), q.dtype
+    if device < 0 or len(qs) != 3 or q.stride(2) != 1:
         raise AssertionError("q must be a CUDA tensor [batch, q_heads, head_dim] with stride 1 in the last "
-                             f"dimension, got {tuple(q.shape)}")
-    if q.dtype not in _DTYPES:
-        raise AssertionError(f"unsupported dtype {q.dtype}; expected float32, bfloat16 or float16")
-    batch, heads, d = q.shape
-    if cache.device != q.device or d != cache.head_dim or heads % cache.num_kv_heads:
+                             f"dimension, got {tuple(qs)}")
+    if q_dtype not in _DTYPES:
+        raise AssertionError(f"unsupported dtype {q_dtype}; expected float32, bfloat16 or float16")
+    batch, heads, d = qs
+    if cache._index != device or d != cache.head_dim or heads % cache.num_kv_heads:
         raise AssertionError(f"q has {heads} heads of {d} on {q.device}, the cache {cache.num_kv_heads} of "
                              f"{cache.head_dim} on {cache.device}")
-    if cache.dtype != q.dtype and cache.dtype != torch.float8_e4m3fn:
-        raise AssertionError(f"a {cache.dtype} cache does not serve {q.dtype} queries")
-    if page_table.dtype != torch.int32 or page_table.device != q.device or page_table.dim() != 2 or \
-            page_table.shape[0] != batch or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+    if cache.dtype is not q_dtype and cache._code != _lib.KV_E4M3:
+        raise AssertionError(f"a {cache.dtype} cache does not serve {q_dtype} queries")
+    ts, tst = page_table.shape, page_table.stride()
+    if page_table.dtype is not _I32 or page_table.get_device() != device or len(ts) != 2 or ts[0] != batch or \
+            (ts[1] > 1 and tst[1] != 1):
         raise AssertionError(f"page_table must be int32 [{batch}, max_pages] on q's device, rows in one piece")
-    _check_index("seq_lens", seq_lens, q, torch.int32)
+    if not _index_fits(seq_lens, batch, _I32, device):
+        _explain_index("seq_lens", batch, _I32)
     if out is None:
-        out = _fresh(q)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
+        out = q.new_empty(batch, heads, d)
+    elif out.shape != qs or out.dtype is not q_dtype or out.get_device() != device or not out.is_contiguous():
         raise AssertionError("out must be contiguous with q's shape, dtype and device")
-    lse = torch.empty(batch, heads, dtype=torch.float32, device=q.device) if return_lse else None
-    max_pages, device, dtype = page_table.shape[1], q.device.index, _DTYPES[q.dtype]
-    nbytes = _attention_workspace(cache.num_pages, cache.page_size, cache.num_kv_heads, d,
-                                  _CACHE_DTYPES[cache.dtype], batch, max_pages, heads, dtype, device)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-    args = _attention_args(q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0,
-                           page_table.data_ptr(), seq_lens.data_ptr(), ws.data_ptr(), nbytes,
-                           cache._address, q.stride()[:2], page_table.stride(0), batch, max_pages, heads,
-                           dtype, d ** -0.5 if scale is None else scale, device)
+    lse = torch.empty(batch, heads, dtype=_F32, device=q.device) if return_lse else None
+    dtype = _DTYPES[q_dtype]
+    nbytes = _attention_workspace(cache.num_pages, cache.page_size, cache.num_kv_heads, d, cache._code, batch,
+                                  ts[1], heads, dtype, device)
+    ws = q.new_empty(nbytes // 2)      # 16-bit or wider elements: at least nbytes
+    a, b, _ = q.stride()
+    args = _ATTN_ARGS.pack(cache._address, q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0,
+                           page_table.data_ptr(), seq_lens.data_ptr(), ws.data_ptr(), nbytes, a, b, tst[0],
+                           batch, ts[1], heads, dtype, d ** -0.5 if scale is None else scale, device)
     check(LIB.rmsnorm_paged_attention(args, _stream_of(device)), "rmsnorm_paged_attention")
     return (out, lse) if return_lse else out
