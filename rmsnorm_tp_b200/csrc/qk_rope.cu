@@ -45,7 +45,7 @@ struct QkBackArgs {
   const void* kw;
   const float* rope;
   const int64_t* positions;
-  float* ws;             // [grid][2 * d] fp32 partials of dweight
+  float* ws;             // [grid][d] fp32 partials of dw: the queries' CTAs, then the keys'
   int64_t tokens, max_pos;
   int hq, hk, d, r;
   int interleaved, norm;
@@ -172,91 +172,90 @@ __global__ void __launch_bounds__(kBlock) qk_rope_any_kernel(const __grid_consta
   if (lane == 0) (is_v ? a.vs : a.ks)[at] = most / kE4M3Max;
 }
 
-// One CTA per 1/gridDim-th of the rows of each operand; every lane adds its
-// pairs' dw into its warp's own slice of shared memory, the warps' slices are
-// added in warp order.
+// CTAs [0, q_blocks) share the queries' rows, the others the keys'; every lane adds its
+// pairs' dw into its warp's own slice of shared memory, the warps' slices are added in
+// warp order.
 template <typename T>
 __global__ void __launch_bounds__(kBlock)
-qk_rope_backward_any_kernel(const __grid_constant__ QkBackArgs a) {
+qk_rope_backward_any_kernel(const __grid_constant__ QkBackArgs a, int q_blocks) {
   extern __shared__ float dw[];     // [kWarps][d]
   ptx::grid_dep_wait();
   const int tid = thread_here(), lane = tid & 31, warp = tid >> 5;
   const int pairs = a.r / 2 + (a.d - a.r + 1) / 2;
+  const bool is_q = (int)blockIdx.x < q_blocks;
+  const int blocks = is_q ? q_blocks : gridDim.x - q_blocks, block = is_q ? blockIdx.x : blockIdx.x - q_blocks;
   float* mine = dw + warp * a.d;
-  for (int part = 0; part < 2; ++part) {
-    const int heads = part == 0 ? a.hq : a.hk;
-    const Rows& xr = part == 0 ? a.q : a.k;
-    const Rows& gr = part == 0 ? a.dqo : a.dko;
-    T* dx = static_cast<T*>(part == 0 ? a.dq : a.dk);
-    const T* w = static_cast<const T*>(part == 0 ? a.qw : a.kw);
-    if (a.norm)
-      for (int i = lane; i < a.d; i += 32) mine[i] = 0.f;
-    __syncwarp();
-    const int64_t rows = a.tokens * heads, step = (int64_t)gridDim.x * kWarps;
-    for (int64_t row = (int64_t)blockIdx.x * kWarps + warp; row < rows; row += step) {
-      const int64_t t = row / heads;
-      const int h = (int)(row - t * heads);
-      const T* x = a.norm ? static_cast<const T*>(xr.p) + t * xr.st + h * xr.sh : nullptr;
-      const T* dy = static_cast<const T*>(gr.p) + t * gr.st + h * gr.sh;
-      const int64_t pos = a.positions[t];
-      const bool known = pos >= 0 && pos < a.max_pos;
-      const float* turn = a.rope + (known ? pos : 0) * a.r;
-      auto value = [&](int u, int& ia, int& ib, float& ga, float& gb) {
-        pair_of(u, a.d, a.r, a.interleaved, ia, ib);
-        ga = Pack<T>::to_f(dy[ia]);
-        gb = ib >= 0 ? Pack<T>::to_f(dy[ib]) : 0.f;
-        if (u < a.r / 2) {
-          const float c = known ? turn[u] : quiet_nan(), s = known ? turn[a.r / 2 + u] : quiet_nan();
-          const float p = ga * c + gb * s;
-          gb = gb * c - ga * s;
-          ga = p;
-        }
-      };
-      float inv = 1.f, k = 0.f;
-      if (a.norm) {
-        float ss = 0.f, sg = 0.f;
-        for (int u = lane; u < pairs; u += 32) {
-          int ia, ib;
-          float ga, gb;
-          value(u, ia, ib, ga, gb);
-          const float xa = Pack<T>::to_f(x[ia]), xb = ib >= 0 ? Pack<T>::to_f(x[ib]) : 0.f;
-          const float wa = Pack<T>::to_f(w[ia]), wb = ib >= 0 ? Pack<T>::to_f(w[ib]) : 0.f;
-          ss = fmaf(xa, xa, fmaf(xb, xb, ss));
-          sg = fmaf(ga * wa, xa, fmaf(gb * wb, xb, sg));
-        }
-        ss = warp_allreduce_sum(ss);
-        sg = warp_allreduce_sum(sg);
-        inv = rsqrtf(ss / (float)a.d + a.eps);
-        k = inv * inv * inv * (sg / (float)a.d);
+  const int heads = is_q ? a.hq : a.hk;
+  const Rows& xr = is_q ? a.q : a.k;
+  const Rows& gr = is_q ? a.dqo : a.dko;
+  T* dx = static_cast<T*>(is_q ? a.dq : a.dk);
+  const T* w = static_cast<const T*>(is_q ? a.qw : a.kw);
+  if (a.norm)
+    for (int i = lane; i < a.d; i += 32) mine[i] = 0.f;
+  __syncwarp();
+  const int64_t rows = a.tokens * heads, step = (int64_t)blocks * kWarps;
+  for (int64_t row = (int64_t)block * kWarps + warp; row < rows; row += step) {
+    const int64_t t = row / heads;
+    const int h = (int)(row - t * heads);
+    const T* x = a.norm ? static_cast<const T*>(xr.p) + t * xr.st + h * xr.sh : nullptr;
+    const T* dy = static_cast<const T*>(gr.p) + t * gr.st + h * gr.sh;
+    const int64_t pos = a.positions[t];
+    const bool known = pos >= 0 && pos < a.max_pos;
+    const float* turn = a.rope + (known ? pos : 0) * a.r;
+    auto value = [&](int u, int& ia, int& ib, float& ga, float& gb) {
+      pair_of(u, a.d, a.r, a.interleaved, ia, ib);
+      ga = Pack<T>::to_f(dy[ia]);
+      gb = ib >= 0 ? Pack<T>::to_f(dy[ib]) : 0.f;
+      if (u < a.r / 2) {
+        const float c = known ? turn[u] : quiet_nan(), s = known ? turn[a.r / 2 + u] : quiet_nan();
+        const float p = ga * c + gb * s;
+        gb = gb * c - ga * s;
+        ga = p;
       }
-      T* y = dx + row * a.d;
+    };
+    float inv = 1.f, k = 0.f;
+    if (a.norm) {
+      float ss = 0.f, sg = 0.f;
       for (int u = lane; u < pairs; u += 32) {
         int ia, ib;
         float ga, gb;
         value(u, ia, ib, ga, gb);
-        if (!a.norm) {
-          y[ia] = Pack<T>::from_f(ga);
-          if (ib >= 0) y[ib] = Pack<T>::from_f(gb);
-          continue;
-        }
-        const float xa = Pack<T>::to_f(x[ia]);
-        y[ia] = Pack<T>::from_f(inv * ga * Pack<T>::to_f(w[ia]) - xa * k);
-        mine[ia] += ga * xa * inv;
-        if (ib >= 0) {
-          const float xb = Pack<T>::to_f(x[ib]);
-          y[ib] = Pack<T>::from_f(inv * gb * Pack<T>::to_f(w[ib]) - xb * k);
-          mine[ib] += gb * xb * inv;
-        }
+        const float xa = Pack<T>::to_f(x[ia]), xb = ib >= 0 ? Pack<T>::to_f(x[ib]) : 0.f;
+        const float wa = Pack<T>::to_f(w[ia]), wb = ib >= 0 ? Pack<T>::to_f(w[ib]) : 0.f;
+        ss = fmaf(xa, xa, fmaf(xb, xb, ss));
+        sg = fmaf(ga * wa, xa, fmaf(gb * wb, xb, sg));
+      }
+      ss = warp_allreduce_sum(ss);
+      sg = warp_allreduce_sum(sg);
+      inv = rsqrtf(ss / (float)a.d + a.eps);
+      k = inv * inv * inv * (sg / (float)a.d);
+    }
+    T* y = dx + row * a.d;
+    for (int u = lane; u < pairs; u += 32) {
+      int ia, ib;
+      float ga, gb;
+      value(u, ia, ib, ga, gb);
+      if (!a.norm) {
+        y[ia] = Pack<T>::from_f(ga);
+        if (ib >= 0) y[ib] = Pack<T>::from_f(gb);
+        continue;
+      }
+      const float xa = Pack<T>::to_f(x[ia]);
+      y[ia] = Pack<T>::from_f(inv * ga * Pack<T>::to_f(w[ia]) - xa * k);
+      mine[ia] += ga * xa * inv;
+      if (ib >= 0) {
+        const float xb = Pack<T>::to_f(x[ib]);
+        y[ib] = Pack<T>::from_f(inv * gb * Pack<T>::to_f(w[ib]) - xb * k);
+        mine[ib] += gb * xb * inv;
       }
     }
-    if (!a.norm) continue;
-    __syncthreads();
-    for (int i = tid; i < a.d; i += kBlock) {
-      float s = 0.f;
-      for (int v = 0; v < kWarps; ++v) s += dw[v * a.d + i];
-      a.ws[((int64_t)blockIdx.x * 2 + part) * a.d + i] = s;
-    }
-    __syncthreads();
+  }
+  if (!a.norm) return;
+  __syncthreads();
+  for (int i = tid; i < a.d; i += kBlock) {
+    float s = 0.f;
+    for (int v = 0; v < kWarps; ++v) s += dw[v * a.d + i];
+    a.ws[(int64_t)blockIdx.x * a.d + i] = s;
   }
 }
 
@@ -286,45 +285,103 @@ struct UnitOf {
   }
 };
 
+// Two fp32 in one register pair: sm_100 multiplies and adds them in one instruction.
+using f2 = unsigned long long;
+__device__ __forceinline__ f2 f2_of(float lo, float hi) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void f2_to(f2 v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ float f2_sum(f2 v) {
+  float a, b;
+  f2_to(v, a, b);
+  return a + b;
+}
+
+// 16 bytes of T as pairs of fp32.
+template <typename T>
+struct Vec {
+  static constexpr int E = Pack<T>::kE, N = E / 2;
+  f2 v[N];
+  __device__ __forceinline__ void from(const uint4& x) {
+    float f[E];
+    Pack<T>::unpack(x, f);
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = f2_of(f[2 * i], f[2 * i + 1]);
+  }
+  __device__ __forceinline__ uint4 to() const {
+    float f[E];
+    floats(f);
+    return Pack<T>::pack(f);
+  }
+  __device__ __forceinline__ void floats(float (&f)[E]) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) f2_to(v[i], f[2 * i], f[2 * i + 1]);
+  }
+};
+
 // Cosines and sines of a unit: table columns [j E, j E + E) and rotary_dim / 2 on, in
-// either pairing.
+// either pairing (neighbours: (sine, -sine) and (cosine, cosine) of one pair in a pair).
 template <typename T>
 struct Turn {
-  static constexpr int E = Pack<T>::kE;
-  float c[E], s[E];
+  static constexpr int E = Pack<T>::kE, N = E / 2;
+  f2 c[N], s[N];
   __device__ __forceinline__ void load(const float* rope, int64_t pos, int64_t max_pos, int r, int j) {
     const bool known = pos >= 0 && pos < max_pos;
-    const float4* row = reinterpret_cast<const float4*>(rope + (known ? pos : 0) * r + j * E);
-    const float4* row2 = reinterpret_cast<const float4*>(rope + (known ? pos : 0) * r + r / 2 + j * E);
+    const float* row = rope + (known ? pos : 0) * r + j * E;
 #pragma unroll
     for (int i = 0; i < E / 4; ++i) {
-      const float4 a = __ldg(row + i), b = __ldg(row2 + i);
-      c[4 * i] = a.x, c[4 * i + 1] = a.y, c[4 * i + 2] = a.z, c[4 * i + 3] = a.w;
-      s[4 * i] = b.x, s[4 * i + 1] = b.y, s[4 * i + 2] = b.z, s[4 * i + 3] = b.w;
+      const float4 a = __ldg(reinterpret_cast<const float4*>(row) + i);
+      const float4 b = __ldg(reinterpret_cast<const float4*>(row + r / 2) + i);
+      c[2 * i] = f2_of(a.x, a.y), c[2 * i + 1] = f2_of(a.z, a.w);
+      s[2 * i] = f2_of(b.x, b.y), s[2 * i + 1] = f2_of(b.z, b.w);
     }
     if (!known)
 #pragma unroll
-      for (int i = 0; i < E; ++i) c[i] = s[i] = quiet_nan();
+      for (int i = 0; i < N; ++i) c[i] = s[i] = f2_of(quiet_nan(), quiet_nan());
   }
   // (a, b) turned by the angle (back: by its negative).
   template <bool kBack>
-  __device__ __forceinline__ void apply(float (&a)[E], float (&b)[E], int interleaved) const {
+  __device__ __forceinline__ void apply(Vec<T>& a, Vec<T>& b, int interleaved) const {
+    const f2 sign = kBack ? f2_of(1.f, -1.f) : f2_of(-1.f, 1.f);
     if (!interleaved) {
+      const f2 minus = f2_of(-1.f, -1.f);
 #pragma unroll
-      for (int i = 0; i < E; ++i) pair<kBack>(a[i], b[i], c[i], s[i]);
+      for (int i = 0; i < N; ++i) {
+        const f2 as = mul2(a.v[i], s[i]), bs = mul2(b.v[i], s[i]);
+        a.v[i] = fma2(a.v[i], c[i], kBack ? bs : mul2(bs, minus));
+        b.v[i] = fma2(b.v[i], c[i], kBack ? mul2(as, minus) : as);
+      }
     } else {
 #pragma unroll
-      for (int i = 0; i < E / 2; ++i) {
-        pair<kBack>(a[2 * i], a[2 * i + 1], c[i], s[i]);
-        pair<kBack>(b[2 * i], b[2 * i + 1], c[E / 2 + i], s[E / 2 + i]);
+      for (int i = 0; i < N; ++i) {
+        neighbours(a.v[i], i, sign);
+        neighbours(b.v[i], N + i, sign);
       }
     }
   }
-  template <bool kBack>
-  static __device__ __forceinline__ void pair(float& a, float& b, float c, float s) {
-    const float x = kBack ? a * c + b * s : a * c - b * s;
-    b = kBack ? b * c - a * s : a * s + b * c;
-    a = x;
+  // pair k of the unit, whose cosine and sine are half of c[k / 2] and s[k / 2]
+  __device__ __forceinline__ void neighbours(f2& v, int k, f2 sign) const {
+    float c0, c1, s0, s1, x, y;
+    f2_to(c[k / 2], c0, c1);
+    f2_to(s[k / 2], s0, s1);
+    f2_to(v, x, y);
+    const float cc = k & 1 ? c1 : c0, ss = k & 1 ? s1 : s0;
+    // (x c -+ y s, y c +- x s)
+    v = fma2(f2_of(y, x), mul2(f2_of(ss, ss), sign), mul2(v, f2_of(cc, cc)));
   }
 };
 
@@ -341,279 +398,324 @@ __device__ __forceinline__ float lanes_max(float v) {
   return v;
 }
 
-// Rows are numbered over tokens, then heads (q, k, v); a warp takes `run` groups of
-// 32 / L neighbouring rows.
-template <typename T, int L, bool kWrite>
-__global__ void __launch_bounds__(kBlock) qk_rope_kernel(const __grid_constant__ QkArgs a, int run) {
-  constexpr int E = Pack<T>::kE, kRows = 32 / L;
-  ptx::grid_dep_wait();
-  ptx::grid_dep_launch_dependents();
-  const int tid = thread_here(), lane = tid & 31, j = lane % L;
-  const UnitOf<T> u(j, a.d, a.r, a.interleaved);
-  const int heads = a.hq + a.hk + (kWrite ? a.hk : 0);
-  const int64_t rows = a.tokens * heads;
-  int64_t row = ((int64_t)blockIdx.x * kWarps + (tid >> 5)) * run * kRows + lane / L;
-  int64_t t = (unsigned)row / (unsigned)heads;   // at most 2^31 rows and a CTA's more
-  int h = (int)(row - t * heads);
-  uint4 wq[2] = {}, wk[2] = {};
-  if (a.norm && u.on) {
-    wq[0] = ptx::ld_cached_v4(static_cast<const T*>(a.qw) + u.ea);
-    wq[1] = ptx::ld_cached_v4(static_cast<const T*>(a.qw) + u.eb);
-    wk[0] = ptx::ld_cached_v4(static_cast<const T*>(a.kw) + u.ea);
-    wk[1] = ptx::ld_cached_v4(static_cast<const T*>(a.kw) + u.eb);
+// Rows of one operand ([tokens, heads] numbered token by token) on their way through a
+// warp: a lane walks down every (32 / L)-th row by a pointer, made anew where the token
+// changes.
+template <typename T, int kRows>
+struct Walk {
+  unsigned row, end = 0;                 // end: first row of the next token
+  const T* p = nullptr;
+  __device__ __forceinline__ explicit Walk(unsigned first) : row(first) {}
+  // Whether the row is a new token's (its t and h are set then); p as for element e0.
+  __device__ __forceinline__ bool enter(const Rows& in, unsigned heads, int e0, unsigned& t, unsigned& h) {
+    if (row < end) return false;
+    t = row / heads;
+    h = row - t * heads;
+    end = (t + 1) * heads;
+    p = static_cast<const T*>(in.p) + t * in.st + (int64_t)h * in.sh + e0;
+    return true;
   }
-  auto fetch = [&](int64_t t, int h, bool live, uint4 (&x)[2]) {
-    if (!live || !u.on) {
-      x[0] = x[1] = make_uint4(0u, 0u, 0u, 0u);
-      return;
-    }
-    const T* p;
-    if (h < a.hq) p = static_cast<const T*>(a.q.p) + t * a.q.st + h * a.q.sh;
-    else if (!kWrite || h < a.hq + a.hk) p = static_cast<const T*>(a.k.p) + t * a.k.st + (h - a.hq) * a.k.sh;
-    else p = static_cast<const T*>(a.v.p) + t * a.v.st + (h - a.hq - a.hk) * a.v.sh;
-    x[0] = ptx::ld_stream_v4(p + u.ea);
-    x[1] = ptx::ld_stream_v4(p + u.eb);
-  };
-  Turn<T> turn;
-  int64_t turn_of = -1, slot = -1;
-  uint4 next[2];
-  fetch(t, h, row < rows, next);
-#pragma unroll 1
-  for (int i = 0; i < run; ++i) {
-    const bool live = row < rows;
-    if (!__any_sync(0xFFFFFFFFu, live)) break;
-    if (live && t != turn_of) {
-      turn_of = t;
-      const int64_t pos = a.positions[t];
-      if (kWrite) slot = a.slots[t];
-      if (u.turned) turn.load(a.rope, pos, a.max_pos, a.r, j);
-    }
-    const uint4 x[2] = {next[0], next[1]};
-    const int64_t t_now = t;
-    const int h_now = h;
+  __device__ __forceinline__ void step(int64_t stride) {
     row += kRows;
-    h += kRows;
-    while (h >= heads) {
-      h -= heads;
-      ++t;
-    }
-    if (i + 1 < run) fetch(t, h, row < rows, next);
+    p += stride;
+  }
+};
 
-    const bool is_q = h_now < a.hq, is_v = kWrite && h_now >= a.hq + a.hk;
-    float ya[E], yb[E];
-    Pack<T>::unpack(x[0], ya);
-    Pack<T>::unpack(x[1], yb);
-    if (a.norm) {
-      float sa = 0.f, sb = 0.f;
+// What becomes of an operand's rows.
+enum Out { kRowsOut, kCacheOut };
+
+// `run` groups of 32 / L rows of one operand. kTurned: normed and turned (else as they are:
+// the values on their way to the cache); kDeep rows are in flight ahead.
+template <typename T, int L, bool kTurned, int kOut>
+__device__ __forceinline__ void qk_rope_rows(const QkArgs& a, const Rows& in, const OutRows& out, const void* w,
+                                             void* cache, float* scales, unsigned heads, unsigned warp, int lane,
+                                             int run) {
+  constexpr int E = Pack<T>::kE, N = E / 2, kRows = 32 / L, kDeep = 2;
+  const int j = lane % L;
+  const UnitOf<T> u(j, a.d, a.r, a.interleaved);
+  const unsigned rows = (unsigned)a.tokens * heads;   // at most 2^31
+  const unsigned first = warp * (unsigned)run * kRows + lane / L;
+  const int64_t in_step = kRows * in.sh;
+  const int across = u.eb - u.ea;
+  Walk<T, kRows> ahead(first);
+  auto fetch = [&](uint4 (&x)[2]) {
+    x[0] = x[1] = make_uint4(0u, 0u, 0u, 0u);
+    if (ahead.row >= rows || !u.on) return;
+    unsigned t, h;
+    ahead.enter(in, heads, u.ea, t, h);
+    x[0] = ptx::ld_stream_v4(ahead.p);
+    x[1] = ptx::ld_stream_v4(ahead.p + across);
+    ahead.step(in_step);
+  };
+  uint4 next[kDeep][2];
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        sa = fmaf(ya[e], ya[e], sa);
-        sb = fmaf(yb[e], yb[e], sb);
-      }
-      const float inv = rsqrtf(lanes_sum<L>(sa + sb) / (float)a.d + a.eps);
-      if (!is_v) {
-        float wa[E], wb[E];
-        Pack<T>::unpack(is_q ? wq[0] : wk[0], wa);
-        Pack<T>::unpack(is_q ? wq[1] : wk[1], wb);
+  for (int i = 0; i < kDeep; ++i) fetch(next[i]);
+  Vec<T> wa, wb;
+  Turn<T> turn;
+  if (kTurned && a.norm && u.on) {
+    wa.from(ptx::ld_cached_v4(static_cast<const T*>(w) + u.ea));
+    wb.from(ptx::ld_cached_v4(static_cast<const T*>(w) + u.eb));
+  }
+  const float rd = 1.f / (float)a.d;
+  unsigned row = first, end = 0;
+  T* to = nullptr;
+  int64_t at = 0;                        // cache row
+  bool keep = kOut == kRowsOut;
+  const int64_t to_step = kOut == kRowsOut ? kRows * out.sh : (int64_t)kRows * a.page * a.d;
+#pragma unroll 1
+  for (int i = 0; i < run; i += kDeep) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          ya[e] = (ya[e] * inv) * wa[e];
-          yb[e] = (yb[e] * inv) * wb[e];
-        }
-      }
-    }
-    if (u.turned && !is_v) turn.template apply<false>(ya, yb, a.interleaved);
-    if (!kWrite || is_q) {
-      if (live && u.on) {
-        T* y = is_q ? static_cast<T*>(a.qo.p) + t_now * a.qo.st + h_now * a.qo.sh
-                    : static_cast<T*>(a.ko.p) + t_now * a.ko.st + (h_now - a.hq) * a.ko.sh;
-        ptx::st_v4(y + u.ea, Pack<T>::pack(ya));
-        ptx::st_v4(y + u.eb, Pack<T>::pack(yb));
-      }
-      if (!kWrite) continue;
-    }
-    if constexpr (kWrite) {
-      const bool keep = live && !is_q && slot >= 0 && slot < a.num_slots;
-      const int64_t at = keep ? cache_row(slot, is_v ? h_now - a.hq - a.hk : h_now - a.hq, a) : 0;
-      void* cache = is_v ? a.vc : a.kc;
-      if (!a.e4m3) {
-        if (keep && u.on) {
-          T* y = static_cast<T*>(cache) + at * a.d;
-          ptx::st_v4(y + u.ea, Pack<T>::pack(ya));
-          ptx::st_v4(y + u.eb, Pack<T>::pack(yb));
-        }
-        continue;
-      }
-      if (!__any_sync(0xFFFFFFFFu, keep)) continue;
-      float most = kE4M3Floor;
-#pragma unroll
-      for (int e = 0; e < E; ++e) most = fmaxf(most, fmaxf(fabsf(ya[e]), fabsf(yb[e])));
-      most = lanes_max<L>(most);
-      if (keep && u.on) {
-        const float to = kE4M3Max / most;
-        unsigned char* y = static_cast<unsigned char*>(cache) + at * a.d;
-        uint32_t ca[E / 4], cb[E / 4];
-#pragma unroll
-        for (int e = 0; e < E / 4; ++e) {
-          ca[e] = e4m3x2_of(ya[4 * e] * to, ya[4 * e + 1] * to) |
-                  (uint32_t)e4m3x2_of(ya[4 * e + 2] * to, ya[4 * e + 3] * to) << 16;
-          cb[e] = e4m3x2_of(yb[4 * e] * to, yb[4 * e + 1] * to) |
-                  (uint32_t)e4m3x2_of(yb[4 * e + 2] * to, yb[4 * e + 3] * to) << 16;
-        }
-        if constexpr (E == 8) {
-          *reinterpret_cast<uint2*>(y + u.ea) = make_uint2(ca[0], ca[1]);
-          *reinterpret_cast<uint2*>(y + u.eb) = make_uint2(cb[0], cb[1]);
+    for (int k = 0; k < kDeep; ++k) {
+      if (i + k >= run || !__any_sync(0xFFFFFFFFu, row < rows)) return;
+      const bool live = row < rows;
+      Vec<T> ya, yb;
+      ya.from(next[k][0]);
+      yb.from(next[k][1]);
+      if (i + k + kDeep < run) fetch(next[k]);
+      if (row >= end && live) {
+        const unsigned t = row / heads, h = row - t * heads;
+        end = row - h + heads;
+        if (kTurned && u.turned) turn.load(a.rope, a.positions[t], a.max_pos, a.r, j);
+        if constexpr (kOut == kRowsOut) {
+          to = static_cast<T*>(out.p) + t * out.st + (int64_t)h * out.sh + u.ea;
         } else {
-          *reinterpret_cast<uint32_t*>(y + u.ea) = ca[0];
-          *reinterpret_cast<uint32_t*>(y + u.eb) = cb[0];
+          const int64_t slot = a.slots[t];
+          keep = slot >= 0 && slot < a.num_slots;
+          at = keep ? cache_row(slot, h, a) : 0;
+          to = static_cast<T*>(cache) + at * a.d + u.ea;
         }
-        if (j == 0) (is_v ? a.vs : a.ks)[at] = most / kE4M3Max;
       }
+      if (kTurned && a.norm) {
+        f2 sa = mul2(ya.v[0], ya.v[0]), sb = mul2(yb.v[0], yb.v[0]);
+#pragma unroll
+        for (int e = 1; e < N; ++e) {
+          sa = fma2(ya.v[e], ya.v[e], sa);
+          sb = fma2(yb.v[e], yb.v[e], sb);
+        }
+        const float inv = rsqrtf(lanes_sum<L>(f2_sum(sa) + f2_sum(sb)) * rd + a.eps);
+        const f2 inv2 = f2_of(inv, inv);
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+          ya.v[e] = mul2(mul2(ya.v[e], inv2), wa.v[e]);
+          yb.v[e] = mul2(mul2(yb.v[e], inv2), wb.v[e]);
+        }
+      }
+      if (kTurned && u.turned) turn.template apply<false>(ya, yb, a.interleaved);
+      if (kOut == kRowsOut || !a.e4m3) {
+        if (live && keep && u.on) {
+          ptx::st_v4(to, ya.to());
+          ptx::st_v4(to + across, yb.to());
+        }
+      } else {
+        float fa[E], fb[E];
+        ya.floats(fa);
+        yb.floats(fb);
+        float most = kE4M3Floor;
+#pragma unroll
+        for (int e = 0; e < E; ++e) most = fmaxf(most, fmaxf(fabsf(fa[e]), fabsf(fb[e])));
+        most = lanes_max<L>(most);
+        if (live && keep && u.on) {
+          const float up = kE4M3Max / most;
+          unsigned char* y = static_cast<unsigned char*>(cache) + at * a.d + u.ea;
+          uint32_t ca[E / 4], cb[E / 4];
+#pragma unroll
+          for (int e = 0; e < E / 4; ++e) {
+            ca[e] = e4m3x2_of(fa[4 * e] * up, fa[4 * e + 1] * up) |
+                    (uint32_t)e4m3x2_of(fa[4 * e + 2] * up, fa[4 * e + 3] * up) << 16;
+            cb[e] = e4m3x2_of(fb[4 * e] * up, fb[4 * e + 1] * up) |
+                    (uint32_t)e4m3x2_of(fb[4 * e + 2] * up, fb[4 * e + 3] * up) << 16;
+          }
+          if constexpr (E == 8) {
+            *reinterpret_cast<uint2*>(y) = make_uint2(ca[0], ca[1]);
+            *reinterpret_cast<uint2*>(y + across) = make_uint2(cb[0], cb[1]);
+          } else {
+            *reinterpret_cast<uint32_t*>(y) = ca[0];
+            *reinterpret_cast<uint32_t*>(y + across) = cb[0];
+          }
+          if (j == 0) scales[at] = most / kE4M3Max;
+        }
+        at += (int64_t)kRows * a.page;
+      }
+      to += to_step;
+      row += kRows;
     }
   }
 }
 
-// The backward: g and x in registers, dw summed per lane over the CTA's rows (a run of
-// each operand's rows for each warp), then over the warp's row groups and the warps in a
-// fixed order.
+// CTAs [0, q_blocks) have the queries' rows, the next ones the keys', then the values'.
+constexpr int kRopeBlock = 128;
+constexpr int kRopeWarps = kRopeBlock / 32;
+
+struct Split {
+  int q_blocks, k_blocks, q_run, k_run;   // CTAs, and groups of rows of a warp
+};
+
+template <typename T, int L, bool kWrite>
+__global__ void __launch_bounds__(kRopeBlock, 5)
+qk_rope_kernel(const __grid_constant__ QkArgs a, const __grid_constant__ Split sp) {
+  ptx::grid_dep_wait();
+  ptx::grid_dep_launch_dependents();
+  const int tid = thread_here(), lane = tid & 31;
+  int block = blockIdx.x;
+  if (block < sp.q_blocks) {
+    qk_rope_rows<T, L, true, kRowsOut>(a, a.q, a.qo, a.qw, nullptr, nullptr, a.hq, block * kRopeWarps + (tid >> 5),
+                                       lane, sp.q_run);
+    return;
+  }
+  block -= sp.q_blocks;
+  if (!kWrite || block < sp.k_blocks) {
+    qk_rope_rows<T, L, true, kWrite ? kCacheOut : kRowsOut>(a, a.k, a.ko, a.kw, a.kc, a.ks, a.hk,
+                                                            block * kRopeWarps + (tid >> 5), lane, sp.k_run);
+    return;
+  }
+  block -= sp.k_blocks;
+  if constexpr (kWrite)
+    qk_rope_rows<T, L, false, kCacheOut>(a, a.v, a.ko, nullptr, a.vc, a.vs, a.hk, block * kRopeWarps + (tid >> 5),
+                                         lane, sp.k_run);
+}
+
+// The backward: g and x in registers, dw summed per lane over the lane's rows, then over
+// the warp's row groups and the CTA's warps in a fixed order. CTAs [0, q_blocks) share the
+// queries' rows equally, the others the keys'.
 template <typename T, int L>
 __global__ void __launch_bounds__(kBlock, 2)
-qk_rope_backward_kernel(const __grid_constant__ QkBackArgs a) {
-  constexpr int E = Pack<T>::kE, kRows = 32 / L;
+qk_rope_backward_kernel(const __grid_constant__ QkBackArgs a, int q_blocks) {
+  constexpr int E = Pack<T>::kE, N = E / 2, kRows = 32 / L;
   extern __shared__ float dw[];     // [kWarps][d]
   ptx::grid_dep_wait();
   ptx::grid_dep_launch_dependents();
   const int tid = thread_here(), lane = tid & 31, warp = tid >> 5, j = lane % L;
   const UnitOf<T> u(j, a.d, a.r, a.interleaved);
-  const int64_t workers = (int64_t)gridDim.x * kWarps, me = (int64_t)blockIdx.x * kWarps + warp;
+  const int across = u.eb - u.ea;
+  const bool is_q = (int)blockIdx.x < q_blocks;
+  const unsigned blocks = is_q ? q_blocks : gridDim.x - q_blocks, block = is_q ? blockIdx.x : blockIdx.x - q_blocks;
+  const unsigned heads = is_q ? a.hq : a.hk;
+  const Rows xr = is_q ? a.q : a.k, gr = is_q ? a.dqo : a.dko;
+  Vec<T> wa = {}, wb = {}, da = {}, db = {};
+  if (a.norm && u.on) {
+    const T* w = static_cast<const T*>(is_q ? a.qw : a.kw);
+    wa.from(ptx::ld_cached_v4(w + u.ea));
+    wb.from(ptx::ld_cached_v4(w + u.eb));
+  }
+  const unsigned rows = (unsigned)a.tokens * heads, groups = (rows + kRows - 1) / kRows;
+  const unsigned workers = blocks * kWarps, me = block * kWarps + warp;
+  const unsigned first = (unsigned)((uint64_t)groups * me / workers);
+  const unsigned n = (unsigned)((uint64_t)groups * (me + 1) / workers) - first;
+  unsigned row = first * kRows + lane / L, end = 0;
+  T* y = static_cast<T*>(is_q ? a.dq : a.dk) + (int64_t)row * a.d + u.ea;
+  Walk<T, kRows> gw(row), xw(row);
+  uint4 x[2] = {}, g[2] = {};
+  auto fetch = [&]() {
+    x[0] = x[1] = g[0] = g[1] = make_uint4(0u, 0u, 0u, 0u);
+    if (gw.row >= rows || !u.on) return;
+    unsigned t, h;
+    gw.enter(gr, heads, u.ea, t, h);
+    g[0] = ptx::ld_stream_v4(gw.p);
+    g[1] = ptx::ld_stream_v4(gw.p + across);
+    gw.step(kRows * gr.sh);
+    if (!a.norm) return;
+    xw.enter(xr, heads, u.ea, t, h);
+    x[0] = ptx::ld_stream_v4(xw.p);
+    x[1] = ptx::ld_stream_v4(xw.p + across);
+    xw.step(kRows * xr.sh);
+  };
   const float rd = 1.f / (float)a.d;
+  Turn<T> turn;
+  if (n > 0) fetch();
 #pragma unroll 1
-  for (int part = 0; part < 2; ++part) {
-    const int heads = part == 0 ? a.hq : a.hk;
-    const Rows xr = part == 0 ? a.q : a.k, gr = part == 0 ? a.dqo : a.dko;
-    T* dx = static_cast<T*>(part == 0 ? a.dq : a.dk);
-    float wa[E] = {}, wb[E] = {}, da[E] = {}, db[E] = {};
-    if (a.norm && u.on) {
-      const T* w = static_cast<const T*>(part == 0 ? a.qw : a.kw);
-      Pack<T>::unpack(ptx::ld_cached_v4(w + u.ea), wa);
-      Pack<T>::unpack(ptx::ld_cached_v4(w + u.eb), wb);
+  for (unsigned i = 0; i < n; ++i) {
+    const bool live = row < rows;
+    if (live && row >= end) {
+      const unsigned t = row / heads;
+      end = (t + 1) * heads;
+      if (u.turned) turn.load(a.rope, a.positions[t], a.max_pos, a.r, j);
     }
-    const int64_t rows = a.tokens * heads, groups = (rows + kRows - 1) / kRows;
-    const int64_t first = groups * me / workers, end = groups * (me + 1) / workers;
-    int64_t row = first * kRows + lane / L;
-    int64_t t = row / heads;
-    int h = (int)(row - t * heads);
-    Turn<T> turn;
-    int64_t turn_of = -1;
-    uint4 x[2], g[2];
-    auto fetch = [&]() {
-      x[0] = x[1] = g[0] = g[1] = make_uint4(0u, 0u, 0u, 0u);
-      if (row >= rows || !u.on) return;
-      const T* p = static_cast<const T*>(gr.p) + t * gr.st + h * gr.sh;
-      g[0] = ptx::ld_stream_v4(p + u.ea);
-      g[1] = ptx::ld_stream_v4(p + u.eb);
-      if (a.norm) {
-        p = static_cast<const T*>(xr.p) + t * xr.st + h * xr.sh;
-        x[0] = ptx::ld_stream_v4(p + u.ea);
-        x[1] = ptx::ld_stream_v4(p + u.eb);
-      }
-    };
-    if (first < end) fetch();
-#pragma unroll 1
-    for (int64_t i = first; i < end; ++i) {
-      const bool live = row < rows;
-      if (live && t != turn_of) {
-        turn_of = t;
-        if (u.turned) turn.load(a.rope, a.positions[t], a.max_pos, a.r, j);
-      }
-      float xa[E], xb[E], ga[E], gb[E];
-      Pack<T>::unpack(x[0], xa);
-      Pack<T>::unpack(x[1], xb);
-      Pack<T>::unpack(g[0], ga);
-      Pack<T>::unpack(g[1], gb);
-      T* y = dx + row * a.d;
-      row += kRows;
-      h += kRows;
-      while (h >= heads) {
-        h -= heads;
-        ++t;
-      }
-      if (i + 1 < end) fetch();
-      if (u.turned && live) turn.template apply<true>(ga, gb, a.interleaved);
-      if (a.norm) {
-        float ss = 0.f, sg = 0.f;
+    Vec<T> xa, xb, ga, gb;
+    xa.from(x[0]);
+    xb.from(x[1]);
+    ga.from(g[0]);
+    gb.from(g[1]);
+    if (i + 1 < n) fetch();
+    if (u.turned && live) turn.template apply<true>(ga, gb, a.interleaved);
+    if (a.norm) {
+      f2 ss = 0ull, sg = 0ull;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          ss = fmaf(xa[e], xa[e], fmaf(xb[e], xb[e], ss));
-          sg = fmaf(ga[e] * wa[e], xa[e], fmaf(gb[e] * wb[e], xb[e], sg));
-        }
-        ss = lanes_sum<L>(ss);
-        sg = lanes_sum<L>(sg);
-        const float inv = rsqrtf(ss * rd + a.eps);
-        const float k = inv * inv * inv * (sg * rd);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float na = ga[e] * inv, nb = gb[e] * inv;
-          da[e] = fmaf(na, xa[e], da[e]);
-          db[e] = fmaf(nb, xb[e], db[e]);
-          ga[e] = na * wa[e] - xa[e] * k;
-          gb[e] = nb * wb[e] - xb[e] * k;
-        }
+      for (int e = 0; e < N; ++e) {
+        ss = fma2(xa.v[e], xa.v[e], fma2(xb.v[e], xb.v[e], ss));
+        sg = fma2(mul2(ga.v[e], wa.v[e]), xa.v[e], fma2(mul2(gb.v[e], wb.v[e]), xb.v[e], sg));
       }
-      if (live && u.on) {
-        ptx::st_v4(y + u.ea, Pack<T>::pack(ga));
-        ptx::st_v4(y + u.eb, Pack<T>::pack(gb));
+      const float sum = lanes_sum<L>(f2_sum(ss)), dot = lanes_sum<L>(f2_sum(sg));
+      const float inv = rsqrtf(sum * rd + a.eps);
+      const float k = -inv * inv * inv * (dot * rd);
+      const f2 inv2 = f2_of(inv, inv), k2 = f2_of(k, k);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        ga.v[e] = mul2(ga.v[e], inv2);
+        gb.v[e] = mul2(gb.v[e], inv2);
+        da.v[e] = fma2(ga.v[e], xa.v[e], da.v[e]);
+        db.v[e] = fma2(gb.v[e], xb.v[e], db.v[e]);
+        ga.v[e] = fma2(ga.v[e], wa.v[e], mul2(xa.v[e], k2));
+        gb.v[e] = fma2(gb.v[e], wb.v[e], mul2(xb.v[e], k2));
       }
     }
-    if (!a.norm) continue;
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-#pragma unroll
-      for (int o = L; o < 32; o <<= 1) {
-        da[e] += __shfl_xor_sync(0xFFFFFFFFu, da[e], o);
-        db[e] += __shfl_xor_sync(0xFFFFFFFFu, db[e], o);
-      }
-    if (lane < L && u.on) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        dw[warp * a.d + u.ea + e] = da[e];
-        dw[warp * a.d + u.eb + e] = db[e];
-      }
+    if (live && u.on) {
+      ptx::st_v4(y, ga.to());
+      ptx::st_v4(y + across, gb.to());
     }
-    __syncthreads();
-    for (int i = tid; i < a.d; i += kBlock) {
-      float s = 0.f;
-      for (int v = 0; v < kWarps; ++v) s += dw[v * a.d + i];
-      a.ws[((int64_t)blockIdx.x * 2 + part) * a.d + i] = s;
+    row += kRows;
+    y += kRows * a.d;
+  }
+  if (!a.norm) return;
+  float fa[E], fb[E];
+  da.floats(fa);
+  db.floats(fb);
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+#pragma unroll
+    for (int o = L; o < 32; o <<= 1) {
+      fa[e] += __shfl_xor_sync(0xFFFFFFFFu, fa[e], o);
+      fb[e] += __shfl_xor_sync(0xFFFFFFFFu, fb[e], o);
     }
-    __syncthreads();
+  if (lane < L && u.on) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      dw[warp * a.d + u.ea + e] = fa[e];
+      dw[warp * a.d + u.eb + e] = fb[e];
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < a.d; i += kBlock) {
+    float s = 0.f;
+    for (int v = 0; v < kWarps; ++v) s += dw[v * a.d + i];
+    a.ws[(int64_t)blockIdx.x * a.d + i] = s;
   }
 }
 
-// dw of both weights from the CTAs' partials ([parts][2 d]): a CTA has 32 columns, its warps
+// dw of both weights from the CTAs' partials: a CTA has 32 columns of one of them, its warps
 // the parts w, w + 32, ..., added in that order and then in warp order.
 constexpr int kDwWarps = 32;
 
 template <typename T>
 __global__ void __launch_bounds__(kDwWarps * 32)
-qk_rope_dw_kernel(const float* ws, int parts, int d, T* dqw, T* dkw) {
+qk_rope_dw_kernel(const float* ws, int q_parts, int parts, int d, T* dqw, T* dkw) {
   __shared__ float s_sum[kDwWarps][32];
   ptx::grid_dep_wait();
   ptx::grid_dep_launch_dependents();
   const int tid = thread_here(), lane = tid & 31, warp = tid >> 5;
-  const int col = blockIdx.x * 32 + lane;
+  const bool is_q = blockIdx.y == 0;
+  const int col = blockIdx.x * 32 + lane, first = is_q ? 0 : q_parts, end = is_q ? q_parts : parts;
   float s = 0.f;
-  if (col < 2 * d) {
+  if (col < d) {
 #pragma unroll 10
-    for (int i = warp; i < parts; i += kDwWarps) s += ws[(int64_t)i * 2 * d + col];
+    for (int i = first + warp; i < end; i += kDwWarps) s += ws[(int64_t)i * d + col];
   }
   s_sum[warp][lane] = s;
   __syncthreads();
-  if (warp != 0 || col >= 2 * d) return;
+  if (warp != 0 || col >= d) return;
   s = 0.f;
 #pragma unroll
   for (int w = 0; w < kDwWarps; ++w) s += s_sum[w][lane];
-  (col < d ? dqw + col : dkw + (col - d))[0] = Pack<T>::from_f(s);
+  (is_q ? dqw : dkw)[col] = Pack<T>::from_f(s);
 }
 
 // Lanes of a row where the vector kernels take it, else 0 (the kernels for any row):
@@ -769,18 +871,34 @@ int run_forward(const char* who, const rmsnorm_qk_rope_args* in, void* stream) {
   const void* fn = in->dtype == RMSNORM_TP_F32    ? forward_fn<float, kWrite>(lanes)
                    : in->dtype == RMSNORM_TP_BF16 ? forward_fn<__nv_bfloat16, kWrite>(lanes)
                                                   : forward_fn<__half, kWrite>(lanes);
-  // groups of rows for each warp: as many as leave every SM 32 warps, at most 8
-  const int64_t groups = lanes ? (rows * lanes + 31) / 32 : rows;
-  int run = 1;
+  const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  cudaError_t e;
   if (lanes) {
-    const int64_t full = 32ll * sm_count(in->device);
-    run = (int)(groups / (full > 0 ? full : 1));
-    run = run < 1 ? 1 : run > 8 ? 8 : run;
+    // groups of rows for each warp: as many as leave every SM 32 warps, at most 8; whole
+    // tokens where that is a few more
+    const int per = 32 / lanes, sms = sm_count(in->device);
+    auto runs = [&](int64_t groups, int heads) {
+      int64_t run = groups / (32ll * (sms > 0 ? sms : 1));
+      run = run < 1 ? 1 : run > 8 ? 8 : run;
+      const int64_t token = heads % per == 0 ? heads / per : 1;
+      return (int)((run + token - 1) / token * token <= 2 * run ? (run + token - 1) / token * token : run);
+    };
+    auto blocks = [&](int64_t groups, int run) {
+      return (int)((groups + (int64_t)run * kRopeWarps - 1) / ((int64_t)run * kRopeWarps));
+    };
+    const int64_t gq = (a.tokens * a.hq + per - 1) / per, gk = (a.tokens * a.hk + per - 1) / per;
+    Split sp;
+    sp.q_run = runs(gq, a.hq);
+    sp.k_run = runs(gk, a.hk);
+    sp.q_blocks = blocks(gq, sp.q_run);
+    sp.k_blocks = blocks(gk, sp.k_run);
+    void* args[] = {&a, &sp};
+    e = launch_dependent(fn, dim3((unsigned)sp.q_blocks + (kWrite ? 2u : 1u) * (unsigned)sp.k_blocks),
+                         dim3(kRopeBlock), 0, args, st);
+  } else {
+    void* args[] = {&a};
+    e = launch_dependent(fn, dim3((unsigned)((rows + kWarps - 1) / kWarps)), dim3(kBlock), 0, args, st);
   }
-  const int64_t blocks = (groups + (int64_t)run * kWarps - 1) / ((int64_t)run * kWarps);
-  void* args[] = {&a, &run};
-  const cudaError_t e = launch_dependent(fn, dim3((unsigned)blocks), dim3(kBlock), 0, args,
-                                         reinterpret_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? RMSNORM_TP_OK : launch_failed(e, who);
 }
 
@@ -799,7 +917,7 @@ int rmsnorm_qk_rope_write(const rmsnorm_qk_rope_args* args, void* stream) {
 
 size_t rmsnorm_qk_rope_backward_workspace_bytes(int32_t head_dim) {
   if (head_dim < 2 || head_dim > RMSNORM_HEAD_DIM_MAX) return 0;
-  return (size_t)rtp::kBackwardMaxGrid * 2u * (size_t)head_dim * sizeof(float);
+  return (size_t)rtp::kBackwardMaxGrid * (size_t)head_dim * sizeof(float);
 }
 
 int rmsnorm_qk_rope_backward(const rmsnorm_qk_rope_backward_args* in, void* stream) {
@@ -844,7 +962,7 @@ int rmsnorm_qk_rope_backward(const rmsnorm_qk_rope_backward_args* in, void* stre
   OnDevice on(in->device);
   if (on.err != cudaSuccess) return launch_failed(on.err, who);
   const cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  int grid = 0;
+  int grid = 0, q_blocks = 0;
   if (in->tokens > 0) {
     QkBackArgs a = {};
     a.dqo = Rows{in->dq_out, in->dq_out_strides[0], in->dq_out_strides[1]};
@@ -872,13 +990,22 @@ int rmsnorm_qk_rope_backward(const rmsnorm_qk_rope_backward_args* in, void* stre
     const int64_t strides = a.dqo.st | a.dqo.sh | a.dko.st | a.dko.sh |
                             (norm ? a.q.st | a.q.sh | a.k.st | a.k.sh : 0);
     const int lanes = lanes_of(a.d, a.r, eb, bits, strides);
-    const int64_t groups = lanes ? (a.tokens * a.hq * lanes + 31) / 32 : a.tokens * a.hq;
-    const int64_t want = (groups + kWarps - 1) / kWarps;
-    grid = (int)(want < kBackwardMaxGrid ? want : kBackwardMaxGrid);
+    // one resident wave of CTAs, shared by q and k as their rows are
+    const int64_t rows_of_cta = (int64_t)kWarps * (lanes ? 32 / lanes : 1);
+    const int64_t wq = (a.tokens * a.hq + rows_of_cta - 1) / rows_of_cta;
+    const int64_t wk = (a.tokens * a.hk + rows_of_cta - 1) / rows_of_cta;
+    if (wq + wk <= kBackwardMaxGrid) {
+      q_blocks = (int)wq;
+      grid = (int)(wq + wk);
+    } else {
+      grid = kBackwardMaxGrid;
+      q_blocks = (int)((wq * grid + (wq + wk) / 2) / (wq + wk));
+      q_blocks = q_blocks < 1 ? 1 : q_blocks >= grid ? grid - 1 : q_blocks;
+    }
     const void* fn = in->dtype == RMSNORM_TP_F32    ? backward_fn<float>(lanes)
                      : in->dtype == RMSNORM_TP_BF16 ? backward_fn<__nv_bfloat16>(lanes)
                                                     : backward_fn<__half>(lanes);
-    void* args[] = {&a};
+    void* args[] = {&a, &q_blocks};
     const size_t smem = norm ? (size_t)kWarps * a.d * sizeof(float) : 0;
     const cudaError_t e = launch_dependent(fn, dim3((unsigned)grid), dim3(kBlock), smem, args, st);
     if (e != cudaSuccess) return launch_failed(e, who);
@@ -888,11 +1015,11 @@ int rmsnorm_qk_rope_backward(const rmsnorm_qk_rope_backward_args* in, void* stre
     int d = in->head_dim;
     void* dqw = in->dq_weight;
     void* dkw = in->dk_weight;
-    void* args[] = {&ws, &grid, &d, &dqw, &dkw};
+    void* args[] = {&ws, &q_blocks, &grid, &d, &dqw, &dkw};
     const void* fn = in->dtype == RMSNORM_TP_F32    ? reinterpret_cast<const void*>(qk_rope_dw_kernel<float>)
                      : in->dtype == RMSNORM_TP_BF16 ? reinterpret_cast<const void*>(qk_rope_dw_kernel<__nv_bfloat16>)
                                                     : reinterpret_cast<const void*>(qk_rope_dw_kernel<__half>);
-    const cudaError_t e = launch_dependent(fn, dim3((2 * d + 31) / 32), dim3(kDwWarps * 32), 0, args, st);
+    const cudaError_t e = launch_dependent(fn, dim3((d + 31) / 32, 2), dim3(kDwWarps * 32), 0, args, st);
     if (e != cudaSuccess) return launch_failed(e, who);
   }
   return RMSNORM_TP_OK;
