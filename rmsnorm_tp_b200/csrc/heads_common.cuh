@@ -108,6 +108,26 @@ __device__ __forceinline__ int thread_here() {
   return t;
 }
 
+// ---- asynchronous copies into shared memory (16 bytes a thread) -----------------
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// With `live` false nothing is read and zeros are written.
+__device__ __forceinline__ void cp_async16_if(uint32_t dst, const void* src, bool live) {
+  const int n = live ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async4_if(uint32_t dst, const void* src, bool live) {
+  const int n = live ? 4 : 0;
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Waits until at most N of this thread's groups are under way.
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 // Page and offset of a slot; 32-bit division where the cache's slots allow it.
 __device__ __forceinline__ void page_of(int64_t slot, int page, int64_t num_slots, int64_t& pg, int& off) {
   if (num_slots <= 0xFFFFFFFFll) {

@@ -205,22 +205,6 @@ struct Shape {
   static_assert(kStages >= 3, "the ring needs three stages");
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async16_if(uint32_t dst, const void* src, bool live) {
-  const int n = live ? 16 : 0;          // 0: zeros, nothing is read
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool live) {
-  const int n = live ? 4 : 0;
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
@@ -448,7 +432,7 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
       if constexpr (kE4M3) {          // lanes 0-15 K's scales, 16-31 V's
         const int64_t r = a.whole_pages ? row + (lane & 15) : row;
         const bool on = (mask >> (lane & 15)) & 1u;
-        cp_async4(dst + kSideOff + lane * 4, (lane < 16 ? a.ks : a.vs) + (on ? r : 0), on);
+        cp_async4_if(dst + kSideOff + lane * 4, (lane < 16 ? a.ks : a.vs) + (on ? r : 0), on);
       }
       if (a.whole_pages && mask == 0xFFFFu) {
         const int64_t from = (row + lr) * S::kRowBytes;

@@ -424,13 +424,36 @@ struct Walk {
 // What becomes of an operand's rows.
 enum Out { kRowsOut, kCacheOut };
 
+// A lane's rows on their way: kStages stages of kVecs 16-byte vectors in shared memory, each
+// written by the lane's own asynchronous copies and read by the lane alone, so that deep
+// loads cost no registers and no barrier.
+template <int kVecs, int kStages>
+struct Ring {
+  static constexpr int kDeep = kStages, kWarpBytes = kStages * kVecs * 512;
+  uint32_t base;                         // of this lane
+  __device__ __forceinline__ Ring(void* smem, int warp, int lane)
+      : base(ptx::smem_addr(smem) + warp * kWarpBytes + lane * 16) {}
+  __device__ __forceinline__ uint32_t at(int stage, int vec) const { return base + (stage * kVecs + vec) * 512; }
+  __device__ __forceinline__ uint4 get(int stage, int vec) const {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(at(stage, vec))
+                 : "memory");
+    return v;
+  }
+};
+
+using RopeRing = Ring<2, 4>;             // x
+using BackRing = Ring<4, 3>;             // dy and x: 48 KB for a CTA's warps
+
 // `run` groups of 32 / L rows of one operand. kTurned: normed and turned (else as they are:
-// the values on their way to the cache); kDeep rows are in flight ahead.
+// the values on their way to the cache).
 template <typename T, int L, bool kTurned, int kOut>
 __device__ __forceinline__ void qk_rope_rows(const QkArgs& a, const Rows& in, const OutRows& out, const void* w,
                                              void* cache, float* scales, unsigned heads, unsigned warp, int lane,
-                                             int run) {
-  constexpr int E = Pack<T>::kE, N = E / 2, kRows = 32 / L, kDeep = 2;
+                                             int run, const RopeRing& ring) {
+  constexpr int E = Pack<T>::kE, N = E / 2, kRows = 32 / L, kDeep = RopeRing::kDeep;
   const int j = lane % L;
   const UnitOf<T> u(j, a.d, a.r, a.interleaved);
   const unsigned rows = (unsigned)a.tokens * heads;   // at most 2^31
@@ -438,18 +461,21 @@ __device__ __forceinline__ void qk_rope_rows(const QkArgs& a, const Rows& in, co
   const int64_t in_step = kRows * in.sh;
   const int across = u.eb - u.ea;
   Walk<T, kRows> ahead(first);
-  auto fetch = [&](uint4 (&x)[2]) {
-    x[0] = x[1] = make_uint4(0u, 0u, 0u, 0u);
-    if (ahead.row >= rows || !u.on) return;
+  auto fetch = [&](int stage) {
+    const bool live = ahead.row < rows && u.on;
     unsigned t, h;
-    ahead.enter(in, heads, u.ea, t, h);
-    x[0] = ptx::ld_stream_v4(ahead.p);
-    x[1] = ptx::ld_stream_v4(ahead.p + across);
+    if (live) ahead.enter(in, heads, u.ea, t, h);
+    const T* p = live ? ahead.p : static_cast<const T*>(in.p);
+    cp_async16_if(ring.at(stage, 0), p, live);
+    cp_async16_if(ring.at(stage, 1), live ? p + across : p, live);
+    cp_commit();
     ahead.step(in_step);
   };
-  uint4 next[kDeep][2];
 #pragma unroll
-  for (int i = 0; i < kDeep; ++i) fetch(next[i]);
+  for (int i = 0; i < kDeep; ++i) {
+    if (i < run) fetch(i);
+    else cp_commit();
+  }
   Vec<T> wa, wb;
   Turn<T> turn;
   if (kTurned && a.norm && u.on) {
@@ -463,83 +489,84 @@ __device__ __forceinline__ void qk_rope_rows(const QkArgs& a, const Rows& in, co
   bool keep = kOut == kRowsOut;
   const int64_t to_step = kOut == kRowsOut ? kRows * out.sh : (int64_t)kRows * a.page * a.d;
 #pragma unroll 1
-  for (int i = 0; i < run; i += kDeep) {
-#pragma unroll
-    for (int k = 0; k < kDeep; ++k) {
-      if (i + k >= run || !__any_sync(0xFFFFFFFFu, row < rows)) return;
-      const bool live = row < rows;
-      Vec<T> ya, yb;
-      ya.from(next[k][0]);
-      yb.from(next[k][1]);
-      if (i + k + kDeep < run) fetch(next[k]);
-      if (row >= end && live) {
-        const unsigned t = row / heads, h = row - t * heads;
-        end = row - h + heads;
-        if (kTurned && u.turned) turn.load(a.rope, a.positions[t], a.max_pos, a.r, j);
-        if constexpr (kOut == kRowsOut) {
-          to = static_cast<T*>(out.p) + t * out.st + (int64_t)h * out.sh + u.ea;
-        } else {
-          const int64_t slot = a.slots[t];
-          keep = slot >= 0 && slot < a.num_slots;
-          at = keep ? cache_row(slot, h, a) : 0;
-          to = static_cast<T*>(cache) + at * a.d + u.ea;
-        }
-      }
-      if (kTurned && a.norm) {
-        f2 sa = mul2(ya.v[0], ya.v[0]), sb = mul2(yb.v[0], yb.v[0]);
-#pragma unroll
-        for (int e = 1; e < N; ++e) {
-          sa = fma2(ya.v[e], ya.v[e], sa);
-          sb = fma2(yb.v[e], yb.v[e], sb);
-        }
-        const float inv = rsqrtf(lanes_sum<L>(f2_sum(sa) + f2_sum(sb)) * rd + a.eps);
-        const f2 inv2 = f2_of(inv, inv);
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-          ya.v[e] = mul2(mul2(ya.v[e], inv2), wa.v[e]);
-          yb.v[e] = mul2(mul2(yb.v[e], inv2), wb.v[e]);
-        }
-      }
-      if (kTurned && u.turned) turn.template apply<false>(ya, yb, a.interleaved);
-      if (kOut == kRowsOut || !a.e4m3) {
-        if (live && keep && u.on) {
-          ptx::st_v4(to, ya.to());
-          ptx::st_v4(to + across, yb.to());
-        }
+  for (int i = 0; i < run; ++i) {
+    const int k = i % kDeep;
+    if (!__any_sync(0xFFFFFFFFu, row < rows)) break;
+    const bool live = row < rows;
+    cp_wait<kDeep - 1>();
+    Vec<T> ya, yb;
+    ya.from(ring.get(k, 0));
+    yb.from(ring.get(k, 1));
+    if (i + kDeep < run) fetch(k);
+    else cp_commit();
+    if (row >= end && live) {
+      const unsigned t = row / heads, h = row - t * heads;
+      end = row - h + heads;
+      if (kTurned && u.turned) turn.load(a.rope, a.positions[t], a.max_pos, a.r, j);
+      if constexpr (kOut == kRowsOut) {
+        to = static_cast<T*>(out.p) + t * out.st + (int64_t)h * out.sh + u.ea;
       } else {
-        float fa[E], fb[E];
-        ya.floats(fa);
-        yb.floats(fb);
-        float most = kE4M3Floor;
-#pragma unroll
-        for (int e = 0; e < E; ++e) most = fmaxf(most, fmaxf(fabsf(fa[e]), fabsf(fb[e])));
-        most = lanes_max<L>(most);
-        if (live && keep && u.on) {
-          const float up = kE4M3Max / most;
-          unsigned char* y = static_cast<unsigned char*>(cache) + at * a.d + u.ea;
-          uint32_t ca[E / 4], cb[E / 4];
-#pragma unroll
-          for (int e = 0; e < E / 4; ++e) {
-            ca[e] = e4m3x2_of(fa[4 * e] * up, fa[4 * e + 1] * up) |
-                    (uint32_t)e4m3x2_of(fa[4 * e + 2] * up, fa[4 * e + 3] * up) << 16;
-            cb[e] = e4m3x2_of(fb[4 * e] * up, fb[4 * e + 1] * up) |
-                    (uint32_t)e4m3x2_of(fb[4 * e + 2] * up, fb[4 * e + 3] * up) << 16;
-          }
-          if constexpr (E == 8) {
-            *reinterpret_cast<uint2*>(y) = make_uint2(ca[0], ca[1]);
-            *reinterpret_cast<uint2*>(y + across) = make_uint2(cb[0], cb[1]);
-          } else {
-            *reinterpret_cast<uint32_t*>(y) = ca[0];
-            *reinterpret_cast<uint32_t*>(y + across) = cb[0];
-          }
-          if (j == 0) scales[at] = most / kE4M3Max;
-        }
-        at += (int64_t)kRows * a.page;
+        const int64_t slot = a.slots[t];
+        keep = slot >= 0 && slot < a.num_slots;
+        at = keep ? cache_row(slot, h, a) : 0;
+        to = static_cast<T*>(cache) + at * a.d + u.ea;
       }
-      to += to_step;
-      row += kRows;
     }
+    if (kTurned && a.norm) {
+      f2 sa = mul2(ya.v[0], ya.v[0]), sb = mul2(yb.v[0], yb.v[0]);
+#pragma unroll
+      for (int e = 1; e < N; ++e) {
+        sa = fma2(ya.v[e], ya.v[e], sa);
+        sb = fma2(yb.v[e], yb.v[e], sb);
+      }
+      const float inv = rsqrtf(lanes_sum<L>(f2_sum(sa) + f2_sum(sb)) * rd + a.eps);
+      const f2 inv2 = f2_of(inv, inv);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        ya.v[e] = mul2(mul2(ya.v[e], inv2), wa.v[e]);
+        yb.v[e] = mul2(mul2(yb.v[e], inv2), wb.v[e]);
+      }
+    }
+    if (kTurned && u.turned) turn.template apply<false>(ya, yb, a.interleaved);
+    if (kOut == kRowsOut || !a.e4m3) {
+      if (live && keep && u.on) {
+        ptx::st_v4(to, ya.to());
+        ptx::st_v4(to + across, yb.to());
+      }
+    } else {
+      float fa[E], fb[E];
+      ya.floats(fa);
+      yb.floats(fb);
+      float most = kE4M3Floor;
+#pragma unroll
+      for (int e = 0; e < E; ++e) most = fmaxf(most, fmaxf(fabsf(fa[e]), fabsf(fb[e])));
+      most = lanes_max<L>(most);
+      if (live && keep && u.on) {
+        const float up = kE4M3Max / most;
+        unsigned char* y = static_cast<unsigned char*>(cache) + at * a.d + u.ea;
+        uint32_t ca[E / 4], cb[E / 4];
+#pragma unroll
+        for (int e = 0; e < E / 4; ++e) {
+          ca[e] = e4m3x2_of(fa[4 * e] * up, fa[4 * e + 1] * up) |
+                  (uint32_t)e4m3x2_of(fa[4 * e + 2] * up, fa[4 * e + 3] * up) << 16;
+          cb[e] = e4m3x2_of(fb[4 * e] * up, fb[4 * e + 1] * up) |
+                  (uint32_t)e4m3x2_of(fb[4 * e + 2] * up, fb[4 * e + 3] * up) << 16;
+        }
+        if constexpr (E == 8) {
+          *reinterpret_cast<uint2*>(y) = make_uint2(ca[0], ca[1]);
+          *reinterpret_cast<uint2*>(y + across) = make_uint2(cb[0], cb[1]);
+        } else {
+          *reinterpret_cast<uint32_t*>(y) = ca[0];
+          *reinterpret_cast<uint32_t*>(y + across) = cb[0];
+        }
+        if (j == 0) scales[at] = most / kE4M3Max;
+      }
+      at += (int64_t)kRows * a.page;
+    }
+    to += to_step;
+    row += kRows;
   }
+  cp_wait<0>();
 }
 
 // CTAs [0, q_blocks) have the queries' rows, the next ones the keys', then the values'.
@@ -555,23 +582,25 @@ __global__ void __launch_bounds__(kRopeBlock, 5)
 qk_rope_kernel(const __grid_constant__ QkArgs a, const __grid_constant__ Split sp) {
   ptx::grid_dep_wait();
   ptx::grid_dep_launch_dependents();
+  __shared__ uint4 smem[kRopeWarps * RopeRing::kWarpBytes / 16];
   const int tid = thread_here(), lane = tid & 31;
+  const RopeRing ring(smem, tid >> 5, lane);
   int block = blockIdx.x;
   if (block < sp.q_blocks) {
     qk_rope_rows<T, L, true, kRowsOut>(a, a.q, a.qo, a.qw, nullptr, nullptr, a.hq, block * kRopeWarps + (tid >> 5),
-                                       lane, sp.q_run);
+                                       lane, sp.q_run, ring);
     return;
   }
   block -= sp.q_blocks;
   if (!kWrite || block < sp.k_blocks) {
     qk_rope_rows<T, L, true, kWrite ? kCacheOut : kRowsOut>(a, a.k, a.ko, a.kw, a.kc, a.ks, a.hk,
-                                                            block * kRopeWarps + (tid >> 5), lane, sp.k_run);
+                                                            block * kRopeWarps + (tid >> 5), lane, sp.k_run, ring);
     return;
   }
   block -= sp.k_blocks;
   if constexpr (kWrite)
     qk_rope_rows<T, L, false, kCacheOut>(a, a.v, a.ko, nullptr, a.vc, a.vs, a.hk, block * kRopeWarps + (tid >> 5),
-                                         lane, sp.k_run);
+                                         lane, sp.k_run, ring);
 }
 
 // The backward: g and x in registers, dw summed per lane over the lane's rows, then over
@@ -580,11 +609,12 @@ qk_rope_kernel(const __grid_constant__ QkArgs a, const __grid_constant__ Split s
 template <typename T, int L>
 __global__ void __launch_bounds__(kBlock, 2)
 qk_rope_backward_kernel(const __grid_constant__ QkBackArgs a, int q_blocks) {
-  constexpr int E = Pack<T>::kE, N = E / 2, kRows = 32 / L;
-  extern __shared__ float dw[];     // [kWarps][d]
+  constexpr int E = Pack<T>::kE, N = E / 2, kRows = 32 / L, kDeep = BackRing::kDeep;
+  extern __shared__ __align__(16) float dw[];   // the ring, then [kWarps][d]
   ptx::grid_dep_wait();
   ptx::grid_dep_launch_dependents();
   const int tid = thread_here(), lane = tid & 31, warp = tid >> 5, j = lane % L;
+  const BackRing ring(dw, warp, lane);
   const UnitOf<T> u(j, a.d, a.r, a.interleaved);
   const int across = u.eb - u.ea;
   const bool is_q = (int)blockIdx.x < q_blocks;
@@ -604,24 +634,30 @@ qk_rope_backward_kernel(const __grid_constant__ QkBackArgs a, int q_blocks) {
   unsigned row = first * kRows + lane / L, end = 0;
   T* y = static_cast<T*>(is_q ? a.dq : a.dk) + (int64_t)row * a.d + u.ea;
   Walk<T, kRows> gw(row), xw(row);
-  uint4 x[2] = {}, g[2] = {};
-  auto fetch = [&]() {
-    x[0] = x[1] = g[0] = g[1] = make_uint4(0u, 0u, 0u, 0u);
-    if (gw.row >= rows || !u.on) return;
+  auto fetch = [&](int stage) {
+    const bool live = gw.row < rows && u.on;
     unsigned t, h;
-    gw.enter(gr, heads, u.ea, t, h);
-    g[0] = ptx::ld_stream_v4(gw.p);
-    g[1] = ptx::ld_stream_v4(gw.p + across);
+    if (live) gw.enter(gr, heads, u.ea, t, h);
+    const T* p = live ? gw.p : static_cast<const T*>(gr.p);
+    cp_async16_if(ring.at(stage, 0), p, live);
+    cp_async16_if(ring.at(stage, 1), live ? p + across : p, live);
     gw.step(kRows * gr.sh);
-    if (!a.norm) return;
-    xw.enter(xr, heads, u.ea, t, h);
-    x[0] = ptx::ld_stream_v4(xw.p);
-    x[1] = ptx::ld_stream_v4(xw.p + across);
-    xw.step(kRows * xr.sh);
+    if (a.norm) {
+      if (live) xw.enter(xr, heads, u.ea, t, h);
+      p = live ? xw.p : static_cast<const T*>(xr.p);
+      cp_async16_if(ring.at(stage, 2), p, live);
+      cp_async16_if(ring.at(stage, 3), live ? p + across : p, live);
+      xw.step(kRows * xr.sh);
+    }
+    cp_commit();
   };
+#pragma unroll
+  for (int i = 0; i < kDeep; ++i) {
+    if (i < (int)n) fetch(i);
+    else cp_commit();
+  }
   const float rd = 1.f / (float)a.d;
   Turn<T> turn;
-  if (n > 0) fetch();
 #pragma unroll 1
   for (unsigned i = 0; i < n; ++i) {
     const bool live = row < rows;
@@ -630,12 +666,17 @@ qk_rope_backward_kernel(const __grid_constant__ QkBackArgs a, int q_blocks) {
       end = (t + 1) * heads;
       if (u.turned) turn.load(a.rope, a.positions[t], a.max_pos, a.r, j);
     }
+    cp_wait<kDeep - 1>();
+    const int stage = i % kDeep;
     Vec<T> xa, xb, ga, gb;
-    xa.from(x[0]);
-    xb.from(x[1]);
-    ga.from(g[0]);
-    gb.from(g[1]);
-    if (i + 1 < n) fetch();
+    ga.from(ring.get(stage, 0));
+    gb.from(ring.get(stage, 1));
+    if (a.norm) {
+      xa.from(ring.get(stage, 2));
+      xb.from(ring.get(stage, 3));
+    }
+    if (i + kDeep < n) fetch(stage);
+    else cp_commit();
     if (u.turned && live) turn.template apply<true>(ga, gb, a.interleaved);
     if (a.norm) {
       f2 ss = 0ull, sg = 0ull;
@@ -665,7 +706,9 @@ qk_rope_backward_kernel(const __grid_constant__ QkBackArgs a, int q_blocks) {
     row += kRows;
     y += kRows * a.d;
   }
+  cp_wait<0>();
   if (!a.norm) return;
+  __syncthreads();                  // every warp is done with its ring
   float fa[E], fb[E];
   da.floats(fa);
   db.floats(fb);
@@ -1006,7 +1049,9 @@ int rmsnorm_qk_rope_backward(const rmsnorm_qk_rope_backward_args* in, void* stre
                      : in->dtype == RMSNORM_TP_BF16 ? backward_fn<__nv_bfloat16>(lanes)
                                                     : backward_fn<__half>(lanes);
     void* args[] = {&a, &q_blocks};
-    const size_t smem = norm ? (size_t)kWarps * a.d * sizeof(float) : 0;
+    // the vector kernels' ring (at most 16 KB of dw lies over it)
+    const size_t sums = norm ? (size_t)kWarps * a.d * sizeof(float) : 0;
+    const size_t smem = lanes ? (size_t)kWarps * BackRing::kWarpBytes : sums;
     const cudaError_t e = launch_dependent(fn, dim3((unsigned)grid), dim3(kBlock), smem, args, st);
     if (e != cudaSuccess) return launch_failed(e, who);
   }
