@@ -128,6 +128,18 @@ __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+// Division of 32-bit numbers under 2^31 by a number that the host knows:
+// n / by = (umulhi(n, mul) + n) >> shift, with mul = floor(2^32 (2^shift - by) / by) + 1.
+struct FastDiv {
+  unsigned by, mul, shift;
+  static FastDiv of(unsigned by) {
+    unsigned shift = 0;   // ceil(log2(by))
+    while ((1ull << shift) < by) ++shift;
+    return FastDiv{by, (unsigned)(((1ull << 32) * ((1ull << shift) - by)) / by + 1), shift};
+  }
+  __device__ __forceinline__ unsigned quotient(unsigned n) const { return (__umulhi(n, mul) + n) >> shift; }
+};
+
 // Page and offset of a slot; 32-bit division where the cache's slots allow it.
 __device__ __forceinline__ void page_of(int64_t slot, int page, int64_t num_slots, int64_t& pg, int& off) {
   if (num_slots <= 0xFFFFFFFFll) {

@@ -68,76 +68,112 @@ struct ReadArgs {
   const int64_t* slots;
   int64_t num_slots, count;
   int page, heads, d;
+  FastDiv units, per_row, page_div;   // of a token (heads * d / 8), of a row (d / 8)
+  int small;                          // num_slots under 2^31
 };
 
 constexpr int kBlock = 256;
 
-// 8 elements from memory in fp32.
+// 8 elements of a cache row, zeros until they are loaded.
 template <typename TC>
-__device__ __forceinline__ void load8(const TC* p, float (&f)[8]) {
-  if constexpr (sizeof(TC) == 1) {
-    uint2 c;
-    asm("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(c.x), "=r"(c.y) : "l"(p));
-    const uint32_t w[2] = {c.x, c.y};
+struct Eight {
+  static constexpr int kWords = sizeof(TC) * 2;
+  uint32_t w[kWords] = {};
+  __device__ __forceinline__ void load(const TC* p) {
+    if constexpr (kWords == 2) {
+      asm("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 v = e4m3x2_to((unsigned short)(w[i / 2] >> (16 * (i & 1))));
-      f[2 * i] = v.x;
-      f[2 * i + 1] = v.y;
+      for (int i = 0; i < kWords; i += 4) {
+        const uint4 x = ptx::ld_stream_v4(reinterpret_cast<const uint32_t*>(p) + i);
+        w[i] = x.x, w[i + 1] = x.y, w[i + 2] = x.z, w[i + 3] = x.w;
+      }
     }
-  } else if constexpr (sizeof(TC) == 2) {
-    Pack<TC>::unpack(ptx::ld_stream_v4(p), f);
-  } else {
-    const uint4 a = ptx::ld_stream_v4(p), b = ptx::ld_stream_v4(p + 4);
-    const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  }
+  // Scaled (e4m3 only) and rounded once.
+  template <typename T>
+  __device__ __forceinline__ void store(T* p, float scale) const {
+    float f[8];
+    if constexpr (kWords == 2) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(w[e]);
+      for (int i = 0; i < 4; ++i) {
+        const float2 x = e4m3x2_to((unsigned short)(w[i / 2] >> (16 * (i & 1))));
+        f[2 * i] = x.x * scale;
+        f[2 * i + 1] = x.y * scale;
+      }
+    } else if constexpr (kWords == 4) {
+      Pack<TC>::unpack(make_uint4(w[0], w[1], w[2], w[3]), f);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(w[e]);
+    }
+    if constexpr (sizeof(T) == 2) {
+      ptx::st_v4(p, Pack<T>::pack(f));
+    } else {
+      const float a[4] = {f[0], f[1], f[2], f[3]}, b[4] = {f[4], f[5], f[6], f[7]};
+      ptx::st_v4(p, Pack<T>::pack(a));
+      ptx::st_v4(p + 4, Pack<T>::pack(b));
+    }
   }
-}
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&f)[8]) {
-  if constexpr (sizeof(T) == 2) {
-    ptx::st_v4(p, Pack<T>::pack(f));
-  } else {
-    const float a[4] = {f[0], f[1], f[2], f[3]}, b[4] = {f[4], f[5], f[6], f[7]};
-    ptx::st_v4(p, Pack<T>::pack(a));
-    ptx::st_v4(p + 4, Pack<T>::pack(b));
-  }
-}
+};
 
-// A thread brings 8 elements of K and of V of one row, so that a warp's 16-bit outputs
-// are 512 bytes in one piece. Bound by HBM: each row read once, written once.
+// A thread brings 8 elements of K and of V of one head of kTokens tokens, all asked for
+// before the first is used; a warp's 16-bit outputs are 512 bytes in one piece. Bound by
+// HBM: each row read once, written once.
+constexpr int kTokens = 4;
+
 template <typename TC, typename T>
 __global__ void __launch_bounds__(kBlock) kv_read_kernel(const __grid_constant__ ReadArgs a) {
   ptx::grid_dep_wait();
   ptx::grid_dep_launch_dependents();
-  const unsigned tid = thread_here();
-  const unsigned per_row = a.d / 8, rows = kBlock / per_row;   // 2 to 32; rows of this CTA
-  const unsigned r = tid / per_row, e0 = (tid - r * per_row) * 8;
-  const int64_t row = (int64_t)blockIdx.x * rows + r;
-  if (r >= rows || row >= a.count * a.heads) return;
-  const int64_t t = (unsigned)row / (unsigned)a.heads;   // at most 2^31 rows
-  const int h = (int)(row - t * a.heads);
-  const int64_t slot = a.slots[t];
-  float k[8] = {}, v[8] = {};
-  if (slot >= 0 && slot < a.num_slots) {
-    int64_t pg;
-    int off;
-    page_of(slot, a.page, a.num_slots, pg, off);
-    const int64_t at = (pg * a.heads + h) * a.page + off;
-    load8(static_cast<const TC*>(a.k) + at * a.d + e0, k);
-    load8(static_cast<const TC*>(a.v) + at * a.d + e0, v);
-    if constexpr (sizeof(TC) == 1) {
-      const float ks = a.ks[at], vs = a.vs[at];
+  const unsigned id = blockIdx.x * kBlock + thread_here();   // under 2^31
+  const unsigned group = a.units.quotient(id), unit = id - group * a.units.by;
+  const unsigned h = a.per_row.quotient(unit), e0 = (unit - h * a.per_row.by) * 8;
+  const int64_t t0 = (int64_t)group * kTokens;
+  if (t0 >= a.count) return;
+  const int n = a.count - t0 < kTokens ? (int)(a.count - t0) : kTokens;
+  int64_t at[kTokens];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        k[e] *= ks;
-        v[e] *= vs;
-      }
+  for (int i = 0; i < kTokens; ++i) at[i] = i < n ? a.slots[t0 + i] : -1;
+#pragma unroll
+  for (int i = 0; i < kTokens; ++i) {
+    if (at[i] < 0 || at[i] >= a.num_slots) {
+      at[i] = -1;
+      continue;
+    }
+    if (a.small) {
+      const unsigned pg = a.page_div.quotient((unsigned)at[i]);
+      at[i] = (int64_t)(pg * (uint64_t)a.heads + h) * a.page + ((unsigned)at[i] - pg * a.page);
+    } else {
+      const int64_t pg = at[i] / a.page;
+      at[i] = (pg * a.heads + h) * a.page + (at[i] - pg * a.page);
     }
   }
-  store8(static_cast<T*>(a.ko) + row * a.d + e0, k);
-  store8(static_cast<T*>(a.vo) + row * a.d + e0, v);
+  Eight<TC> k[kTokens], v[kTokens];
+  float ks[kTokens], vs[kTokens];
+#pragma unroll
+  for (int i = 0; i < kTokens; ++i) {
+    ks[i] = vs[i] = 1.f;
+    if (at[i] < 0) continue;
+    k[i].load(static_cast<const TC*>(a.k) + at[i] * a.d + e0);
+    v[i].load(static_cast<const TC*>(a.v) + at[i] * a.d + e0);
+    if constexpr (sizeof(TC) == 1) {
+      ks[i] = a.ks[at[i]];
+      vs[i] = a.vs[at[i]];
+    }
+  }
+  const int64_t step = (int64_t)a.heads * a.d;
+  T* ko = static_cast<T*>(a.ko) + t0 * step + (int64_t)h * a.d + e0;
+  T* vo = static_cast<T*>(a.vo) + t0 * step + (int64_t)h * a.d + e0;
+#pragma unroll
+  for (int i = 0; i < kTokens; ++i) {
+    if (i < n) {
+      k[i].template store<T>(ko, ks[i]);
+      v[i].template store<T>(vo, vs[i]);
+    }
+    ko += step;
+    vo += step;
+  }
 }
 
 template <typename T>
@@ -166,23 +202,39 @@ extern "C" int rmsnorm_kv_read(const rmsnorm_kv_cache* c, void* k_out, void* v_o
   if (rc != RMSNORM_TP_OK) return rc;
   if (dtype != RMSNORM_TP_F32 && dtype != RMSNORM_TP_BF16 && dtype != RMSNORM_TP_F16)
     return refuse(RMSNORM_TP_ERR_INVALID, "%s: unknown dtype %d", who, dtype);
-  if (count < 0 || count > (int64_t(1) << 31) / c->kv_heads)
-    return refuse(RMSNORM_TP_ERR_INVALID, "%s: %lld slots of %d heads: at most 2^31 rows", who,
-                  (long long)count, c->kv_heads);
+  // a thread for every 8 elements of 4 tokens, numbered in 31 bits
+  if (count < 0 || (count + kTokens) * (int64_t)c->kv_heads * (c->head_dim / 8) / kTokens >= (int64_t(1) << 31) - kBlock)
+    return refuse(RMSNORM_TP_ERR_INVALID, "%s: %lld slots of %d heads of %d: at most 2^36 elements", who,
+                  (long long)count, c->kv_heads, c->head_dim);
   if (count == 0) return RMSNORM_TP_OK;
   if (!k_out || !v_out || !slots) return refuse(RMSNORM_TP_ERR_INVALID, "%s: NULL tensor pointer", who);
   if ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15u)
     return refuse(RMSNORM_TP_ERR_INVALID, "%s: the outputs must be 16-byte aligned", who);
-  ReadArgs a{c->k,  c->v,  c->k_scale, c->v_scale, k_out, v_out, slots, c->num_pages * c->page_size,
-             count, c->page_size, c->kv_heads, c->head_dim};
+  ReadArgs a = {};
+  a.k = c->k;
+  a.v = c->v;
+  a.ks = c->k_scale;
+  a.vs = c->v_scale;
+  a.ko = k_out;
+  a.vo = v_out;
+  a.slots = slots;
+  a.num_slots = c->num_pages * c->page_size;
+  a.count = count;
+  a.page = c->page_size;
+  a.heads = c->kv_heads;
+  a.d = c->head_dim;
+  a.per_row = FastDiv::of(c->head_dim / 8);
+  a.units = FastDiv::of((unsigned)c->kv_heads * (c->head_dim / 8));
+  a.page_div = FastDiv::of(c->page_size);
+  a.small = a.num_slots < (int64_t(1) << 31);
   OnDevice on(device);
   if (on.err != cudaSuccess) return launch_failed(on.err, who);
   const void* fn = dtype == RMSNORM_TP_F32    ? read_fn<float>(c->dtype)
                    : dtype == RMSNORM_TP_BF16 ? read_fn<__nv_bfloat16>(c->dtype)
                                               : read_fn<__half>(c->dtype);
-  const int64_t per_block = kBlock / (c->head_dim / 8), rows = count * c->kv_heads;
+  const int64_t threads = (count + kTokens - 1) / kTokens * a.units.by;
   void* args[] = {&a};
-  const cudaError_t e = launch_dependent(fn, dim3((unsigned)((rows + per_block - 1) / per_block)),
-                                         dim3(kBlock), 0, args, reinterpret_cast<cudaStream_t>(stream));
+  const cudaError_t e = launch_dependent(fn, dim3((unsigned)((threads + kBlock - 1) / kBlock)), dim3(kBlock),
+                                         0, args, reinterpret_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? RMSNORM_TP_OK : launch_failed(e, who);
 }

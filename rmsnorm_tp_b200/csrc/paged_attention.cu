@@ -29,7 +29,7 @@ struct AttnArgs {
   int segments;         // kv heads * row_groups
   int q_pairs;          // the queries' elements can be read two at a time
   int whole_pages;      // pages of 16 k tokens
-  unsigned page_mul, page_shift;   // t / page = (umulhi(t, mul) + t) >> shift for t < 2^31
+  FastDiv page_div;
   float scale_log2;     // scale * log2(e): scores in base 2
 };
 
@@ -414,7 +414,7 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
   // else lane l (and l + 16) knows the row of token l
   auto look_up = [&]() {
     const int t = ahead.tile * kTile + lane_tok;
-    const unsigned pg = (__umulhi((unsigned)t, a.page_mul) + (unsigned)t) >> a.page_shift;
+    const unsigned pg = a.page_div.quotient(t);
     page_off = t - (int)pg * a.page;
     page_id = t < ahead.len ? a.table[ahead.b * a.table_stride + pg] : -1;
   };
@@ -1044,10 +1044,7 @@ int rmsnorm_paged_attention(const rmsnorm_paged_attention_args* in, void* stream
     a.row_groups = row_groups_of(in, k);
     a.segments = a.hk * a.row_groups;
     a.whole_pages = a.page % 16 == 0;
-    unsigned shift = 0;   // ceil(log2(page))
-    while ((1ull << shift) < (unsigned)a.page) ++shift;
-    a.page_shift = shift;
-    a.page_mul = (unsigned)(((1ull << 32) * ((1ull << shift) - (unsigned)a.page)) / (unsigned)a.page + 1);
+    a.page_div = FastDiv::of(a.page);
     if (in->device >= kMaxDevices || !k.ready[in->device]) {
       const cudaError_t e =
           cudaFuncSetAttribute(k.main, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem);

@@ -398,29 +398,6 @@ __device__ __forceinline__ float lanes_max(float v) {
   return v;
 }
 
-// Rows of one operand ([tokens, heads] numbered token by token) on their way through a
-// warp: a lane walks down every (32 / L)-th row by a pointer, made anew where the token
-// changes.
-template <typename T, int kRows>
-struct Walk {
-  unsigned row, end = 0;                 // end: first row of the next token
-  const T* p = nullptr;
-  __device__ __forceinline__ explicit Walk(unsigned first) : row(first) {}
-  // Whether the row is a new token's (its t and h are set then); p as for element e0.
-  __device__ __forceinline__ bool enter(const Rows& in, unsigned heads, int e0, unsigned& t, unsigned& h) {
-    if (row < end) return false;
-    t = row / heads;
-    h = row - t * heads;
-    end = (t + 1) * heads;
-    p = static_cast<const T*>(in.p) + t * in.st + (int64_t)h * in.sh + e0;
-    return true;
-  }
-  __device__ __forceinline__ void step(int64_t stride) {
-    row += kRows;
-    p += stride;
-  }
-};
-
 // What becomes of an operand's rows.
 enum Out { kRowsOut, kCacheOut };
 
@@ -434,6 +411,13 @@ struct Ring {
   __device__ __forceinline__ Ring(void* smem, int warp, int lane)
       : base(ptx::smem_addr(smem) + warp * kWarpBytes + lane * 16) {}
   __device__ __forceinline__ uint32_t at(int stage, int vec) const { return base + (stage * kVecs + vec) * 512; }
+  __device__ __forceinline__ static int after(int stage) { return stage + 1 == kStages ? 0 : stage + 1; }
+  // For lanes that no copy is made for.
+  __device__ __forceinline__ void zero() const {
+#pragma unroll
+    for (int i = 0; i < kStages * kVecs; ++i)
+      asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(base + i * 512), "r"(0) : "memory");
+  }
   __device__ __forceinline__ uint4 get(int stage, int vec) const {
     uint4 v;
     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
@@ -460,17 +444,25 @@ __device__ __forceinline__ void qk_rope_rows(const QkArgs& a, const Rows& in, co
   const unsigned first = warp * (unsigned)run * kRows + lane / L;
   const int64_t in_step = kRows * in.sh;
   const int across = u.eb - u.ea;
-  Walk<T, kRows> ahead(first);
+  // the lane walks down its rows ([tokens, heads] numbered token by token) by a pointer that
+  // is made anew where the token changes
+  unsigned ahead = first, ahead_end = 0;
+  const T* from = nullptr;
   auto fetch = [&](int stage) {
-    const bool live = ahead.row < rows && u.on;
-    unsigned t, h;
-    if (live) ahead.enter(in, heads, u.ea, t, h);
-    const T* p = live ? ahead.p : static_cast<const T*>(in.p);
-    cp_async16_if(ring.at(stage, 0), p, live);
-    cp_async16_if(ring.at(stage, 1), live ? p + across : p, live);
+    if (ahead < rows && u.on) {
+      if (ahead >= ahead_end) {
+        const unsigned t = ahead / heads, h = ahead - t * heads;
+        ahead_end = ahead - h + heads;
+        from = static_cast<const T*>(in.p) + t * in.st + (int64_t)h * in.sh + u.ea;
+      }
+      cp_async16(ring.at(stage, 0), from);
+      cp_async16(ring.at(stage, 1), from + across);
+      from += in_step;
+    }
     cp_commit();
-    ahead.step(in_step);
+    ahead += kRows;
   };
+  if (!u.on) ring.zero();
 #pragma unroll
   for (int i = 0; i < kDeep; ++i) {
     if (i < run) fetch(i);
@@ -484,21 +476,22 @@ __device__ __forceinline__ void qk_rope_rows(const QkArgs& a, const Rows& in, co
   }
   const float rd = 1.f / (float)a.d;
   unsigned row = first, end = 0;
+  int stage = 0;
   T* to = nullptr;
   int64_t at = 0;                        // cache row
   bool keep = kOut == kRowsOut;
   const int64_t to_step = kOut == kRowsOut ? kRows * out.sh : (int64_t)kRows * a.page * a.d;
 #pragma unroll 1
   for (int i = 0; i < run; ++i) {
-    const int k = i % kDeep;
     if (!__any_sync(0xFFFFFFFFu, row < rows)) break;
     const bool live = row < rows;
     cp_wait<kDeep - 1>();
     Vec<T> ya, yb;
-    ya.from(ring.get(k, 0));
-    yb.from(ring.get(k, 1));
-    if (i + kDeep < run) fetch(k);
+    ya.from(ring.get(stage, 0));
+    yb.from(ring.get(stage, 1));
+    if (i + kDeep < run) fetch(stage);
     else cp_commit();
+    stage = ring.after(stage);
     if (row >= end && live) {
       const unsigned t = row / heads, h = row - t * heads;
       end = row - h + heads;
@@ -633,24 +626,31 @@ qk_rope_backward_kernel(const __grid_constant__ QkBackArgs a, int q_blocks) {
   const unsigned n = (unsigned)((uint64_t)groups * (me + 1) / workers) - first;
   unsigned row = first * kRows + lane / L, end = 0;
   T* y = static_cast<T*>(is_q ? a.dq : a.dk) + (int64_t)row * a.d + u.ea;
-  Walk<T, kRows> gw(row), xw(row);
+  unsigned ahead = row, ahead_end = 0;
+  const T* gp = nullptr;
+  const T* xp = nullptr;
+  const int64_t g_step = kRows * gr.sh, x_step = kRows * xr.sh;
   auto fetch = [&](int stage) {
-    const bool live = gw.row < rows && u.on;
-    unsigned t, h;
-    if (live) gw.enter(gr, heads, u.ea, t, h);
-    const T* p = live ? gw.p : static_cast<const T*>(gr.p);
-    cp_async16_if(ring.at(stage, 0), p, live);
-    cp_async16_if(ring.at(stage, 1), live ? p + across : p, live);
-    gw.step(kRows * gr.sh);
-    if (a.norm) {
-      if (live) xw.enter(xr, heads, u.ea, t, h);
-      p = live ? xw.p : static_cast<const T*>(xr.p);
-      cp_async16_if(ring.at(stage, 2), p, live);
-      cp_async16_if(ring.at(stage, 3), live ? p + across : p, live);
-      xw.step(kRows * xr.sh);
+    if (ahead < rows && u.on) {
+      if (ahead >= ahead_end) {
+        const unsigned t = ahead / heads, h = ahead - t * heads;
+        ahead_end = ahead - h + heads;
+        gp = static_cast<const T*>(gr.p) + t * gr.st + (int64_t)h * gr.sh + u.ea;
+        xp = static_cast<const T*>(xr.p) + t * xr.st + (int64_t)h * xr.sh + u.ea;
+      }
+      cp_async16(ring.at(stage, 0), gp);
+      cp_async16(ring.at(stage, 1), gp + across);
+      gp += g_step;
+      if (a.norm) {
+        cp_async16(ring.at(stage, 2), xp);
+        cp_async16(ring.at(stage, 3), xp + across);
+        xp += x_step;
+      }
     }
     cp_commit();
+    ahead += kRows;
   };
+  if (!u.on) ring.zero();
 #pragma unroll
   for (int i = 0; i < kDeep; ++i) {
     if (i < (int)n) fetch(i);
@@ -658,6 +658,7 @@ qk_rope_backward_kernel(const __grid_constant__ QkBackArgs a, int q_blocks) {
   }
   const float rd = 1.f / (float)a.d;
   Turn<T> turn;
+  int stage = 0;
 #pragma unroll 1
   for (unsigned i = 0; i < n; ++i) {
     const bool live = row < rows;
@@ -667,8 +668,7 @@ qk_rope_backward_kernel(const __grid_constant__ QkBackArgs a, int q_blocks) {
       if (u.turned) turn.load(a.rope, a.positions[t], a.max_pos, a.r, j);
     }
     cp_wait<kDeep - 1>();
-    const int stage = i % kDeep;
-    Vec<T> xa, xb, ga, gb;
+    Vec<T> xa = {}, xb = {}, ga, gb;
     ga.from(ring.get(stage, 0));
     gb.from(ring.get(stage, 1));
     if (a.norm) {
@@ -677,6 +677,8 @@ qk_rope_backward_kernel(const __grid_constant__ QkBackArgs a, int q_blocks) {
     }
     if (i + kDeep < n) fetch(stage);
     else cp_commit();
+    stage = ring.after(stage);
+    if (!live) xa = xb = ga = gb = Vec<T>{};   // behind the last row: nothing for dw
     if (u.turned && live) turn.template apply<true>(ga, gb, a.interleaved);
     if (a.norm) {
       f2 ss = 0ull, sg = 0ull;
