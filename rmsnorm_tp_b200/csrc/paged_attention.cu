@@ -160,9 +160,10 @@ __global__ void __launch_bounds__(kAnyBlock) attention_join_any_kernel(const __g
 // in the loop; the loads run ahead over the borders of sequences); the warps' results are
 // joined at a sequence's end.
 //
-// All (sequence, kv head, 8 or 16 query heads) are laid behind one another in tiles, and
-// each CTA takes an equal run of tiles, from the lengths on the device: ragged batches
-// balance to a tile and nothing on the host knows a length. A run that ends inside a
+// All (sequence, kv head, 8 or 16 query heads) are laid behind one another in tiles, each
+// with one share more for its begin and end, and each CTA takes an equal run of shares, from
+// the lengths on the device: ragged batches balance to a tile and nothing on the host knows
+// a length. A run that ends inside a
 // sequence leaves its reference, sum and o in the workspace (at most two such parts for
 // each CTA), and the join kernel adds them in CTA order.
 //
@@ -173,6 +174,7 @@ constexpr int kWarps = 4;
 constexpr int kBlock = 32 * kWarps;
 constexpr int kTile = 16 * kWarps;      // tokens of a CTA's tile
 constexpr float kSlack = 8.f;           // log2 of the largest exponential
+constexpr int kSegment = 1;             // cost of a segment's begin and end, in tiles
 
 // A segment (query heads of one kv head of one sequence) whose tiles several CTAs have:
 // `owner` to `last`; owner < 0: none.
@@ -196,11 +198,14 @@ struct Shape {
   static constexpr int kRowsAtOnce = 32 / kLanes;
   static constexpr int kJoinPitch = D / 2 + 4;
   static constexpr int kJoin = kWarps * 8 * kJoinPitch * 4;
-  // two CTAs of at most 110 KB on an SM where at least three stages fit, else one
+  // three CTAs of at most 73 KB on an SM (and 168 registers a thread: NG = 1) where at
+  // least three stages fit, else two of 110 KB, else one
+  static constexpr int kThree = NG == 1 ? (73 * 1024 - kJoin) / (kWarps * kStage) : 0;
   static constexpr int kTwo = (110 * 1024 - kJoin) / (kWarps * kStage);
   static constexpr int kOne = (220 * 1024 - kJoin) / (kWarps * kStage);
-  static constexpr int kCtas = kTwo >= 3 ? 2 : 1;
-  static constexpr int kStages = kCtas == 2 ? (kTwo > 6 ? 6 : kTwo) : (kOne > 6 ? 6 : kOne);
+  static constexpr int kCtas = kThree >= 3 ? 3 : kTwo >= 3 ? 2 : 1;
+  static constexpr int kFit = kCtas == 3 ? kThree : kCtas == 2 ? kTwo : kOne;
+  static constexpr int kStages = kFit > 6 ? 6 : kFit;
   static constexpr int kSmem = kJoin + kWarps * kStages * kStage;
   static_assert(kStages >= 3, "the ring needs three stages");
 };
@@ -286,8 +291,10 @@ __device__ __forceinline__ float ref_of(float m) { return m == -INFINITY ? 0.f :
 
 // Place in the row of tiles: tile `tile` of the `tiles` of segment (sequence b, kv head,
 // group of its query heads).
+// `rem`: what is left of the CTA's run, from this tile on.
 struct Place {
   int b, kvh, rg, tile, tiles, len;
+  int64_t rem;
 };
 
 // a / b of non-negative numbers, in 32 bits where they fit (a 64-bit division takes some
@@ -299,9 +306,15 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
 
 __device__ __forceinline__ int tiles_of(int64_t len) { return (int)((len + kTile - 1) / kTile); }
 
-// To the next tile; the caller knows that there is one.
+// Shares of a sequence's segment: its tiles, and kSegment for its queries and its join.
+__device__ __forceinline__ int64_t shares_of(int64_t len) { return len == 0 ? 0 : tiles_of(len) + kSegment; }
+
+// To the next tile, if rem says that there is one.
 __device__ __forceinline__ void advance(const AttnArgs& a, Place& p) {
+  --p.rem;
   if (++p.tile < p.tiles) return;
+  p.rem -= kSegment;
+  if (p.rem <= 0) return;
   p.tile = 0;
   if (++p.rg < a.row_groups) return;
   p.rg = 0;
@@ -339,11 +352,11 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
   const int tid = thread_here(), lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, qd = lane & 3;
 
-  // this CTA's run of tiles [t0, t1): every thread sums the tiles of a run of sequences
+  // this CTA's run of shares [t0, t1): every thread sums those of a run of sequences
   const int64_t per = (a.batch + kBlock - 1) / kBlock;
   int64_t mine = 0;
   for (int64_t b = tid * per; b < (tid + 1) * per && b < a.batch; ++b)
-    mine += (int64_t)tiles_of(length_of(a, b)) * a.segments;
+    mine += shares_of(length_of(a, b)) * a.segments;
   int64_t upto = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -362,18 +375,18 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
   Seg* meta = reinterpret_cast<Seg*>(a.part) + 2 * me;   // the segment that began before, and one left open
   if (tid < 2) meta[tid] = Seg{0, 0, -1, -1};
   if (me >= workers) return;
-  // the first `more` CTAs have one tile more than the others
+  // the first `more` CTAs have one share more than the others
   const int64_t each = quotient(total, workers), more = total - each * workers;
   const int64_t t0 = me * each + (me < more ? me : more), t1 = t0 + each + (me < more ? 1 : 0);
-  auto worker_of = [&](int64_t tile) {
+  auto worker_of = [&](int64_t share) {
     const int64_t line = more * (each + 1);
-    return (int)(tile < line ? quotient(tile, each + 1) : more + quotient(tile - line, each));
+    return (int)(share < line ? quotient(share, each + 1) : more + quotient(share - line, each));
   };
   if (upto - mine <= t0 && t0 < upto) {
     int64_t rest = t0 - (upto - mine);
     int64_t b = tid * per;
     for (;; ++b) {
-      const int64_t n = (int64_t)tiles_of(length_of(a, b)) * a.segments;
+      const int64_t n = shares_of(length_of(a, b)) * a.segments;
       if (rest < n) break;
       rest -= n;
     }
@@ -385,11 +398,13 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
   at.b = s_b;
   at.len = (int)length_of(a, at.b);
   at.tiles = tiles_of(at.len);
-  const int hs = (int)quotient(s_rest, at.tiles);
-  at.tile = (int)(s_rest - (int64_t)hs * at.tiles);
+  const int hs = (int)quotient(s_rest, at.tiles + kSegment);
+  const int into_segment = (int)(s_rest - (int64_t)hs * (at.tiles + kSegment)) - kSegment;
+  at.tile = into_segment > 0 ? into_segment : 0;
+  at.rem = t1 - t0 + (into_segment < 0 ? into_segment : 0);
+  if (at.rem <= 0) return;              // a run of nothing but a segment's extra share
   at.kvh = hs / a.row_groups;
   at.rg = hs - at.kvh * a.row_groups;
-  const int n = (int)(t1 - t0);
   if (tid == 0 && at.tile > 0)
     meta[0] = Seg{at.b, hs, worker_of(t0 - at.tile), worker_of(t0 - at.tile + at.tiles - 1)};
 
@@ -407,7 +422,6 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
   const uint32_t to1 = lr * S::kPitch + (S::kSwizzle ? lc ^ ((lr + S::kRowsAtOnce) & 7) : lc) * 16;
   const int lane_tok = warp * 16 + (a.whole_pages ? 0 : lane & 15);
   Place ahead = at;
-  int left = n;                       // tiles not yet asked for
   uint32_t into = 0;                  // stage that the next tile goes to
   int32_t page_id = -1, page_off = 0; // read one tile early
   // pages of 16 k tokens: the warp's 16 tokens lie in one page, one row behind another;
@@ -420,7 +434,7 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
   };
   look_up();
   auto send = [&]() {
-    if (left > 0) {
+    if (ahead.rem > 0) {
       const uint32_t dst = ring + into * S::kStage;
       const bool live = (unsigned)page_id < (unsigned)a.num_pages;
       const int64_t row = live ? ((int64_t)page_id * a.hk + ahead.kvh) * a.page + page_off : 0;
@@ -463,10 +477,8 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
         }
       }
       into = into + 1 == S::kStages ? 0 : into + 1;
-      if (--left > 0) {
-        advance(a, ahead);
-        look_up();
-      }
+      advance(a, ahead);
+      if (ahead.rem > 0) look_up();
     }
     cp_commit();
   };
@@ -486,31 +498,38 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
   const uint32_t v_chunk = kE4M3 ? k_chunk : (lane >> 3) & 1;
   const uint32_t k_row = k_tok * S::kPitch, v_row = S::kOperand + v_tok * S::kPitch;
 
+  const int group = a.hq / a.hk;
+  auto load_q = [&](const Place& p) {
+    const int first = p.rg * kRows, rows = min(kRows, group - first);
+    const unsigned short* qu = static_cast<const unsigned short*>(a.q) + p.b * a.qst +
+                               (int64_t)(p.kvh * group + first) * a.qsh;
+#pragma unroll
+    for (int x = 0; x < NG; ++x)
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int r = 8 * x + g;
+          // e4m3: a thread's four K codes are neighbours, so its k index runs 4 qd .. 4 qd + 3
+          const int e = ks * 16 + (kE4M3 ? 4 * qd + 2 * j : 2 * qd + 8 * j);
+          uint32_t v = 0;
+          if (r < rows) {
+            const unsigned short* at = qu + r * a.qsh + e;
+            v = a.q_pairs ? *reinterpret_cast<const uint32_t*>(at) : at[0] | (uint32_t)at[1] << 16;
+          }
+          q[x][ks][j] = v;
+        }
+  };
+  load_q(at);
 #pragma unroll 1
-  for (int i = 0; i < n;) {
+  while (at.rem > 0) {
     // ---- a segment, or what this CTA has of it ----
     const bool began = at.tile == 0;
-    const int group = a.hq / a.hk, first = at.rg * kRows, rows = min(kRows, group - first);
-    const int end = min(at.tiles, at.tile + (n - i));
+    const int first = at.rg * kRows, rows = min(kRows, group - first);
+    const int end = (int)min((int64_t)at.tiles, at.tile + at.rem);
     {
-      const unsigned short* qu = static_cast<const unsigned short*>(a.q) + at.b * a.qst +
-                                 (int64_t)(at.kvh * group + first) * a.qsh;
 #pragma unroll
       for (int x = 0; x < NG; ++x) {
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int r = 8 * x + g;
-            // e4m3: a thread's four K codes are neighbours, so its k index runs 4 qd .. 4 qd + 3
-            const int e = ks * 16 + (kE4M3 ? 4 * qd + 2 * j : 2 * qd + 8 * j);
-            uint32_t v = 0;
-            if (r < rows) {
-              const unsigned short* p = qu + r * a.qsh + e;
-              v = a.q_pairs ? *reinterpret_cast<const uint32_t*>(p) : p[0] | (uint32_t)p[1] << 16;
-            }
-            q[x][ks][j] = v;
-          }
         unit[x][0] = unit[x][1] = a.scale_log2;
         if constexpr (kE4M3) {
           // fp16 beside the fp16 that the codes become: each head scaled by a power of two so
@@ -689,7 +708,12 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
     }
 
     const bool last = end == at.tiles, whole = began && last;
-    i += end - at.tile;
+    // the next segment's queries, asked for before the join
+    Place next = at;
+    next.tile = end - 1;
+    next.rem = at.rem - (end - 1 - at.tile);
+    advance(a, next);
+    if (next.rem > 0) load_q(next);
     {
       // ---- the warps' results of the segment, joined: half of 8 heads' elements at a time
 #pragma unroll
@@ -770,40 +794,37 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
         }
       }
     }
-    if (i < n) {
-      at.tile = at.tiles - 1;
-      advance(a, at);
-    }
+    at = next;
   }
   cp_wait<0>();
 }
 
-// Joins what the CTAs left of a segment. Every CTA that had a part of it takes an equal
-// share of its elements over all parts: 4 elements of a head for a thread, the parts
-// divided over neighbouring threads. A thread's (reference, sum, elements) and its
-// neighbours' are joined as a softmax's halves are, in a fixed tree.
+// Joins what the CTAs left of a segment: every CTA that had a part of it takes an equal
+// share of its elements over all parts. A thread adds 4 elements of a head over some of the
+// parts (neighbouring threads the others), then the threads and warps of these
+// elements are added in a fixed order. Bound by latency (a few L2 round trips), so it is
+// kept short rather than unrolled.
 constexpr int kJoinBlock = 256;
 
+// Reference, sum and 4 elements of a softmax over some of the tokens.
 struct Part {
-  float m, l;
-  float4 y;
-  __device__ __forceinline__ void add(float m2, float l2, const float4& y2) {
-    const float top = fmaxf(m, m2), ref = ref_of(top);
-    const float f = ex2(m - ref), f2 = ex2(m2 - ref);
+  float m, v[5];
+  __device__ __forceinline__ void to(float top) {
+    const float f = ex2(m - ref_of(top));
     m = top;
-    l = l * f + l2 * f2;
-    y.x = y.x * f + y2.x * f2;
-    y.y = y.y * f + y2.y * f2;
-    y.z = y.z * f + y2.z * f2;
-    y.w = y.w * f + y2.w * f2;
+#pragma unroll
+    for (int j = 0; j < 5; ++j) v[j] *= f;
+  }
+  __device__ __forceinline__ void add(const Part& p) {
+#pragma unroll
+    for (int j = 0; j < 5; ++j) v[j] += p.v[j];
   }
 };
 
 template <typename TQ, int D, int NG>
 __global__ void __launch_bounds__(kJoinBlock) attention_join_kernel(const __grid_constant__ AttnArgs a) {
   constexpr int kRows = 8 * NG, kUnits = D / 4;
-  __shared__ float s_m[kJoinBlock / 32], s_l[kJoinBlock / 32];
-  __shared__ float4 s_y[kJoinBlock / 32];
+  __shared__ Part s_part[kJoinBlock / 32];
   ptx::grid_dep_wait();
   ptx::grid_dep_launch_dependents();
   const int tid = thread_here();
@@ -817,53 +838,66 @@ __global__ void __launch_bounds__(kJoinBlock) attention_join_kernel(const __grid
   for (int which = 0; which < 2; ++which) {
     const Seg seg{both[which].x, both[which].y, both[which].z, both[which].w};
     if (seg.owner < 0) continue;
-    const int kvh = seg.hs / a.row_groups, first = (seg.hs - kvh * a.row_groups) * kRows;
+    const int kvh = a.row_groups == 1 ? seg.hs : seg.hs / a.row_groups;
+    const int first = (seg.hs - kvh * a.row_groups) * kRows;
     const int rows = min(kRows, group - first), parts = seg.last - seg.owner + 1, p = (int)me - seg.owner;
     const int u0 = rows * kUnits * p / parts, u1 = rows * kUnits * (p + 1) / parts;
     // threads of one unit: a power of two, no more than half of them idle
     int lg = 0;
     while ((2 << lg) * (u1 - u0) <= kJoinBlock && (1 << lg) < parts) ++lg;
     const int slices = 1 << lg, at_once = kJoinBlock >> lg;
+#pragma unroll 1
     for (int ub = u0; ub < u1; ub += at_once) {
-      const int u = ub + (tid >> lg), r = u / kUnits, e = (u - r * kUnits) * 4;
-      Part mine{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+      const int u = ub + (tid >> lg), r = u / kUnits, e = (u % kUnits) * 4;
+      Part mine{-INFINITY, {0.f, 0.f, 0.f, 0.f, 0.f}};
       if (u < u1) {
-#pragma unroll 4
+#pragma unroll 2
         for (int i = tid & (slices - 1); i < parts; i += slices) {
           const int64_t at = (2ll * (seg.owner + i) + (i == 0 ? 1 : 0)) * kRows + r;
           const float2 ml = *reinterpret_cast<const float2*>(pm + at * 2);
-          mine.add(ml.x, ml.y, *reinterpret_cast<const float4*>(po + at * D + e));
+          const float4 y = *reinterpret_cast<const float4*>(po + at * D + e);
+          Part one{ml.x, {ml.y, y.x, y.y, y.z, y.w}};
+          const float top = fmaxf(mine.m, ml.x);
+          mine.to(top);
+          one.to(top);
+          mine.add(one);
         }
       }
-      for (int o = min(slices, 32) >> 1; o > 0; o >>= 1) {
-        const float m2 = __shfl_xor_sync(0xFFFFFFFFu, mine.m, o), l2 = __shfl_xor_sync(0xFFFFFFFFu, mine.l, o);
-        const float4 y2 = make_float4(__shfl_xor_sync(0xFFFFFFFFu, mine.y.x, o), __shfl_xor_sync(0xFFFFFFFFu, mine.y.y, o),
-                                      __shfl_xor_sync(0xFFFFFFFFu, mine.y.z, o), __shfl_xor_sync(0xFFFFFFFFu, mine.y.w, o));
-        mine.add(m2, l2, y2);
-      }
+      const int lanes = min(slices, 32);
+      float top = mine.m;
+#pragma unroll 1
+      for (int o = lanes >> 1; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+      mine.to(top);
+#pragma unroll 1
+      for (int o = lanes >> 1; o > 0; o >>= 1)
+#pragma unroll
+        for (int j = 0; j < 5; ++j) mine.v[j] += __shfl_xor_sync(0xFFFFFFFFu, mine.v[j], o);
       if (slices > 32) {              // several warps for one unit
         __syncthreads();
-        if ((tid & 31) == 0) {
-          s_m[tid >> 5] = mine.m;
-          s_l[tid >> 5] = mine.l;
-          s_y[tid >> 5] = mine.y;
-        }
+        if ((tid & 31) == 0) s_part[tid >> 5] = mine;
         __syncthreads();
-        if ((tid & (slices - 1)) == 0)
+        if ((tid & (slices - 1)) == 0) {
+          const Part* others = s_part + (tid >> 5);
+#pragma unroll 1
+          for (int w = 1; w < slices / 32; ++w) top = fmaxf(top, others[w].m);
+          mine.to(top);
+#pragma unroll 1
           for (int w = 1; w < slices / 32; ++w) {
-            const int v = (tid >> 5) + w;
-            mine.add(s_m[v], s_l[v], s_y[v]);
+            Part other = others[w];
+            other.to(top);
+            mine.add(other);
           }
+        }
       }
       if (u < u1 && (tid & (slices - 1)) == 0) {
         const int64_t row = (int64_t)seg.b * a.hq + kvh * group + first + r;
-        const float d = mine.l == 0.f ? 1.f : mine.l;
+        const float over = 1.f / (mine.v[0] == 0.f ? 1.f : mine.v[0]);   // no weight at all: o is 0
         constexpr bool kQBf16 = __is_same(TQ, __nv_bfloat16);
         uint2 out;
-        out.x = pack2<kQBf16>(mine.y.x / d, mine.y.y / d);
-        out.y = pack2<kQBf16>(mine.y.z / d, mine.y.w / d);
+        out.x = pack2<kQBf16>(mine.v[1] * over, mine.v[2] * over);
+        out.y = pack2<kQBf16>(mine.v[3] * over, mine.v[4] * over);
         *reinterpret_cast<uint2*>(static_cast<TQ*>(a.out) + row * D + e) = out;
-        if (a.lse && e == 0) a.lse[row] = kLn2 * (ref_of(mine.m) + log2f(mine.l));
+        if (a.lse && e == 0) a.lse[row] = kLn2 * (ref_of(top) + log2f(mine.v[0]));
       }
     }
   }

@@ -412,11 +412,11 @@ struct Ring {
       : base(ptx::smem_addr(smem) + warp * kWarpBytes + lane * 16) {}
   __device__ __forceinline__ uint32_t at(int stage, int vec) const { return base + (stage * kVecs + vec) * 512; }
   __device__ __forceinline__ static int after(int stage) { return stage + 1 == kStages ? 0 : stage + 1; }
-  // For lanes that no copy is made for.
-  __device__ __forceinline__ void zero() const {
+  // In place of a copy that is not made.
+  __device__ __forceinline__ void zero(int stage) const {
 #pragma unroll
-    for (int i = 0; i < kStages * kVecs; ++i)
-      asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(base + i * 512), "r"(0) : "memory");
+    for (int i = 0; i < kVecs; ++i)
+      asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at(stage, i)), "r"(0) : "memory");
   }
   __device__ __forceinline__ uint4 get(int stage, int vec) const {
     uint4 v;
@@ -458,11 +458,12 @@ __device__ __forceinline__ void qk_rope_rows(const QkArgs& a, const Rows& in, co
       cp_async16(ring.at(stage, 0), from);
       cp_async16(ring.at(stage, 1), from + across);
       from += in_step;
+    } else {
+      ring.zero(stage);
     }
     cp_commit();
     ahead += kRows;
   };
-  if (!u.on) ring.zero();
 #pragma unroll
   for (int i = 0; i < kDeep; ++i) {
     if (i < run) fetch(i);
@@ -646,11 +647,12 @@ qk_rope_backward_kernel(const __grid_constant__ QkBackArgs a, int q_blocks) {
         cp_async16(ring.at(stage, 3), xp + across);
         xp += x_step;
       }
+    } else {
+      ring.zero(stage);
     }
     cp_commit();
     ahead += kRows;
   };
-  if (!u.on) ring.zero();
 #pragma unroll
   for (int i = 0; i < kDeep; ++i) {
     if (i < (int)n) fetch(i);
@@ -668,9 +670,10 @@ qk_rope_backward_kernel(const __grid_constant__ QkBackArgs a, int q_blocks) {
       if (u.turned) turn.load(a.rope, a.positions[t], a.max_pos, a.r, j);
     }
     cp_wait<kDeep - 1>();
-    Vec<T> xa = {}, xb = {}, ga, gb;
+    Vec<T> xa, xb, ga, gb;              // zeros behind the last row
     ga.from(ring.get(stage, 0));
     gb.from(ring.get(stage, 1));
+    if (u.turned && live) turn.template apply<true>(ga, gb, a.interleaved);
     if (a.norm) {
       xa.from(ring.get(stage, 2));
       xb.from(ring.get(stage, 3));
@@ -678,8 +681,6 @@ qk_rope_backward_kernel(const __grid_constant__ QkBackArgs a, int q_blocks) {
     if (i + kDeep < n) fetch(stage);
     else cp_commit();
     stage = ring.after(stage);
-    if (!live) xa = xb = ga = gb = Vec<T>{};   // behind the last row: nothing for dw
-    if (u.turned && live) turn.template apply<true>(ga, gb, a.interleaved);
     if (a.norm) {
       f2 ss = 0ull, sg = 0ull;
 #pragma unroll
