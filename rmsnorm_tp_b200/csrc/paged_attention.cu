@@ -174,12 +174,15 @@ constexpr int kWarps = 4;
 constexpr int kBlock = 32 * kWarps;
 constexpr int kTile = 16 * kWarps;      // tokens of a CTA's tile
 constexpr float kSlack = 8.f;           // log2 of the largest exponential
+constexpr int kJoinBlock = 256;         // threads of the join kernel
 constexpr int kSegment = 1;             // cost of a segment's begin and end, in tiles
 
-// A segment (query heads of one kv head of one sequence) whose tiles several CTAs have:
-// `owner` to `last`; owner < 0: none.
-struct alignas(16) Seg {
-  int32_t b, hs, owner, last;
+// One CTA's share in the join of a segment (query heads of one kv head of one sequence)
+// whose tiles `parts` CTAs from `owner` on have: units (4 elements) [u0, u1) of its rows
+// from `row` on, 2^lg threads for each. parts == 0: none.
+struct alignas(16) Share {
+  int64_t row;
+  int32_t owner, parts, u0, u1, lg, pad;
 };
 
 template <int D, bool kE4M3, int NG>
@@ -372,8 +375,8 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
   }
   const int64_t workers = total < gridDim.x ? total : gridDim.x;
   const int64_t me = blockIdx.x;
-  Seg* meta = reinterpret_cast<Seg*>(a.part) + 2 * me;   // the segment that began before, and one left open
-  if (tid < 2) meta[tid] = Seg{0, 0, -1, -1};
+  Share* meta = reinterpret_cast<Share*>(a.part) + 2 * me;   // of the segment that began before, and one left open
+  if (tid < 2) meta[tid].parts = 0;
   if (me >= workers) return;
   // the first `more` CTAs have one share more than the others
   const int64_t each = quotient(total, workers), more = total - each * workers;
@@ -405,8 +408,19 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
   if (at.rem <= 0) return;              // a run of nothing but a segment's extra share
   at.kvh = hs / a.row_groups;
   at.rg = hs - at.kvh * a.row_groups;
-  if (tid == 0 && at.tile > 0)
-    meta[0] = Seg{at.b, hs, worker_of(t0 - at.tile), worker_of(t0 - at.tile + at.tiles - 1)};
+  const int group = a.hq / a.hk;
+  auto row_of = [&](const Place& p) { return (int64_t)p.b * a.hq + p.kvh * group + p.rg * kRows; };
+  // this CTA's share in a segment whose first tile lies in share `from` of the run
+  auto share_of = [&](const Place& p, int64_t from) {
+    const int owner = worker_of(from), parts = worker_of(from + p.tiles - 1) - owner + 1, i = (int)me - owner;
+    const int units = min(kRows, group - p.rg * kRows) * (D / 4);
+    const int u0 = units * i / parts, u1 = units * (i + 1) / parts;
+    // a power of two of threads for a unit, no more than half of them idle
+    int lg = 0;
+    while ((2 << lg) * (u1 - u0) <= kJoinBlock && (1 << lg) < parts) ++lg;
+    return Share{row_of(p), owner, parts, u0, u1, lg, 0};
+  };
+  if (tid == 0 && at.tile > 0) meta[0] = share_of(at, t0 - at.tile);
 
   float* join = reinterpret_cast<float*>(smem);
   unsigned char* ring_p = smem + S::kJoin + warp * S::kStages * S::kStage;
@@ -498,7 +512,6 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
   const uint32_t v_chunk = kE4M3 ? k_chunk : (lane >> 3) & 1;
   const uint32_t k_row = k_tok * S::kPitch, v_row = S::kOperand + v_tok * S::kPitch;
 
-  const int group = a.hq / a.hk;
   auto load_q = [&](const Place& p) {
     const int first = p.rg * kRows, rows = min(kRows, group - first);
     const unsigned short* qu = static_cast<const unsigned short*>(a.q) + p.b * a.qst +
@@ -525,7 +538,7 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
   while (at.rem > 0) {
     // ---- a segment, or what this CTA has of it ----
     const bool began = at.tile == 0;
-    const int first = at.rg * kRows, rows = min(kRows, group - first);
+    const int rows = min(kRows, group - at.rg * kRows);
     const int end = (int)min((int64_t)at.tiles, at.tile + at.rem);
     {
 #pragma unroll
@@ -727,14 +740,14 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
             s_l[warp][8 * x + 2 * qd + h] = sum;
           }
         }
-      const int64_t out_row = (int64_t)at.b * a.hq + at.kvh * group + first;
+      const int64_t out_row = row_of(at);
       // the part of a segment that began before, or of one left open
       const int64_t slot = 2 * me + (began ? 1 : 0);
-      float* pm = reinterpret_cast<float*>(reinterpret_cast<Seg*>(a.part) + 2 * gridDim.x) + slot * kRows * 2;
-      float* po = reinterpret_cast<float*>(reinterpret_cast<Seg*>(a.part) + 2 * gridDim.x) +
+      float* pm = reinterpret_cast<float*>(reinterpret_cast<Share*>(a.part) + 2 * gridDim.x) + slot * kRows * 2;
+      float* po = reinterpret_cast<float*>(reinterpret_cast<Share*>(a.part) + 2 * gridDim.x) +
                   2ll * gridDim.x * kRows * 2 + slot * kRows * D;
       if (tid == 0 && began && !last)
-        meta[1] = Seg{at.b, at.kvh * a.row_groups + at.rg, (int)me, worker_of(t1 + (at.tiles - end) - 1)};
+        meta[1] = share_of(at, t1 - end);
       constexpr int kHalf = D / 2;
 #pragma unroll
       for (int x = 0; x < NG; ++x) {
@@ -804,7 +817,6 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
 // parts (neighbouring threads the others), then the threads and warps of these
 // elements are added in a fixed order. Bound by latency (a few L2 round trips), so it is
 // kept short rather than unrolled.
-constexpr int kJoinBlock = 256;
 
 // Reference, sum and 4 elements of a softmax over some of the tokens.
 struct Part {
@@ -829,41 +841,38 @@ __global__ void __launch_bounds__(kJoinBlock) attention_join_kernel(const __grid
   ptx::grid_dep_launch_dependents();
   const int tid = thread_here();
   const int64_t workers = gridDim.x, me = blockIdx.x;
-  const Seg* meta = reinterpret_cast<const Seg*>(a.part);
-  const float* pm = reinterpret_cast<const float*>(meta + 2 * workers);
+  const Share* shares = reinterpret_cast<const Share*>(a.part);
+  const float* pm = reinterpret_cast<const float*>(shares + 2 * workers);
   const float* po = pm + 2 * workers * kRows * 2;
-  const int4 both[2] = {*reinterpret_cast<const int4*>(meta + 2 * me), *reinterpret_cast<const int4*>(meta + 2 * me + 1)};
-  const int group = a.hq / a.hk;
 #pragma unroll 1
   for (int which = 0; which < 2; ++which) {
-    const Seg seg{both[which].x, both[which].y, both[which].z, both[which].w};
-    if (seg.owner < 0) continue;
-    const int kvh = a.row_groups == 1 ? seg.hs : seg.hs / a.row_groups;
-    const int first = (seg.hs - kvh * a.row_groups) * kRows;
-    const int rows = min(kRows, group - first), parts = seg.last - seg.owner + 1, p = (int)me - seg.owner;
-    const int u0 = rows * kUnits * p / parts, u1 = rows * kUnits * (p + 1) / parts;
-    // threads of one unit: a power of two, no more than half of them idle
-    int lg = 0;
-    while ((2 << lg) * (u1 - u0) <= kJoinBlock && (1 << lg) < parts) ++lg;
-    const int slices = 1 << lg, at_once = kJoinBlock >> lg;
+    const Share sh = shares[2 * me + which];
+    if (sh.parts == 0) continue;
+    const int slices = 1 << sh.lg, lanes = min(slices, 32);
 #pragma unroll 1
-    for (int ub = u0; ub < u1; ub += at_once) {
-      const int u = ub + (tid >> lg), r = u / kUnits, e = (u % kUnits) * 4;
+    for (int ub = sh.u0; ub < sh.u1; ub += kJoinBlock >> sh.lg) {
+      const int u = ub + (tid >> sh.lg), r = u / kUnits, e = (u % kUnits) * 4;
+      if (slices <= 32 && ub + ((tid & ~31) >> sh.lg) >= sh.u1) break;   // nothing for this warp
       Part mine{-INFINITY, {0.f, 0.f, 0.f, 0.f, 0.f}};
-      if (u < u1) {
-#pragma unroll 2
-        for (int i = tid & (slices - 1); i < parts; i += slices) {
-          const int64_t at = (2ll * (seg.owner + i) + (i == 0 ? 1 : 0)) * kRows + r;
-          const float2 ml = *reinterpret_cast<const float2*>(pm + at * 2);
-          const float4 y = *reinterpret_cast<const float4*>(po + at * D + e);
-          Part one{ml.x, {ml.y, y.x, y.y, y.z, y.w}};
-          const float top = fmaxf(mine.m, ml.x);
+      int i = tid & (slices - 1);       // up to a power of two: parts may be fewer
+      if (u < sh.u1 && i < sh.parts) {
+        // the owner's part is that of a segment left open, the others' of one begun before
+        const int first = (2 * sh.owner + (i == 0 ? 1 : 2 * i)) * kRows + r;   // under 2^15 rows
+        const float* ml = pm + first * 2;
+        const float4* y = reinterpret_cast<const float4*>(po + (int64_t)first * D + e);
+        mine = Part{ml[0], {ml[1], y->x, y->y, y->z, y->w}};
+#pragma unroll 1
+        for (i += slices; i < sh.parts; i += slices) {
+          const int at = (2 * (sh.owner + i)) * kRows + r;
+          ml = pm + at * 2;
+          y = reinterpret_cast<const float4*>(po + (int64_t)at * D + e);
+          Part one{ml[0], {ml[1], y->x, y->y, y->z, y->w}};
+          const float top = fmaxf(mine.m, one.m);
           mine.to(top);
           one.to(top);
           mine.add(one);
         }
       }
-      const int lanes = min(slices, 32);
       float top = mine.m;
 #pragma unroll 1
       for (int o = lanes >> 1; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
@@ -889,8 +898,8 @@ __global__ void __launch_bounds__(kJoinBlock) attention_join_kernel(const __grid
           }
         }
       }
-      if (u < u1 && (tid & (slices - 1)) == 0) {
-        const int64_t row = (int64_t)seg.b * a.hq + kvh * group + first + r;
+      if (u < sh.u1 && (tid & (slices - 1)) == 0) {
+        const int64_t row = sh.row + r;
         const float over = 1.f / (mine.v[0] == 0.f ? 1.f : mine.v[0]);   // no weight at all: o is 0
         constexpr bool kQBf16 = __is_same(TQ, __nv_bfloat16);
         uint2 out;
@@ -1022,7 +1031,7 @@ size_t rmsnorm_paged_attention_workspace_bytes(const rmsnorm_paged_attention_arg
   const Kernels k = find_kernels(a);
   if (k.main != nullptr)
     return (size_t)worker_count(a, k, sms) * 2 *
-           (sizeof(Seg) + k.rows * (size_t)(a->cache->head_dim + 2) * sizeof(float));
+           (sizeof(Share) + k.rows * (size_t)(a->cache->head_dim + 2) * sizeof(float));
   return (size_t)a->batch * a->q_heads * any_splits(a, sms) * (a->cache->head_dim + 2) * sizeof(float);
 }
 

@@ -442,6 +442,8 @@ __device__ __forceinline__ void qk_rope_rows(const QkArgs& a, const Rows& in, co
   const UnitOf<T> u(j, a.d, a.r, a.interleaved);
   const unsigned rows = (unsigned)a.tokens * heads;   // at most 2^31
   const unsigned first = warp * (unsigned)run * kRows + lane / L;
+  if (first - lane / L >= rows) return;
+  run = min(run, (int)((rows - (first - lane / L) + kRows - 1) / kRows));   // groups with a row
   const int64_t in_step = kRows * in.sh;
   const int across = u.eb - u.ea;
   // the lane walks down its rows ([tokens, heads] numbered token by token) by a pointer that
@@ -484,7 +486,6 @@ __device__ __forceinline__ void qk_rope_rows(const QkArgs& a, const Rows& in, co
   const int64_t to_step = kOut == kRowsOut ? kRows * out.sh : (int64_t)kRows * a.page * a.d;
 #pragma unroll 1
   for (int i = 0; i < run; ++i) {
-    if (!__any_sync(0xFFFFFFFFu, row < rows)) break;
     const bool live = row < rows;
     cp_wait<kDeep - 1>();
     Vec<T> ya, yb;
