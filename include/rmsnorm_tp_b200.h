@@ -353,7 +353,8 @@ int rmsnorm_kv_read(const rmsnorm_kv_cache* cache, void* k_out, void* v_out, con
  * exponentials. Scores, softmax and sums in fp32. The work is divided over the
  * cached length as the lengths on the device say. q and the cache of one dtype,
  * or an e4m3 cache. workspace: rmsnorm_paged_attention_workspace_bytes(args)
- * bytes of device memory, of its own for every call in flight. */
+ * bytes of device memory (16-byte aligned; 0: none is used, or the arguments are
+ * refused), of its own for every call in flight. */
 typedef struct rmsnorm_paged_attention_args {
   const rmsnorm_kv_cache* cache;
   const void* q;              /* [batch, q_heads, head_dim] */

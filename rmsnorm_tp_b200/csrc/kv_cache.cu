@@ -125,7 +125,6 @@ constexpr int kTokens = 4;
 template <typename TC, typename T>
 __global__ void __launch_bounds__(kBlock) kv_read_kernel(const __grid_constant__ ReadArgs a) {
   ptx::grid_dep_wait();
-  ptx::grid_dep_launch_dependents();
   const unsigned id = blockIdx.x * kBlock + thread_here();   // under 2^31
   const unsigned group = a.units.quotient(id), unit = id - group * a.units.by;
   const unsigned h = a.per_row.quotient(unit), e0 = (unit - h * a.per_row.by) * 8;

@@ -29,6 +29,7 @@ struct AttnArgs {
   int segments;         // kv heads * row_groups
   int q_pairs;          // the queries' elements can be read two at a time
   int whole_pages;      // pages of 16 k tokens
+  int undivided;        // a CTA for each segment, which no other shares
   FastDiv page_div;
   float scale_log2;     // scale * log2(e): scores in base 2
 };
@@ -350,64 +351,79 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
   __shared__ int64_t s_scan[kWarps];
   __shared__ int64_t s_rest;
   __shared__ int s_b;
+  // No early launch of the next kernel: its CTAs took registers on some SMs while this
+  // one's wave was being placed, so that these SMs ran one CTA fewer (2048 segments of 1024
+  // tokens, head_dim 64: 109 us a call back to back, 79 without).
   ptx::grid_dep_wait();
-  ptx::grid_dep_launch_dependents();
   const int tid = thread_here(), lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, qd = lane & 3;
 
   // this CTA's run of shares [t0, t1): every thread sums those of a run of sequences
-  const int64_t per = (a.batch + kBlock - 1) / kBlock;
-  int64_t mine = 0;
-  for (int64_t b = tid * per; b < (tid + 1) * per && b < a.batch; ++b)
-    mine += shares_of(length_of(a, b)) * a.segments;
-  int64_t upto = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
-    if (lane >= o) upto += v;
-  }
-  if (lane == 31) s_scan[warp] = upto;
-  __syncthreads();
-  int64_t total = 0;
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) upto += s_scan[w];
-    total += s_scan[w];
-  }
-  const int64_t workers = total < gridDim.x ? total : gridDim.x;
+  int64_t each = 0, more = 0, t0 = 0, t1 = 0;
   const int64_t me = blockIdx.x;
-  Share* meta = reinterpret_cast<Share*>(a.part) + 2 * me;   // of the segment that began before, and one left open
-  if (tid < 2) meta[tid].parts = 0;
-  if (me >= workers) return;
-  // the first `more` CTAs have one share more than the others
-  const int64_t each = quotient(total, workers), more = total - each * workers;
-  const int64_t t0 = me * each + (me < more ? me : more), t1 = t0 + each + (me < more ? 1 : 0);
+  Share* meta = reinterpret_cast<Share*>(a.part) + 2 * me;   // (divided) of the segment that began before, and one left open
+  Place at;
+  int hs;
+  if (a.undivided) {
+    at.b = (int)((unsigned)blockIdx.x / (unsigned)a.segments);
+    hs = (int)((unsigned)blockIdx.x - (unsigned)at.b * a.segments);
+    at.len = (int)length_of(a, at.b);
+    at.tiles = tiles_of(at.len);
+    at.tile = 0;
+    at.rem = at.tiles;
+  } else {
+    const int64_t per = (a.batch + kBlock - 1) / kBlock;
+    int64_t mine = 0;
+    for (int64_t b = tid * per; b < (tid + 1) * per && b < a.batch; ++b)
+      mine += shares_of(length_of(a, b)) * a.segments;
+    int64_t upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    if (lane == 31) s_scan[warp] = upto;
+    __syncthreads();
+    int64_t total = 0;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) upto += s_scan[w];
+      total += s_scan[w];
+    }
+    const int64_t workers = total < gridDim.x ? total : gridDim.x;
+    if (tid < 2) meta[tid].parts = 0;
+    if (me >= workers) return;
+    // the first `more` CTAs have one share more than the others
+    each = quotient(total, workers);
+    more = total - each * workers;
+    t0 = me * each + (me < more ? me : more);
+    t1 = t0 + each + (me < more ? 1 : 0);
+    if (upto - mine <= t0 && t0 < upto) {
+      int64_t rest = t0 - (upto - mine);
+      int64_t b = tid * per;
+      for (;; ++b) {
+        const int64_t n = shares_of(length_of(a, b)) * a.segments;
+        if (rest < n) break;
+        rest -= n;
+      }
+      s_b = (int)b;
+      s_rest = rest;
+    }
+    __syncthreads();
+    at.b = s_b;
+    at.len = (int)length_of(a, at.b);
+    at.tiles = tiles_of(at.len);
+    hs = (int)quotient(s_rest, at.tiles + kSegment);
+    const int into_segment = (int)(s_rest - (int64_t)hs * (at.tiles + kSegment)) - kSegment;
+    at.tile = into_segment > 0 ? into_segment : 0;
+    at.rem = t1 - t0 + (into_segment < 0 ? into_segment : 0);
+    if (at.rem <= 0) return;            // a run of nothing but a segment's extra share
+  }
+  at.kvh = hs / a.row_groups;
+  at.rg = hs - at.kvh * a.row_groups;
   auto worker_of = [&](int64_t share) {
     const int64_t line = more * (each + 1);
     return (int)(share < line ? quotient(share, each + 1) : more + quotient(share - line, each));
   };
-  if (upto - mine <= t0 && t0 < upto) {
-    int64_t rest = t0 - (upto - mine);
-    int64_t b = tid * per;
-    for (;; ++b) {
-      const int64_t n = shares_of(length_of(a, b)) * a.segments;
-      if (rest < n) break;
-      rest -= n;
-    }
-    s_b = (int)b;
-    s_rest = rest;
-  }
-  __syncthreads();
-  Place at;
-  at.b = s_b;
-  at.len = (int)length_of(a, at.b);
-  at.tiles = tiles_of(at.len);
-  const int hs = (int)quotient(s_rest, at.tiles + kSegment);
-  const int into_segment = (int)(s_rest - (int64_t)hs * (at.tiles + kSegment)) - kSegment;
-  at.tile = into_segment > 0 ? into_segment : 0;
-  at.rem = t1 - t0 + (into_segment < 0 ? into_segment : 0);
-  if (at.rem <= 0) return;              // a run of nothing but a segment's extra share
-  at.kvh = hs / a.row_groups;
-  at.rg = hs - at.kvh * a.row_groups;
   const int group = a.hq / a.hk;
   auto row_of = [&](const Place& p) { return (int64_t)p.b * a.hq + p.kvh * group + p.rg * kRows; };
   // this CTA's share in a segment whose first tile lies in share `from` of the run
@@ -421,6 +437,13 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
     return Share{row_of(p), owner, parts, u0, u1, lg, 0};
   };
   if (tid == 0 && at.tile > 0) meta[0] = share_of(at, t0 - at.tile);
+  if (at.rem == 0) {                    // undivided, and the sequence has no tokens
+    const int rows = min(kRows, group - at.rg * kRows);
+    for (int i = tid; i < rows * D; i += kBlock)
+      static_cast<TQ*>(a.out)[row_of(at) * D + i] = Pack<TQ>::from_f(0.f);
+    if (a.lse && tid < rows) a.lse[row_of(at) + tid] = -INFINITY;
+    return;
+  }
 
   float* join = reinterpret_cast<float*>(smem);
   unsigned char* ring_p = smem + S::kJoin + warp * S::kStages * S::kStage;
@@ -838,7 +861,6 @@ __global__ void __launch_bounds__(kJoinBlock) attention_join_kernel(const __grid
   constexpr int kRows = 8 * NG, kUnits = D / 4;
   __shared__ Part s_part[kJoinBlock / 32];
   ptx::grid_dep_wait();
-  ptx::grid_dep_launch_dependents();
   const int tid = thread_here();
   const int64_t workers = gridDim.x, me = blockIdx.x;
   const Share* shares = reinterpret_cast<const Share*>(a.part);
@@ -970,6 +992,15 @@ Kernels find_kernels(const rmsnorm_paged_attention_args* a) {
 int row_groups_of(const rmsnorm_paged_attention_args* a, const Kernels& k) {
   return (a->q_heads / a->cache->kv_heads + k.rows - 1) / k.rows;
 }
+// Whether each segment gets a CTA of its own and there is no join: up to 8 tiles (512
+// tokens) of capacity. Divided and undivided, device time of 4 sequences of one kv head of
+// 128: 7.9 and 5.9 us at 256 tokens, 8.4 and 10.5 at 512, 8.2 and 13.3 at 768, where the
+// second launch and the workspace cost the host 4 us; 128 such segments: 9.9 and 7.9, 12.9
+// and 10.7, 14.4 and 13.7.
+bool undivided(const rmsnorm_paged_attention_args* a, const Kernels& k) {
+  const int64_t tiles = (a->max_pages * a->cache->page_size + kTile - 1) / kTile;
+  return tiles <= 8 && a->batch * a->cache->kv_heads * row_groups_of(a, k) < (int64_t(1) << 30);
+}
 // CTAs of the main kernel: one resident wave, or a tile each of the longest lengths.
 int64_t worker_count(const rmsnorm_paged_attention_args* a, const Kernels& k, int sms) {
   const int64_t tiles = (a->max_pages * a->cache->page_size + kTile - 1) / kTile;
@@ -1029,6 +1060,7 @@ size_t rmsnorm_paged_attention_workspace_bytes(const rmsnorm_paged_attention_arg
     return 0;
   }
   const Kernels k = find_kernels(a);
+  if (k.main != nullptr && undivided(a, k)) return 0;
   if (k.main != nullptr)
     return (size_t)worker_count(a, k, sms) * 2 *
            (sizeof(Share) + k.rows * (size_t)(a->cache->head_dim + 2) * sizeof(float));
@@ -1052,7 +1084,7 @@ int rmsnorm_paged_attention(const rmsnorm_paged_attention_args* in, void* stream
   const int sms = sm_count(in->device);
   if (sms < 1) return refuse(RMSNORM_TP_ERR_CUDA, "%s: no device %d", who, in->device);
   const size_t need = rmsnorm_paged_attention_workspace_bytes(in);
-  if (!in->workspace || in->workspace_bytes < (int64_t)need)
+  if (need > 0 && (!in->workspace || in->workspace_bytes < (int64_t)need))
     return refuse(RMSNORM_TP_ERR_INVALID, "%s: workspace of %lld bytes < %zu", who,
                   (long long)in->workspace_bytes, need);
   AttnArgs a = {};
@@ -1093,6 +1125,11 @@ int rmsnorm_paged_attention(const rmsnorm_paged_attention_args* in, void* stream
           cudaFuncSetAttribute(k.main, cudaFuncAttributeMaxDynamicSharedMemorySize, k.smem);
       if (e != cudaSuccess) return launch_failed(e, who);
       if (in->device < kMaxDevices) k.ready[in->device] = true;
+    }
+    a.undivided = undivided(in, k);
+    if (a.undivided) {
+      const cudaError_t e = launch_dependent(k.main, dim3((unsigned)(a.batch * a.segments)), dim3(kBlock), k.smem, args, st);
+      return e == cudaSuccess ? RMSNORM_TP_OK : launch_failed(e, who);
     }
     const unsigned n = (unsigned)worker_count(in, k, sms);
     cudaError_t e = launch_dependent(k.main, dim3(n), dim3(kBlock), k.smem, args, st);

@@ -576,7 +576,6 @@ template <typename T, int L, bool kWrite>
 __global__ void __launch_bounds__(kRopeBlock, 5)
 qk_rope_kernel(const __grid_constant__ QkArgs a, const __grid_constant__ Split sp) {
   ptx::grid_dep_wait();
-  ptx::grid_dep_launch_dependents();
   __shared__ uint4 smem[kRopeWarps * RopeRing::kWarpBytes / 16];
   const int tid = thread_here(), lane = tid & 31;
   const RopeRing ring(smem, tid >> 5, lane);
@@ -607,7 +606,6 @@ qk_rope_backward_kernel(const __grid_constant__ QkBackArgs a, int q_blocks) {
   constexpr int E = Pack<T>::kE, N = E / 2, kRows = 32 / L, kDeep = BackRing::kDeep;
   extern __shared__ __align__(16) float dw[];   // the ring, then [kWarps][d]
   ptx::grid_dep_wait();
-  ptx::grid_dep_launch_dependents();
   const int tid = thread_here(), lane = tid & 31, warp = tid >> 5, j = lane % L;
   const BackRing ring(dw, warp, lane);
   const UnitOf<T> u(j, a.d, a.r, a.interleaved);
@@ -747,7 +745,6 @@ __global__ void __launch_bounds__(kDwWarps * 32)
 qk_rope_dw_kernel(const float* ws, int q_parts, int parts, int d, T* dqw, T* dkw) {
   __shared__ float s_sum[kDwWarps][32];
   ptx::grid_dep_wait();
-  ptx::grid_dep_launch_dependents();
   const int tid = thread_here(), lane = tid & 31, warp = tid >> 5;
   const bool is_q = blockIdx.y == 0;
   const int col = blockIdx.x * 32 + lane, first = is_q ? 0 : q_parts, end = is_q ? q_parts : parts;

@@ -339,17 +339,14 @@ def _attention_args(q, out, lse, page_table, seq_lens, ws, ws_bytes, cache_addre
 @functools.lru_cache(maxsize=4096)
 def _attention_workspace(num_pages, page_size, kv_heads, head_dim, cache_dtype, batch, max_pages, q_heads,
                          dtype, device) -> int:
-    """Bytes for a call of these sizes (a function of sizes alone); raises what the
-    library refuses."""
+    """Bytes for a call of these sizes (a function of sizes alone); 0 where none is used,
+    and for what the call itself will refuse."""
     some = 256   # an address that the size check takes and never follows
     cache = ctypes.create_string_buffer(_CACHE.pack(some, some, some, some, num_pages, page_size, kv_heads,
                                                     head_dim, cache_dtype))
-    nbytes = LIB.rmsnorm_paged_attention_workspace_bytes(_attention_args(
+    return LIB.rmsnorm_paged_attention_workspace_bytes(_attention_args(
         some, some, 0, some, some, 0, 0, ctypes.addressof(cache), (0, 0), 0, batch, max_pages, q_heads,
         dtype, 1.0, device))
-    if nbytes == 0 and batch > 0:
-        raise _lib.RMSNormTPError(_lib.ERR_INVALID, f"rmsnorm_paged_attention: {_lib.last_error()}")
-    return nbytes
 
 
 def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tensor, seq_lens: torch.Tensor,
@@ -392,10 +389,10 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tens
     dtype = _DTYPES[q_dtype]
     nbytes = _attention_workspace(cache.num_pages, cache.page_size, cache.num_kv_heads, d, cache._code, batch,
                                   ts[1], heads, dtype, device)
-    ws = q.new_empty(nbytes // 2)      # 16-bit or wider elements: at least nbytes
+    ws = q.new_empty(nbytes // 2) if nbytes else None    # 16-bit or wider elements: at least nbytes
     a, b, _ = q.stride()
     args = _ATTN_ARGS.pack(cache._address, q.data_ptr(), out.data_ptr(), lse.data_ptr() if return_lse else 0,
-                           page_table.data_ptr(), seq_lens.data_ptr(), ws.data_ptr(), nbytes, a, b, tst[0],
+                           page_table.data_ptr(), seq_lens.data_ptr(), ws.data_ptr() if nbytes else 0, nbytes, a, b, tst[0],
                            batch, ts[1], heads, dtype, d ** -0.5 if scale is None else scale, device)
     check(LIB.rmsnorm_paged_attention(args, _stream_of(device)), "rmsnorm_paged_attention")
     return (out, lse) if return_lse else out
