@@ -34,6 +34,7 @@ struct AttnArgs {
   float scale_log2;     // scale * log2(e): scores in base 2
 };
 
+constexpr int64_t kMostTiles = int64_t(1) << 36;   // of all heads: a CTA's share of them is an int
 constexpr int64_t kMostTokens = (int64_t(1) << 31) - 128;   // a tile's last token is an int
 constexpr float kLn2 = 0.69314718055994531f;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -195,8 +196,9 @@ struct Shape {
   static constexpr bool kSwizzle = kChunks % 8 == 0;
   static constexpr int kPitch = (kSwizzle ? kChunks : (kChunks | 1)) * 16;
   static constexpr int kOperand = 16 * kPitch;               // one warp's K (or V) tile
-  static constexpr int kSide = kE4M3 ? 128 + 16 : 16;        // its scales and its mask
-  static constexpr int kStage = 2 * kOperand + kSide;
+  static constexpr int kSide = kE4M3 ? 128 + 16 : 16;        // its scales and its mask, behind the rings
+  static constexpr int kTiles = 2 * kOperand;
+  static constexpr int kStage = kTiles + kSide;
   // lanes that load one row, and rows of one load instruction
   static constexpr int kLanes = kChunks % 8 == 0 ? 8 : kChunks % 4 == 0 ? 4 : 2;
   static constexpr int kRowsAtOnce = 32 / kLanes;
@@ -297,8 +299,7 @@ __device__ __forceinline__ float ref_of(float m) { return m == -INFINITY ? 0.f :
 // group of its query heads).
 // `rem`: what is left of the CTA's run, from this tile on.
 struct Place {
-  int b, kvh, rg, tile, tiles, len;
-  int64_t rem;
+  int b, kvh, rg, tile, tiles, len, rem;
 };
 
 // a / b of non-negative numbers, in 32 bits where they fit (a 64-bit division takes some
@@ -346,7 +347,7 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
   constexpr float kLift = kBf16 || kE4M3 ? 1.f : 128.f;
   constexpr int KS = D / 16;
   constexpr int kRows = 8 * NG;
-  extern __shared__ __align__(128) unsigned char smem[];
+  extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows], s_v[kWarps][kRows];
   __shared__ int64_t s_scan[kWarps];
   __shared__ int64_t s_rest;
@@ -415,7 +416,7 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
     hs = (int)quotient(s_rest, at.tiles + kSegment);
     const int into_segment = (int)(s_rest - (int64_t)hs * (at.tiles + kSegment)) - kSegment;
     at.tile = into_segment > 0 ? into_segment : 0;
-    at.rem = t1 - t0 + (into_segment < 0 ? into_segment : 0);
+    at.rem = (int)(t1 - t0) + (into_segment < 0 ? into_segment : 0);   // under 2^31: kMostTiles
     if (at.rem <= 0) return;            // a run of nothing but a segment's extra share
   }
   at.kvh = hs / a.row_groups;
@@ -446,14 +447,16 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
   }
 
   float* join = reinterpret_cast<float*>(smem);
-  unsigned char* ring_p = smem + S::kJoin + warp * S::kStages * S::kStage;
-  const uint32_t ring = ptx::smem_addr(ring_p);
+  static_assert(S::kJoin % 128 == 0 && (!S::kSwizzle || S::kPitch % 128 == 0),
+                "the swizzle's address bits are those of a chunk in 128 bytes");
+  const uint32_t ring = ptx::smem_addr(smem) + S::kJoin + warp * S::kStages * S::kTiles;
+  unsigned char* sides = smem + S::kJoin + kWarps * S::kStages * S::kTiles + warp * S::kStages * S::kSide;
 
   // ---- loads ----
   const int lr = lane / S::kLanes, lc = lane % S::kLanes;
   const unsigned char* kp = static_cast<const unsigned char*>(a.k) + lc * 16;
   const unsigned char* vp = static_cast<const unsigned char*>(a.v) + lc * 16;
-  constexpr uint32_t kSideOff = 2 * S::kOperand, kMaskOff = kSideOff + (kE4M3 ? 128 : 0);
+  constexpr uint32_t kMaskOff = kE4M3 ? 128 : 0;
   // this lane's chunk of its row in the tile, for rows lr and lr + 4 of 8
   const uint32_t to0 = lr * S::kPitch + (S::kSwizzle ? lc ^ (lr & 7) : lc) * 16;
   const uint32_t to1 = lr * S::kPitch + (S::kSwizzle ? lc ^ ((lr + S::kRowsAtOnce) & 7) : lc) * 16;
@@ -461,29 +464,36 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
   Place ahead = at;
   uint32_t into = 0;                  // stage that the next tile goes to
   int32_t page_id = -1, page_off = 0; // read one tile early
+  int table_of = -1;
+  const int32_t* table = nullptr;     // of sequence table_of
   // pages of 16 k tokens: the warp's 16 tokens lie in one page, one row behind another;
   // else lane l (and l + 16) knows the row of token l
   auto look_up = [&]() {
     const int t = ahead.tile * kTile + lane_tok;
     const unsigned pg = a.page_div.quotient(t);
     page_off = t - (int)pg * a.page;
-    page_id = t < ahead.len ? a.table[ahead.b * a.table_stride + pg] : -1;
+    if (table_of != ahead.b) {
+      table_of = ahead.b;
+      table = a.table + table_of * a.table_stride;
+    }
+    page_id = t < ahead.len ? table[pg] : -1;
   };
   look_up();
   auto send = [&]() {
     if (ahead.rem > 0) {
-      const uint32_t dst = ring + into * S::kStage;
+      const uint32_t dst = ring + into * S::kTiles;
+      unsigned char* side = sides + into * S::kSide;
       const bool live = (unsigned)page_id < (unsigned)a.num_pages;
       const int64_t row = live ? ((int64_t)page_id * a.hk + ahead.kvh) * a.page + page_off : 0;
       const int rest = ahead.len - (ahead.tile * kTile + lane_tok);
       unsigned mask;
       if (a.whole_pages) mask = !live ? 0u : rest >= 16 ? 0xFFFFu : (1u << rest) - 1u;
       else mask = __ballot_sync(0xFFFFFFFFu, live) & 0xFFFFu;
-      if (lane == 0) *reinterpret_cast<unsigned*>(ring_p + into * S::kStage + kMaskOff) = mask;
+      if (lane == 0) *reinterpret_cast<unsigned*>(side + kMaskOff) = mask;
       if constexpr (kE4M3) {          // lanes 0-15 K's scales, 16-31 V's
         const int64_t r = a.whole_pages ? row + (lane & 15) : row;
         const bool on = (mask >> (lane & 15)) & 1u;
-        cp_async4_if(dst + kSideOff + lane * 4, (lane < 16 ? a.ks : a.vs) + (on ? r : 0), on);
+        cp_async4_if(ptx::smem_addr(side) + lane * 4, (lane < 16 ? a.ks : a.vs) + (on ? r : 0), on);
       }
       if (a.whole_pages && mask == 0xFFFFu) {
         const int64_t from = (row + lr) * S::kRowBytes;
@@ -533,7 +543,11 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
   // V^T: 16-bit (chunk, next chunk) x (tokens 0-7, 8-15), e4m3 as K
   const uint32_t v_tok = kE4M3 ? k_tok : (lane >> 4) * 8 + (lane & 7);
   const uint32_t v_chunk = kE4M3 ? k_chunk : (lane >> 3) & 1;
-  const uint32_t k_row = k_tok * S::kPitch, v_row = S::kOperand + v_tok * S::kPitch;
+  const uint32_t k_lane = k_tok * S::kPitch + (S::kSwizzle ? k_chunk ^ (k_tok & 7) : k_chunk) * 16;
+  const uint32_t v_lane = S::kOperand + v_tok * S::kPitch + (S::kSwizzle ? v_chunk ^ (v_tok & 7) : v_chunk) * 16;
+  auto chunk = [](uint32_t at, uint32_t c) {
+    return S::kSwizzle ? (at ^ ((c & 7u) * 16)) + (c & ~7u) * 16 : at + c * 16;
+  };
 
   auto load_q = [&](const Place& p) {
     const int first = p.rg * kRows, rows = min(kRows, group - first);
@@ -562,7 +576,7 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
     // ---- a segment, or what this CTA has of it ----
     const bool began = at.tile == 0;
     const int rows = min(kRows, group - at.rg * kRows);
-    const int end = (int)min((int64_t)at.tiles, at.tile + at.rem);
+    const int end = min(at.tiles - at.tile, at.rem) + at.tile;
     {
 #pragma unroll
       for (int x = 0; x < NG; ++x) {
@@ -608,10 +622,12 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
       cp_wait<S::kStages - 2>();
       __syncwarp();
       send();                           // into the stage that every lane left in the last turn
-      const uint32_t base = ring + stage * S::kStage;
-      const unsigned char* side = ring_p + stage * S::kStage + kSideOff;
+      // swizzled: chunk c + k_chunk (c even) of row k_tok lies at the address of chunk k_chunk
+      // with the low bits of c flipped
+      const uint32_t k_at = ring + stage * S::kTiles + k_lane, v_at = ring + stage * S::kTiles + v_lane;
+      const unsigned char* side = sides + stage * S::kSide;
       stage = stage + 1 == S::kStages ? 0 : stage + 1;
-      const unsigned mask = *reinterpret_cast<const unsigned*>(side + (kE4M3 ? 128 : 0));
+      const unsigned mask = *reinterpret_cast<const unsigned*>(side + kMaskOff);
       if (mask != 0u) {
         float s[NG][4];                 // (token g, heads 2 qd, 2 qd + 1), (token g + 8, the same)
         {
@@ -624,17 +640,15 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
           for (int ks = 0; ks < KS; ks += 2) {
             uint32_t r[4], r2[4];
             if constexpr (kE4M3) {
-              const uint32_t c = ks + k_chunk;
               uint32_t w[4];
-              ldsm4(w, base + k_row + (S::kSwizzle ? c ^ (k_tok & 7) : c) * 16);
+              ldsm4(w, chunk(k_at, ks));
               r[0] = e4m3x2_f16x2(w[0]), r[2] = e4m3x2_f16x2(w[0] >> 16);
               r[1] = e4m3x2_f16x2(w[1]), r[3] = e4m3x2_f16x2(w[1] >> 16);
               r2[0] = e4m3x2_f16x2(w[2]), r2[2] = e4m3x2_f16x2(w[2] >> 16);
               r2[1] = e4m3x2_f16x2(w[3]), r2[3] = e4m3x2_f16x2(w[3] >> 16);
             } else {
-              const uint32_t c = 2 * ks + k_chunk;
-              ldsm4(r, base + k_row + (S::kSwizzle ? c ^ (k_tok & 7) : c) * 16);
-              ldsm4(r2, base + k_row + (S::kSwizzle ? (c + 2) ^ (k_tok & 7) : c + 2) * 16);
+              ldsm4(r, chunk(k_at, 2 * ks));
+              ldsm4(r2, chunk(k_at, 2 * ks + 2));
             }
 #pragma unroll
             for (int x = 0; x < NG; ++x) {
@@ -714,8 +728,7 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
 #pragma unroll
         for (int j = 0; j < KS; j += kE4M3 ? 2 : 1) {
           uint32_t r[4], r2[4];
-          const uint32_t c = (kE4M3 ? j : 2 * j) + v_chunk;
-          const uint32_t from = base + v_row + (S::kSwizzle ? c ^ (v_tok & 7) : c) * 16;
+          const uint32_t from = chunk(v_at, kE4M3 ? j : 2 * j);
           if constexpr (kE4M3) {
             // bytes of w: (token 2 qd: elements 2 g, 2 g + 1), (token 2 qd + 1: the same), so row g
             // of the product is element 2 g and row g + 8 element 2 g + 1
@@ -1042,6 +1055,9 @@ int check_attention(const char* who, const rmsnorm_paged_attention_args* a) {
   if (a->max_pages < 0 || a->max_pages * (int64_t)c->page_size > kMostTokens)
     return refuse(RMSNORM_TP_ERR_INVALID, "%s: %lld pages of %d tokens: a sequence holds at most 2^31 - 128",
                   who, (long long)a->max_pages, c->page_size);
+  if ((a->max_pages * (int64_t)c->page_size / kTile + 2) * a->batch * a->q_heads > kMostTiles)
+    return refuse(RMSNORM_TP_ERR_INVALID, "%s: %lld sequences of %d heads and %lld tokens: too many", who,
+                  (long long)a->batch, a->q_heads, (long long)(a->max_pages * (int64_t)c->page_size));
   if (a->device < 0) return refuse(RMSNORM_TP_ERR_INVALID, "%s: device %d", who, a->device);
   return RMSNORM_TP_OK;
 }
