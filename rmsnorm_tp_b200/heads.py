@@ -64,20 +64,28 @@ def _weight_fits(t: torch.Tensor, d: int, dtype: torch.dtype, device: int) -> bo
     return t.dtype is dtype and t.get_device() == device and t.shape == (d,) and t.is_contiguous()
 
 
+def _contiguous_like(t: torch.Tensor) -> torch.Tensor:
+    """A fresh contiguous tensor (empty_like, the faster call, keeps the order of strides)."""
+    out = torch.empty_like(t)
+    return out if out.is_contiguous() else t.new_empty(t.shape)
+
+
 def _turn_sizes(q, k, q_weight, k_weight, rope, positions):
     """(device, dtype, tokens, q heads, kv heads, head_dim, table rows, rotary_dim) of
     operands that fit together; AssertionError for others."""
     qs, ks, rs = q.shape, k.shape, rope.shape
     if len(qs) == 3 and len(ks) == 3 and len(rs) == 2:
-        tokens, hq, d = qs
+        (tokens, hq, d), (tokens_k, hk, dk), (most, r) = qs, ks, rs
         device, dtype = q.get_device(), q.dtype
-        if (device >= 0 and dtype in _DTYPES and q.stride(2) == 1 and _rows_fit(k, tokens, ks[1], d, dtype, device)
+        if (device >= 0 and dtype in _DTYPES and q.stride(2) == 1 and tokens_k == tokens and dk == d
+                and k.dtype is dtype and k.get_device() == device and k.stride(2) == 1
                 and rope.dtype is _F32 and rope.get_device() == device and rope.is_contiguous()
-                and _index_fits(positions, tokens, _I64, device)
+                and positions.dtype is _I64 and positions.get_device() == device and positions.shape == (tokens,)
+                and positions.is_contiguous()
                 and (q_weight is None and k_weight is None
                      or q_weight is not None and k_weight is not None
                      and _weight_fits(q_weight, d, dtype, device) and _weight_fits(k_weight, d, dtype, device))):
-            return device, dtype, tokens, hq, ks[1], d, rs[0], rs[1]
+            return device, dtype, tokens, hq, hk, d, most, r
     _explain_turn(q, k, q_weight, k_weight, rope, positions)
 
 
@@ -162,7 +170,7 @@ def qk_norm_rope_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.T
         _explain_rows("dq_out", dq_out, q, hq)
     if not _rows_fit(dk_out, tokens, hk, d, dtype, device):
         _explain_rows("dk_out", dk_out, q, hk)
-    dq, dk = q.new_empty(tokens, hq, d), k.new_empty(tokens, hk, d)
+    dq, dk = _contiguous_like(q), _contiguous_like(k)
     if q_weight is None:
         dqw = dkw = None
         weights = (0, 0, 0, 0)
@@ -382,7 +390,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tens
     if not _index_fits(seq_lens, batch, _I32, device):
         _explain_index("seq_lens", batch, _I32)
     if out is None:
-        out = q.new_empty(batch, heads, d)
+        out = _contiguous_like(q)
     elif out.shape != qs or out.dtype is not q_dtype or out.get_device() != device or not out.is_contiguous():
         raise AssertionError("out must be contiguous with q's shape, dtype and device")
     lse = torch.empty(batch, heads, dtype=_F32, device=q.device) if return_lse else None
