@@ -358,7 +358,7 @@ int rmsnorm_kv_read(const rmsnorm_kv_cache* cache, void* k_out, void* v_out, con
 typedef struct rmsnorm_paged_attention_args {
   const rmsnorm_kv_cache* cache;
   const void* q;              /* [batch, q_heads, head_dim] */
-  void* out;                  /* [batch, q_heads, head_dim] contiguous */
+  void* out;                  /* [batch, q_heads, head_dim] contiguous, 16-byte aligned */
   float* lse;                 /* [batch, q_heads], or NULL */
   const int32_t* page_table;  /* [batch, max_pages], rows page_table_stride apart */
   const int32_t* seq_lens;    /* [batch] */

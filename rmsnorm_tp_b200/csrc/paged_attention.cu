@@ -1091,6 +1091,8 @@ int rmsnorm_paged_attention(const rmsnorm_paged_attention_args* in, void* stream
   const rmsnorm_kv_cache* c = in->cache;
   if (!in->q || !in->out || !in->seq_lens || (in->max_pages > 0 && !in->page_table))
     return refuse(RMSNORM_TP_ERR_INVALID, "%s: NULL tensor pointer", who);
+  if ((reinterpret_cast<uintptr_t>(in->out) | reinterpret_cast<uintptr_t>(in->workspace)) & 15u)
+    return refuse(RMSNORM_TP_ERR_INVALID, "%s: out and the workspace must be 16-byte aligned", who);
   const int eb = elem_bytes(in->dtype);
   const int64_t so[2] = {(int64_t)in->q_heads * c->head_dim, c->head_dim};
   const View q = view_of(in->q, in->batch, in->q_heads, c->head_dim, in->q_strides, eb);

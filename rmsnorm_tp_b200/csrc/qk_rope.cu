@@ -52,6 +52,7 @@ struct QkBackArgs {
   float eps;
 };
 
+constexpr int kMaxParts = 1024;        // most CTAs of a backward call: the workspace's rows
 constexpr int kBlock = 256;
 constexpr int kWarps = kBlock / 32;
 
@@ -429,7 +430,7 @@ struct Ring {
 };
 
 using RopeRing = Ring<2, 4>;             // x
-using BackRing = Ring<4, 3>;             // dy and x: 48 KB for a CTA's warps
+using BackRing = Ring<4, 3>;             // dy and x
 
 // `run` groups of 32 / L rows of one operand. kTurned: normed and turned (else as they are:
 // the values on their way to the cache).
@@ -573,7 +574,7 @@ struct Split {
 };
 
 template <typename T, int L, bool kWrite>
-__global__ void __launch_bounds__(kRopeBlock, 5)
+__global__ void __launch_bounds__(kRopeBlock, 6)
 qk_rope_kernel(const __grid_constant__ QkArgs a, const __grid_constant__ Split sp) {
   ptx::grid_dep_wait();
   __shared__ uint4 smem[kRopeWarps * RopeRing::kWarpBytes / 16];
@@ -600,11 +601,13 @@ qk_rope_kernel(const __grid_constant__ QkArgs a, const __grid_constant__ Split s
 // The backward: g and x in registers, dw summed per lane over the lane's rows, then over
 // the warp's row groups and the CTA's warps in a fixed order. CTAs [0, q_blocks) share the
 // queries' rows equally, the others the keys'.
+constexpr int kBackCtas = 4;               // resident on an SM (128 registers a thread)
+
 template <typename T, int L>
-__global__ void __launch_bounds__(kBlock, 2)
+__global__ void __launch_bounds__(kRopeBlock, kBackCtas)
 qk_rope_backward_kernel(const __grid_constant__ QkBackArgs a, int q_blocks) {
   constexpr int E = Pack<T>::kE, N = E / 2, kRows = 32 / L, kDeep = BackRing::kDeep;
-  extern __shared__ __align__(16) float dw[];   // the ring, then [kWarps][d]
+  extern __shared__ __align__(16) float dw[];   // the rings, then [kRopeWarps][d]
   ptx::grid_dep_wait();
   const int tid = thread_here(), lane = tid & 31, warp = tid >> 5, j = lane % L;
   const BackRing ring(dw, warp, lane);
@@ -621,7 +624,7 @@ qk_rope_backward_kernel(const __grid_constant__ QkBackArgs a, int q_blocks) {
     wb.from(ptx::ld_cached_v4(w + u.eb));
   }
   const unsigned rows = (unsigned)a.tokens * heads, groups = (rows + kRows - 1) / kRows;
-  const unsigned workers = blocks * kWarps, me = block * kWarps + warp;
+  const unsigned workers = blocks * kRopeWarps, me = block * kRopeWarps + warp;
   const unsigned first = (unsigned)((uint64_t)groups * me / workers);
   const unsigned n = (unsigned)((uint64_t)groups * (me + 1) / workers) - first;
   unsigned row = first * kRows + lane / L, end = 0;
@@ -710,6 +713,7 @@ qk_rope_backward_kernel(const __grid_constant__ QkBackArgs a, int q_blocks) {
   }
   cp_wait<0>();
   if (!a.norm) return;
+  ptx::grid_dep_launch_dependents();   // the sum of dw may come to the SMs (and waits)
   __syncthreads();                  // every warp is done with its ring
   float fa[E], fb[E];
   da.floats(fa);
@@ -729,9 +733,9 @@ qk_rope_backward_kernel(const __grid_constant__ QkBackArgs a, int q_blocks) {
     }
   }
   __syncthreads();
-  for (int i = tid; i < a.d; i += kBlock) {
+  for (int i = tid; i < a.d; i += kRopeBlock) {
     float s = 0.f;
-    for (int v = 0; v < kWarps; ++v) s += dw[v * a.d + i];
+    for (int v = 0; v < kRopeWarps; ++v) s += dw[v * a.d + i];
     a.ws[(int64_t)blockIdx.x * a.d + i] = s;
   }
 }
@@ -750,7 +754,7 @@ qk_rope_dw_kernel(const float* ws, int q_parts, int parts, int d, T* dqw, T* dkw
   const int col = blockIdx.x * 32 + lane, first = is_q ? 0 : q_parts, end = is_q ? q_parts : parts;
   float s = 0.f;
   if (col < d) {
-#pragma unroll 10
+#pragma unroll 12
     for (int i = first + warp; i < end; i += kDwWarps) s += ws[(int64_t)i * d + col];
   }
   s_sum[warp][lane] = s;
@@ -961,7 +965,7 @@ int rmsnorm_qk_rope_write(const rmsnorm_qk_rope_args* args, void* stream) {
 
 size_t rmsnorm_qk_rope_backward_workspace_bytes(int32_t head_dim) {
   if (head_dim < 2 || head_dim > RMSNORM_HEAD_DIM_MAX) return 0;
-  return (size_t)rtp::kBackwardMaxGrid * (size_t)head_dim * sizeof(float);
+  return (size_t)rtp::kMaxParts * (size_t)head_dim * sizeof(float);
 }
 
 int rmsnorm_qk_rope_backward(const rmsnorm_qk_rope_backward_args* in, void* stream) {
@@ -1035,14 +1039,17 @@ int rmsnorm_qk_rope_backward(const rmsnorm_qk_rope_backward_args* in, void* stre
                             (norm ? a.q.st | a.q.sh | a.k.st | a.k.sh : 0);
     const int lanes = lanes_of(a.d, a.r, eb, bits, strides);
     // one resident wave of CTAs, shared by q and k as their rows are
-    const int64_t rows_of_cta = (int64_t)kWarps * (lanes ? 32 / lanes : 1);
+    const int sms = sm_count(in->device), warps = lanes ? kRopeWarps : kWarps;
+    const int most = min(kMaxParts, lanes ? sms * kBackCtas : 2 * sms);
+    if (most < 2) return refuse(RMSNORM_TP_ERR_CUDA, "%s: no device %d", who, in->device);
+    const int64_t rows_of_cta = (int64_t)warps * (lanes ? 32 / lanes : 1);
     const int64_t wq = (a.tokens * a.hq + rows_of_cta - 1) / rows_of_cta;
     const int64_t wk = (a.tokens * a.hk + rows_of_cta - 1) / rows_of_cta;
-    if (wq + wk <= kBackwardMaxGrid) {
+    if (wq + wk <= most) {
       q_blocks = (int)wq;
       grid = (int)(wq + wk);
     } else {
-      grid = kBackwardMaxGrid;
+      grid = most;
       q_blocks = (int)((wq * grid + (wq + wk) / 2) / (wq + wk));
       q_blocks = q_blocks < 1 ? 1 : q_blocks >= grid ? grid - 1 : q_blocks;
     }
@@ -1050,10 +1057,10 @@ int rmsnorm_qk_rope_backward(const rmsnorm_qk_rope_backward_args* in, void* stre
                      : in->dtype == RMSNORM_TP_BF16 ? backward_fn<__nv_bfloat16>(lanes)
                                                     : backward_fn<__half>(lanes);
     void* args[] = {&a, &q_blocks};
-    // the vector kernels' ring (at most 16 KB of dw lies over it)
-    const size_t sums = norm ? (size_t)kWarps * a.d * sizeof(float) : 0;
-    const size_t smem = lanes ? (size_t)kWarps * BackRing::kWarpBytes : sums;
-    const cudaError_t e = launch_dependent(fn, dim3((unsigned)grid), dim3(kBlock), smem, args, st);
+    // the vector kernels' rings (at most 8 KB of dw lies over them)
+    const size_t sums = norm ? (size_t)warps * a.d * sizeof(float) : 0;
+    const size_t smem = lanes ? (size_t)warps * BackRing::kWarpBytes : sums;
+    const cudaError_t e = launch_dependent(fn, dim3((unsigned)grid), dim3(warps * 32), smem, args, st);
     if (e != cudaSuccess) return launch_failed(e, who);
   }
   if (norm) {   // no tokens: zeros

@@ -134,7 +134,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
     rotary_dim, and elements behind it are not turned. Pairs are (i, i + rotary_dim / 2),
     or with ``interleaved`` (2i, 2i + 1). ``positions`` int64 [tokens]; one outside the
     table makes the token's turned elements NaN. ``q_out`` / ``k_out`` receive the results
-    instead of fresh tensors and may be q / k themselves. fp32 inside, rounded once."""
+    instead of fresh tensors and may be q / k themselves. fp32 inside, rounded once. Not
+    recorded for autograd: see ``qk_norm_rope_with_grad``."""
     device, dtype, tokens, hq, hk, d, most, r = _turn_sizes(q, k, q_weight, k_weight, rope, positions)
     if q_out is None:
         q_out = torch.empty_like(q)
@@ -209,6 +210,7 @@ class _QkNormRopeFunction(torch.autograd.Function):
         return qk_norm_rope(q, k, q_weight, k_weight, rope, positions, eps, interleaved)
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, dq_out, dk_out):
         q, k, q_weight, k_weight, rope, positions = ctx.saved_tensors
         dq_out = dq_out if dq_out.stride(2) == 1 else dq_out.contiguous()
@@ -220,8 +222,19 @@ class _QkNormRopeFunction(torch.autograd.Function):
 def qk_norm_rope_with_grad(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor],
                            k_weight: Optional[torch.Tensor], rope: torch.Tensor, positions: torch.Tensor,
                            eps: float = 1e-6, interleaved: bool = False):
-    """``qk_norm_rope`` recorded for autograd; its backward runs the backward kernel."""
+    """``qk_norm_rope`` recorded for autograd; its backward runs the backward kernel (once:
+    it is not differentiable itself)."""
     return _QkNormRopeFunction.apply(q, k, q_weight, k_weight, rope, positions, eps, interleaved)
+
+
+def _held(i: int, doc: str) -> property:
+    """A tensor whose address the native handle holds: changed in place only."""
+
+    def put(self, value):
+        if value is not self._tensors[i]:    # (`cache.k *= 2` puts back what it got)
+            raise AttributeError("a PagedKVCache keeps its tensors; change them in place")
+
+    return property(lambda self: self._tensors[i], put, doc=doc)
 
 
 class PagedKVCache:
@@ -276,7 +289,7 @@ class PagedKVCache:
         self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = k.shape
         if self.head_dim % 16 or not 16 <= self.head_dim <= 256:
             raise AssertionError(f"head_dim {self.head_dim} must be a multiple of 16, at most 256")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._tensors = k, v, k_scale, v_scale
         self.dtype, self.device, self._index = k.dtype, k.device, k.get_device()
         self._code = _CACHE_DTYPES[k.dtype]
         self._struct = ctypes.create_string_buffer(_CACHE.pack(
@@ -284,6 +297,11 @@ class PagedKVCache:
             v_scale.data_ptr() if e4m3 else 0, self.num_pages, self.page_size, self.num_kv_heads,
             self.head_dim, self._code))
         self._address = ctypes.addressof(self._struct)
+
+    k = _held(0, "keys, or their codes")
+    v = _held(1, "values, or their codes")
+    k_scale = _held(2, "scales of the keys' codes, or None")
+    v_scale = _held(3, "scales of the values' codes, or None")
 
     def read(self, slots: torch.Tensor, dtype: Optional[torch.dtype] = None):
         """(k, v) [count, kv_heads, head_dim] of ``dtype``: the rows at ``slots`` (int64

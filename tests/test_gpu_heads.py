@@ -1,11 +1,15 @@
 """GPU parity of the operators on query / key heads, the paged cache and the single-token
 attention against the formulas in 64 bits (heads_oracle), at sizes, strides, masks and
 values where they can go wrong; the run of them together between the package's norms."""
+import subprocess
+import sys
+
 import pytest
 import torch
 
 import heads_oracle as H
 import rmsnorm_tp_b200 as rtp
+from conftest import ROOT
 
 pytestmark = pytest.mark.gpu
 
@@ -163,6 +167,9 @@ def test_autograd_with_shared_and_broadcast_inputs():
     H.within(k.grad, dk, sk, "dk")
     H.within(one.grad, dq.sum(0, keepdim=True), sq.sum(0, keepdim=True) + (tokens + 2) * H.U32 * dq.abs().sum(0), "dq")
     H.within(w.grad, dwq + dwk, s1 + s2 + 4 * H.U32 * (dwq.abs() + dwk.abs()), "dw")
+    with pytest.raises(RuntimeError):                   # no gradient of the gradient
+        z = rtp.qk_norm_rope_with_grad(k, k, w, w, rope, pos, EPS)[0].square().sum()
+        torch.autograd.grad(torch.autograd.grad(z, k, create_graph=True)[0].sum(), k)
     # only one output used: the other's gradient is zero
     a, b = (t.detach().clone().requires_grad_() for t in (q, k))
     rtp.qk_norm_rope_with_grad(a, b, None, None, rope, pos, EPS)[0].sum().backward()
@@ -458,6 +465,77 @@ def test_two_streams_and_two_captured_graphs():
     assert torch.equal(held[0], rtp.paged_attention(qs[0], cache, tables[0], lens[0]))
 
 
+@pytest.mark.parametrize("dtype,held", [(BF16, BF16), (F16, E4M3), (F32, F32)])
+@pytest.mark.parametrize("longest", [300, 3000])
+def test_attention_of_queries_at_odd_addresses(dtype, held, longest):
+    """Queries whose elements no 4-byte load takes, and outputs given; an output that no
+    vector store takes is refused."""
+    page, d, lens = 16, 64, [longest, 1, 17]
+    cache = _filled(29, 220, page, 1, d, held)
+    table, lens_t = _table(29, lens, page, 220), torch.tensor(lens, dtype=torch.int32, device="cuda")
+    q = _normal(_gen(29), 3, 9, d + 1).to(dtype)[:, 1:, 1:]
+    want, _ = _check_attention(q, cache, table, lens_t)
+    room = torch.full((3 * 8 * d + 16,), 5.0, dtype=dtype, device="cuda")
+    out = room[8:-8].view(3, 8, d)
+    assert rtp.paged_attention(q, cache, table, lens_t, out=out) is out and torch.equal(out, want)
+    assert (room[:8] == 5).all() and (room[-8:] == 5).all()
+    with pytest.raises(rtp.RMSNormTPError, match="aligned"):
+        rtp.paged_attention(q, cache, table, lens_t, out=room[1:3 * 8 * d + 1].view(3, 8, d))
+
+
+def test_results_do_not_depend_on_dependent_launch():
+    page, d = 16, 128
+    cache = _filled(30, 300, page, 2, d, BF16)
+    lens_t = torch.tensor([4000, 0, 3, 700], dtype=torch.int32, device="cuda")
+    table = _table(30, lens_t.tolist(), page, 300)
+    q, k, v = _heads(30, 4, 8, 2, d, BF16)
+    w, _ = _weights(30, d, BF16)
+    rope, pos = rtp.rope_table(64, d, device="cuda"), _positions(30, 4, 64)
+    dq, dk, _ = _heads(32, 4, 8, 2, d, BF16, "own")
+
+    def all_of_them():
+        a, b = rtp.qk_norm_rope(q, k, w, w, rope, pos)
+        out = rtp.paged_attention(a, cache, table, lens_t, return_lse=True)
+        return [a, b, *out, *rtp.qk_norm_rope_backward(dq, dk, q, k, w, w, rope, pos)]
+
+    want = all_of_them()
+    rtp.set_dependent_launch(False)
+    try:
+        for a, b in zip(want, all_of_them()):
+            assert torch.equal(a, b)
+    finally:
+        rtp.set_dependent_launch(True)
+
+
+def test_first_calls_inside_a_capture():
+    """A process whose first call of each operator is captured (its kernels are loaded and
+    their shared-memory limits raised during the capture)."""
+    code = """
+import torch, rmsnorm_tp_b200 as rtp
+g = torch.Generator(device="cuda").manual_seed(1)
+q, k, v = (torch.randn(5, n, 128, generator=g, device="cuda").bfloat16() for n in (8, 2, 2))
+w = torch.ones(128, device="cuda").bfloat16()
+rope, pos = rtp.rope_table(64, 128, device="cuda"), torch.arange(5, device="cuda")
+cache = rtp.PagedKVCache(64, 16, 2, 128, torch.float8_e4m3fn)
+slots = torch.arange(5, device="cuda") * 3
+table = torch.arange(60, dtype=torch.int32, device="cuda").expand(5, 60)
+lens = torch.tensor([13, 900, 0, 5, 1], dtype=torch.int32, device="cuda")
+def run():
+    a = rtp.qk_norm_rope_write(q, k, v, w, w, rope, pos, cache, slots)
+    return [a, *rtp.paged_attention(a, cache, table, lens, return_lse=True), *cache.read(slots),
+            *rtp.qk_norm_rope(q, k, w, w, rope, pos), *rtp.qk_norm_rope_backward(q, k, q, k, w, w, rope, pos)]
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    held = run()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(held, run()))
+"""
+    res = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0, res.stderr[-2000:]
+
+
 def test_captured_turn_write_read_and_backward():
     tokens, hq, hk, d = 40, 8, 2, 128
     q, k, v = _heads(35, tokens, hq, hk, d, BF16)
@@ -531,6 +609,8 @@ def test_python_surface_refuses():
             rtp.PagedKVCache(**{**dict(num_pages=2, page_size=16, num_kv_heads=1, head_dim=64), **bad})
     with pytest.raises(AssertionError):
         rtp.PagedKVCache.from_tensors(cache.k, cache.v, k_scale=rope)
+    with pytest.raises(AttributeError):
+        cache.k = cache.v
     with pytest.raises(AssertionError):
         cache.read(slots.int())
     with pytest.raises(AssertionError):

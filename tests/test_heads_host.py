@@ -74,7 +74,7 @@ def test_null_arguments_and_empty_calls():
     assert L.rmsnorm_kv_read(None, None, None, None, 1, 0, 0, None) == _lib.ERR_INVALID
     assert _forward(tokens=0, q=0, k=0, qo=0, ko=0, pos=0) == _lib.OK
     assert L.rmsnorm_qk_rope_backward_workspace_bytes(0) == 0
-    assert L.rmsnorm_qk_rope_backward_workspace_bytes(128) == 296 * 128 * 4
+    assert L.rmsnorm_qk_rope_backward_workspace_bytes(128) == 1024 * 128 * 4
 
 
 @pytest.mark.parametrize("cache", [
@@ -96,7 +96,7 @@ def test_write_checks():
     assert call(cache=e4m3, dtype=_lib.F32) == _lib.ERR_CUDA
 
 
-def _back(dqo=Q, dko=K, q=0x3000000, k=0x4000000, dq=QO, dk=KO, dw=W, dkw=W, qw=W, kw=W, ws=V, nbytes=296 * 64 * 4,
+def _back(dqo=Q, dko=K, q=0x3000000, k=0x4000000, dq=QO, dk=KO, dw=W, dkw=W, qw=W, kw=W, ws=V, nbytes=1024 * 64 * 4,
           tokens=8, r=64):
     s = (256, 64, 128, 64)
     return L.rmsnorm_qk_rope_backward(heads._BACK_ARGS.pack(
@@ -107,7 +107,7 @@ def _back(dqo=Q, dko=K, q=0x3000000, k=0x4000000, dq=QO, dk=KO, dw=W, dkw=W, qw=
 def test_backward_checks():
     assert _back() == _lib.ERR_CUDA
     assert _back(q=0, k=0, dw=0, qw=0, kw=0, ws=0, nbytes=0) == _lib.ERR_CUDA      # rotation alone
-    for kw in (dict(dw=0), dict(dkw=0), dict(ws=0), dict(nbytes=296 * 64 * 4 - 1), dict(qw=0), dict(q=0), dict(dq=Q),
+    for kw in (dict(dw=0), dict(dkw=0), dict(ws=0), dict(nbytes=1024 * 64 * 4 - 1), dict(qw=0), dict(q=0), dict(dq=Q),
                dict(dk=0x4000000), dict(dk=QO + 512), dict(dqo=0), dict(r=1), dict(tokens=-1)):
         assert _back(**kw) == _lib.ERR_INVALID, kw
 
@@ -122,7 +122,8 @@ def test_attention_refuses_before_any_cuda_call():
     keep, at = _cache()
     for kw in (dict(hq=3), dict(hq=0), dict(dtype=_lib.F16), dict(dtype=9), dict(batch=-1), dict(batch=65536),
                dict(pages=-1), dict(pages=1 << 27), dict(q=0), dict(out=0), dict(lens=0), dict(table=0),
-               dict(out=Q), dict(qs=(-256, 64))):
+               dict(out=Q), dict(qs=(-256, 64)), dict(out=QO + 8), dict(ws=V + 4),
+               dict(batch=65535, hq=65536, pages=1 << 26)):
         assert L.rmsnorm_paged_attention(_attn(at, **kw), None) == _lib.ERR_INVALID, kw
         assert _lib.last_error().startswith("paged_attention:")
     assert L.rmsnorm_paged_attention(_attn(at, batch=0, q=0, out=0), None) == _lib.OK
