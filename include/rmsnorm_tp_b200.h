@@ -301,9 +301,9 @@ int rmsnorm_qk_rope_write(const rmsnorm_qk_rope_args* args, void* stream);
 /* Gradients of rmsnorm_qk_rope_forward, with g = R^T dy and inv the forward's
  * factor: dx = inv g w - x inv^3 mean(g w x), dw = sum over tokens and heads of
  * g x inv (without weights dx = g, and q, k may be NULL). dq and dk are
- * contiguous [tokens, heads, head_dim] and overlap no input. workspace:
- * rmsnorm_qk_rope_backward_workspace_bytes(head_dim) bytes of device memory, 16-byte
- * aligned (fp32 partials of dw, summed in a fixed order: deterministic). */
+ * contiguous [tokens, heads, head_dim] and overlap no input. workspace: with
+ * weights, rmsnorm_qk_rope_backward_workspace_bytes(sizes) bytes of device memory (fp32
+ * partials of dw; 0: none is used). The sums of dw run in a fixed order. */
 typedef struct rmsnorm_qk_rope_backward_args {
   const void* dq_out;         /* [tokens, q_heads, head_dim] */
   const void* dk_out;         /* [tokens, kv_heads, head_dim] */
@@ -335,7 +335,8 @@ typedef struct rmsnorm_qk_rope_backward_args {
   int32_t device;
 } rmsnorm_qk_rope_backward_args;
 
-size_t rmsnorm_qk_rope_backward_workspace_bytes(int32_t head_dim);
+size_t rmsnorm_qk_rope_backward_workspace_bytes(int64_t tokens, int32_t q_heads, int32_t kv_heads,
+                                                int32_t head_dim, int32_t rotary_dim, int32_t dtype);
 int rmsnorm_qk_rope_backward(const rmsnorm_qk_rope_backward_args* args, void* stream);
 
 /* k_out and v_out [count, kv_heads, head_dim] contiguous of `dtype`: the cache's

@@ -150,7 +150,7 @@ SIGNATURES = {
     # packed argument structures: see heads.py
     "rmsnorm_qk_rope_forward": (_i32, [ctypes.c_char_p, _c_void_p]),
     "rmsnorm_qk_rope_write": (_i32, [ctypes.c_char_p, _c_void_p]),
-    "rmsnorm_qk_rope_backward_workspace_bytes": (_sz, [_i32]),
+    "rmsnorm_qk_rope_backward_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32, _i32, _i32]),
     "rmsnorm_qk_rope_backward": (_i32, [ctypes.c_char_p, _c_void_p]),
     "rmsnorm_kv_read": (_i32, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _i32, _i32, _c_void_p]),
     "rmsnorm_paged_attention_workspace_bytes": (_sz, [ctypes.c_char_p]),

@@ -46,8 +46,9 @@ int sm_count(int device);
 
 // Launch with programmatic stream serialization when dependent launch is on.
 // Every kernel launched through here starts with grid_dep_wait().
+// cluster > 0: in clusters of so many CTAs.
 cudaError_t launch_dependent(const void* fn, dim3 grid, dim3 block, size_t smem, void** args,
-                             cudaStream_t stream);
+                             cudaStream_t stream, int cluster = 0);
 
 inline int launch_failed(cudaError_t e, const char* who) {
   cudaGetLastError();   // a refused launch leaves the error behind otherwise

@@ -21,18 +21,24 @@ int sm_count(int device) {
 }
 
 cudaError_t launch_dependent(const void* fn, dim3 grid, dim3 block, size_t smem, void** args,
-                             cudaStream_t stream) {
-  if (!get_dependent_launch()) return cudaLaunchKernel(fn, grid, block, args, smem, stream);
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+                             cudaStream_t stream, int cluster) {
+  cudaLaunchAttribute attr[2];
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = block;
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  if (get_dependent_launch()) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 0) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = (unsigned)cluster;
+    attr[cfg.numAttrs].val.clusterDim.y = 1;
+    attr[cfg.numAttrs++].val.clusterDim.z = 1;
+  }
   return cudaLaunchKernelExC(&cfg, fn, args);
 }
 

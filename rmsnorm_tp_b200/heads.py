@@ -179,9 +179,9 @@ def qk_norm_rope_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.T
     else:
         dqw, dkw = torch.empty_like(q_weight), torch.empty_like(k_weight)
         weights = (dqw.data_ptr(), dkw.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr())
-        nbytes = _backward_workspace(d)
-        ws = rope.new_empty(nbytes // 4)
-        ws_ptr = ws.data_ptr()
+        nbytes = _backward_workspace(tokens, hq, hk, d, r, _DTYPES[dtype])
+        ws = rope.new_empty(nbytes // 4) if nbytes else None
+        ws_ptr = ws.data_ptr() if nbytes else 0
     a, b, _ = dq_out.stride()
     c, e, _ = dk_out.stride()
     f, g, _ = q.stride()
@@ -194,10 +194,11 @@ def qk_norm_rope_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.T
     return dq, dk, dqw, dkw
 
 
-@functools.lru_cache(maxsize=None)
-def _backward_workspace(head_dim: int) -> int:
-    """Bytes of the workspace (a function of the size alone)."""
-    return LIB.rmsnorm_qk_rope_backward_workspace_bytes(head_dim)
+@functools.lru_cache(maxsize=4096)
+def _backward_workspace(*sizes: int) -> int:
+    """Bytes of the workspace (a function of the sizes alone); 0 where none is used, and for
+    what the call itself will refuse."""
+    return LIB.rmsnorm_qk_rope_backward_workspace_bytes(*sizes)
 
 
 class _QkNormRopeFunction(torch.autograd.Function):

@@ -16,10 +16,10 @@ from rmsnorm_tp_b200 import _lib, heads
 L = _lib.LIB
 # addresses that a refused call never follows; device -1 makes an accepted one end in
 # cudaSetDevice, before any launch
-Q, K, V, QO, KO, W, TABLE, POS, SLOTS = (0x100000 * i for i in range(1, 10))
+Q, K, V, QO, KO, W, TABLE, POS, SLOTS = (0x10000000 * i for i in range(1, 10))
 
 
-def _cache(pages=4, page=16, heads_=2, dim=64, dtype=_lib.BF16, k=0x10000000, v=0x20000000, ks=0, vs=0):
+def _cache(pages=4, page=16, heads_=2, dim=64, dtype=_lib.BF16, k=0xD0000000, v=0xE0000000, ks=0, vs=0):
     buf = ctypes.create_string_buffer(heads._CACHE.pack(k, v, ks, vs, pages, page, heads_, dim, dtype))
     return buf, ctypes.addressof(buf)
 
@@ -73,13 +73,16 @@ def test_null_arguments_and_empty_calls():
     assert L.rmsnorm_paged_attention(None, None) == _lib.ERR_INVALID
     assert L.rmsnorm_kv_read(None, None, None, None, 1, 0, 0, None) == _lib.ERR_INVALID
     assert _forward(tokens=0, q=0, k=0, qo=0, ko=0, pos=0) == _lib.OK
-    assert L.rmsnorm_qk_rope_backward_workspace_bytes(0) == 0
-    assert L.rmsnorm_qk_rope_backward_workspace_bytes(128) == 1024 * 128 * 4
+    ws = L.rmsnorm_qk_rope_backward_workspace_bytes
+    assert ws(8192, 32, 8, 128, 128, _lib.BF16) == 1024 * 128 * 4
+    assert ws(8, 4, 2, 50, 20, _lib.BF16) == 1024 * 50 * 4          # no vector rows: two kernels
+    assert ws(8, 4, 2, 64, 64, _lib.BF16) == ws(0, 4, 2, 64, 64, _lib.BF16) == 0       # one cluster
+    assert ws(8, 4, 2, 0, 64, _lib.BF16) == ws(-1, 4, 2, 64, 64, _lib.BF16) == ws(8, 4, 2, 64, 64, 7) == 0
 
 
 @pytest.mark.parametrize("cache", [
     dict(heads_=1), dict(dim=128), dict(dtype=_lib.F16), dict(dtype=4), dict(dtype=_lib.KV_E4M3), dict(page=0),
-    dict(pages=-1), dict(k=0), dict(k=0x10000008)])
+    dict(pages=-1), dict(k=0), dict(k=0xD0000008)])
 def test_write_refuses_caches(cache):
     keep, at = _cache(**cache)
     assert L.rmsnorm_qk_rope_write(_rope(v=V, slots=SLOTS, cache=at), None) == _lib.ERR_INVALID
@@ -96,8 +99,8 @@ def test_write_checks():
     assert call(cache=e4m3, dtype=_lib.F32) == _lib.ERR_CUDA
 
 
-def _back(dqo=Q, dko=K, q=0x3000000, k=0x4000000, dq=QO, dk=KO, dw=W, dkw=W, qw=W, kw=W, ws=V, nbytes=1024 * 64 * 4,
-          tokens=8, r=64):
+def _back(dqo=Q, dko=K, q=0xB0000000, k=0xC0000000, dq=QO, dk=KO, dw=W, dkw=W, qw=W, kw=W, ws=V, nbytes=1024 * 64 * 4,
+          tokens=8000, r=64):
     s = (256, 64, 128, 64)
     return L.rmsnorm_qk_rope_backward(heads._BACK_ARGS.pack(
         dqo, dko, q, k, dq, dk, dw, dkw, qw, kw, TABLE, POS, ws, nbytes, *s, *s, tokens, 100, 4, 2, 64, r, _lib.BF16, 0,
@@ -107,8 +110,9 @@ def _back(dqo=Q, dko=K, q=0x3000000, k=0x4000000, dq=QO, dk=KO, dw=W, dkw=W, qw=
 def test_backward_checks():
     assert _back() == _lib.ERR_CUDA
     assert _back(q=0, k=0, dw=0, qw=0, kw=0, ws=0, nbytes=0) == _lib.ERR_CUDA      # rotation alone
+    assert _back(tokens=8, ws=0, nbytes=0) == _lib.ERR_CUDA                        # one cluster
     for kw in (dict(dw=0), dict(dkw=0), dict(ws=0), dict(nbytes=1024 * 64 * 4 - 1), dict(qw=0), dict(q=0), dict(dq=Q),
-               dict(dk=0x4000000), dict(dk=QO + 512), dict(dqo=0), dict(r=1), dict(tokens=-1)):
+               dict(dk=0xC0000000), dict(dk=QO + 512), dict(tokens=8, dw=0), dict(tokens=8, dq=Q), dict(dqo=0), dict(r=1), dict(tokens=-1)):
         assert _back(**kw) == _lib.ERR_INVALID, kw
 
 
