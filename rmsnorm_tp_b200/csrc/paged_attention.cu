@@ -28,7 +28,7 @@ struct AttnArgs {
   int row_groups;       // groups of 8 (16) query heads that share a kv head
   int segments;         // kv heads * row_groups
   int q_pairs;          // the queries' elements can be read two at a time
-  int whole_pages;      // pages of 16 k tokens
+  int whole_pages;      // pages hold whole tiles of a warp
   int undivided;        // a CTA for each segment, which no other shares
   FastDiv page_div;
   float scale_log2;     // scale * log2(e): scores in base 2
@@ -174,7 +174,6 @@ __global__ void __launch_bounds__(kAnyBlock) attention_join_any_kernel(const __g
 // rescaling; exponentials are then at most 2^8.
 constexpr int kWarps = 4;
 constexpr int kBlock = 32 * kWarps;
-constexpr int kTile = 16 * kWarps;      // tokens of a CTA's tile
 constexpr float kSlack = 8.f;           // log2 of the largest exponential
 constexpr int kJoinBlock = 256;         // threads of the join kernel
 constexpr int kSegment = 1;             // cost of a segment's begin and end, in tiles
@@ -195,8 +194,16 @@ struct Shape {
   // either way 8 rows of one chunk fall into 8 different bank groups
   static constexpr bool kSwizzle = kChunks % 8 == 0;
   static constexpr int kPitch = (kSwizzle ? kChunks : (kChunks | 1)) * 16;
-  static constexpr int kOperand = 16 * kPitch;               // one warp's K (or V) tile
-  static constexpr int kSide = kE4M3 ? 128 + 16 : 16;        // its scales and its mask, behind the rings
+  // tokens of a warp's tile, in blocks of 16: two where a row is short (e4m3) and the
+  // registers allow it, so that the loop's own work is shared by more of them. 64 sequences
+  // of 4096 tokens and 4 kv heads, one and two blocks: head_dim 64 42 and 36 us, 128 55 and
+  // 53, 256 115 and 96; but 96 56 and 60, 192 83 and 93 (fewer CTAs fit), which keep one.
+  static constexpr int kBlocks = kE4M3 && NG == 1 && D != 96 && D != 192 ? 2 : 1;
+  static constexpr int kTok = 16 * kBlocks;
+  static constexpr int kTile = kTok * kWarps;                // of a CTA's tile
+  static constexpr int kOperand = kTok * kPitch;             // one warp's K (or V) tile
+  static constexpr int kScales = kE4M3 ? 8 * kTok : 0;       // bytes of its scales
+  static constexpr int kSide = kScales + 16;                 // they and its mask, behind the rings
   static constexpr int kTiles = 2 * kOperand;
   static constexpr int kStage = kTiles + kSide;
   // lanes that load one row, and rows of one load instruction
@@ -309,12 +316,15 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
   return a / b;
 }
 
+template <int kTile>
 __device__ __forceinline__ int tiles_of(int64_t len) { return (int)((len + kTile - 1) / kTile); }
 
 // Shares of a sequence's segment: its tiles, and kSegment for its queries and its join.
-__device__ __forceinline__ int64_t shares_of(int64_t len) { return len == 0 ? 0 : tiles_of(len) + kSegment; }
+template <int kTile>
+__device__ __forceinline__ int64_t shares_of(int64_t len) { return len == 0 ? 0 : tiles_of<kTile>(len) + kSegment; }
 
 // To the next tile, if rem says that there is one.
+template <int kTile>
 __device__ __forceinline__ void advance(const AttnArgs& a, Place& p) {
   --p.rem;
   if (++p.tile < p.tiles) return;
@@ -329,7 +339,7 @@ __device__ __forceinline__ void advance(const AttnArgs& a, Place& p) {
     ++p.b;
     p.len = (int)length_of(a, p.b);
   } while (p.len == 0);
-  p.tiles = tiles_of(p.len);
+  p.tiles = tiles_of<kTile>(p.len);
 }
 
 // NG: groups of 8 query heads that one CTA holds.
@@ -345,7 +355,8 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
   // fp16 numerators run up to 2^15, so that fp16's smallest number is 2^-39 of the largest
   constexpr float kLiftLog2 = kBf16 || kE4M3 ? 0.f : 15.f - kSlack;
   constexpr float kLift = kBf16 || kE4M3 ? 1.f : 128.f;
-  constexpr int KS = D / 16;
+  constexpr int KS = D / 16, MB = S::kBlocks, kTok = S::kTok, kTile = S::kTile;
+  constexpr unsigned kAll = kTok == 32 ? ~0u : 0xFFFFu;
   constexpr int kRows = 8 * NG;
   extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ float s_m[kWarps][kRows], s_l[kWarps][kRows], s_v[kWarps][kRows];
@@ -369,14 +380,14 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
     at.b = (int)((unsigned)blockIdx.x / (unsigned)a.segments);
     hs = (int)((unsigned)blockIdx.x - (unsigned)at.b * a.segments);
     at.len = (int)length_of(a, at.b);
-    at.tiles = tiles_of(at.len);
+    at.tiles = tiles_of<kTile>(at.len);
     at.tile = 0;
     at.rem = at.tiles;
   } else {
     const int64_t per = (a.batch + kBlock - 1) / kBlock;
     int64_t mine = 0;
     for (int64_t b = tid * per; b < (tid + 1) * per && b < a.batch; ++b)
-      mine += shares_of(length_of(a, b)) * a.segments;
+      mine += shares_of<kTile>(length_of(a, b)) * a.segments;
     int64_t upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -402,7 +413,7 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
       int64_t rest = t0 - (upto - mine);
       int64_t b = tid * per;
       for (;; ++b) {
-        const int64_t n = shares_of(length_of(a, b)) * a.segments;
+        const int64_t n = shares_of<kTile>(length_of(a, b)) * a.segments;
         if (rest < n) break;
         rest -= n;
       }
@@ -412,7 +423,7 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
     __syncthreads();
     at.b = s_b;
     at.len = (int)length_of(a, at.b);
-    at.tiles = tiles_of(at.len);
+    at.tiles = tiles_of<kTile>(at.len);
     hs = (int)quotient(s_rest, at.tiles + kSegment);
     const int into_segment = (int)(s_rest - (int64_t)hs * (at.tiles + kSegment)) - kSegment;
     at.tile = into_segment > 0 ? into_segment : 0;
@@ -456,18 +467,17 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
   const int lr = lane / S::kLanes, lc = lane % S::kLanes;
   const unsigned char* kp = static_cast<const unsigned char*>(a.k) + lc * 16;
   const unsigned char* vp = static_cast<const unsigned char*>(a.v) + lc * 16;
-  constexpr uint32_t kMaskOff = kE4M3 ? 128 : 0;
   // this lane's chunk of its row in the tile, for rows lr and lr + 4 of 8
   const uint32_t to0 = lr * S::kPitch + (S::kSwizzle ? lc ^ (lr & 7) : lc) * 16;
   const uint32_t to1 = lr * S::kPitch + (S::kSwizzle ? lc ^ ((lr + S::kRowsAtOnce) & 7) : lc) * 16;
-  const int lane_tok = warp * 16 + (a.whole_pages ? 0 : lane & 15);
+  const int lane_tok = warp * kTok + (a.whole_pages ? 0 : lane & (kTok - 1));
   Place ahead = at;
   uint32_t into = 0;                  // stage that the next tile goes to
   int32_t page_id = -1, page_off = 0; // read one tile early
   int table_of = -1;
   const int32_t* table = nullptr;     // of sequence table_of
-  // pages of 16 k tokens: the warp's 16 tokens lie in one page, one row behind another;
-  // else lane l (and l + 16) knows the row of token l
+  // whole pages of tiles: the warp's tokens lie in one page, one row behind another; else
+  // lane l (for 16 tokens also l + 16) knows the row of token l
   auto look_up = [&]() {
     const int t = ahead.tile * kTile + lane_tok;
     const unsigned pg = a.page_div.quotient(t);
@@ -487,20 +497,21 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
       const int64_t row = live ? ((int64_t)page_id * a.hk + ahead.kvh) * a.page + page_off : 0;
       const int rest = ahead.len - (ahead.tile * kTile + lane_tok);
       unsigned mask;
-      if (a.whole_pages) mask = !live ? 0u : rest >= 16 ? 0xFFFFu : (1u << rest) - 1u;
-      else mask = __ballot_sync(0xFFFFFFFFu, live) & 0xFFFFu;
-      if (lane == 0) *reinterpret_cast<unsigned*>(side + kMaskOff) = mask;
-      if constexpr (kE4M3) {          // lanes 0-15 K's scales, 16-31 V's
-        const int64_t r = a.whole_pages ? row + (lane & 15) : row;
-        const bool on = (mask >> (lane & 15)) & 1u;
-        cp_async4_if(ptx::smem_addr(side) + lane * 4, (lane < 16 ? a.ks : a.vs) + (on ? r : 0), on);
+      if (a.whole_pages) mask = !live ? 0u : rest >= kTok ? kAll : (1u << rest) - 1u;
+      else mask = __ballot_sync(0xFFFFFFFFu, live) & kAll;
+      if (lane == 0) *reinterpret_cast<unsigned*>(side + S::kScales) = mask;
+      if constexpr (kE4M3) {          // K's scales, then V's: for 16 tokens half the lanes each
+        const int64_t r = a.whole_pages ? row + (lane & (kTok - 1)) : row;
+        const bool on = (mask >> (lane & (kTok - 1))) & 1u;
+        cp_async4_if(ptx::smem_addr(side) + lane * 4, (lane < kTok ? a.ks : a.vs) + (on ? r : 0), on);
+        if (kTok == 32) cp_async4_if(ptx::smem_addr(side) + 128 + lane * 4, a.vs + (on ? r : 0), on);
       }
-      if (a.whole_pages && mask == 0xFFFFu) {
+      if (a.whole_pages && mask == kAll) {
         const int64_t from = (row + lr) * S::kRowBytes;
         const unsigned char* kf = kp + from;
         const unsigned char* vf = vp + from;
 #pragma unroll
-        for (int i = 0; i < 16 / S::kRowsAtOnce; ++i)
+        for (int i = 0; i < kTok / S::kRowsAtOnce; ++i)
 #pragma unroll
           for (int k = 0; k < S::kChunks / S::kLanes; ++k) {
             const uint32_t to = dst + (i & 1 ? to1 : to0) + i * S::kRowsAtOnce * S::kPitch + k * S::kLanes * 16;
@@ -510,7 +521,7 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
           }
       } else {
 #pragma unroll
-        for (int i = 0; i < 16 / S::kRowsAtOnce; ++i) {
+        for (int i = 0; i < kTok / S::kRowsAtOnce; ++i) {
           const int r = i * S::kRowsAtOnce + lr;
           const int64_t from = (a.whole_pages ? row + r : __shfl_sync(0xFFFFFFFFu, row, r)) * S::kRowBytes;
           const bool on = (mask >> r) & 1u;
@@ -524,7 +535,7 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
         }
       }
       into = into + 1 == S::kStages ? 0 : into + 1;
-      advance(a, ahead);
+      advance<kTile>(a, ahead);
       if (ahead.rem > 0) look_up();
     }
     cp_commit();
@@ -627,71 +638,84 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
       const uint32_t k_at = ring + stage * S::kTiles + k_lane, v_at = ring + stage * S::kTiles + v_lane;
       const unsigned char* side = sides + stage * S::kSide;
       stage = stage + 1 == S::kStages ? 0 : stage + 1;
-      const unsigned mask = *reinterpret_cast<const unsigned*>(side + kMaskOff);
+      const unsigned mask = *reinterpret_cast<const unsigned*>(side + S::kScales);
       if (mask != 0u) {
-        float s[NG][4];                 // (token g, heads 2 qd, 2 qd + 1), (token g + 8, the same)
-        {
+        // (token g, heads 2 qd, 2 qd + 1), (token g + 8, the same) of each block
+        float s[MB][NG][4];
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) {
           float s2[NG][4];              // the odd steps' sums: two chains instead of one
 #pragma unroll
           for (int x = 0; x < NG; ++x)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[x][j] = s2[x][j] = 0.f;
+            for (int j = 0; j < 4; ++j) s[mb][x][j] = s2[x][j] = 0.f;
 #pragma unroll
           for (int ks = 0; ks < KS; ks += 2) {
             uint32_t r[4], r2[4];
+            const uint32_t from = k_at + mb * 16 * S::kPitch;
             if constexpr (kE4M3) {
               uint32_t w[4];
-              ldsm4(w, chunk(k_at, ks));
+              ldsm4(w, chunk(from, ks));
               r[0] = e4m3x2_f16x2(w[0]), r[2] = e4m3x2_f16x2(w[0] >> 16);
               r[1] = e4m3x2_f16x2(w[1]), r[3] = e4m3x2_f16x2(w[1] >> 16);
               r2[0] = e4m3x2_f16x2(w[2]), r2[2] = e4m3x2_f16x2(w[2] >> 16);
               r2[1] = e4m3x2_f16x2(w[3]), r2[3] = e4m3x2_f16x2(w[3] >> 16);
             } else {
-              ldsm4(r, chunk(k_at, 2 * ks));
-              ldsm4(r2, chunk(k_at, 2 * ks + 2));
+              ldsm4(r, chunk(from, 2 * ks));
+              ldsm4(r2, chunk(from, 2 * ks + 2));
             }
 #pragma unroll
             for (int x = 0; x < NG; ++x) {
-              mma<kBf16>(s[x], r, q[x][ks][0], q[x][ks][1]);
+              mma<kBf16>(s[mb][x], r, q[x][ks][0], q[x][ks][1]);
               mma<kBf16>(s2[x], r2, q[x][ks + 1][0], q[x][ks + 1][1]);
             }
           }
 #pragma unroll
           for (int x = 0; x < NG; ++x)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[x][j] += s2[x][j];
+            for (int j = 0; j < 4; ++j) s[mb][x][j] += s2[x][j];
         }
-        const bool on[2] = {(bool)((mask >> g) & 1u), (bool)((mask >> (g + 8)) & 1u)};
-        float ksc[2] = {1.f, 1.f}, lv[2] = {0.f, 0.f};
-        if constexpr (kE4M3) {
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            ksc[t] = reinterpret_cast<const float*>(side)[8 * t + g];
-            lv[t] = lg2(reinterpret_cast<const float*>(side)[16 + 8 * t + g]);
-          }
-        }
+        // tokens g + 8 t of all blocks
+        bool on[2 * MB];
+        float lv[2 * MB];
         bool rise = false;
 #pragma unroll
-        for (int x = 0; x < NG; ++x)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int t = j >> 1, h = j & 1;
-            s[x][j] = on[t] ? s[x][j] * (kE4M3 ? unit[x][h] * ksc[t] : unit[x][h]) : -INFINITY;
-            rise |= s[x][j] > m[x][h] + kSlack;
-            if constexpr (kE4M3) rise |= on[t] && s[x][j] + lv[t] > mv[x][h] + kSlack;
+        for (int t = 0; t < 2 * MB; ++t) {
+          on[t] = (mask >> (g + 8 * t)) & 1u;
+          float ksc = 1.f;
+          lv[t] = 0.f;
+          if constexpr (kE4M3) {
+            ksc = reinterpret_cast<const float*>(side)[8 * t + g];
+            lv[t] = lg2(reinterpret_cast<const float*>(side)[kTok + 8 * t + g]);
           }
+#pragma unroll
+          for (int x = 0; x < NG; ++x)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              float& v = s[t >> 1][x][2 * (t & 1) + h];
+              v = on[t] ? v * (kE4M3 ? unit[x][h] * ksc : unit[x][h]) : -INFINITY;
+              rise |= v > m[x][h] + kSlack;
+              if constexpr (kE4M3) rise |= on[t] && v + lv[t] > mv[x][h] + kSlack;
+            }
+        }
         if (__any_sync(0xFFFFFFFFu, rise)) {
 #pragma unroll
           for (int x = 0; x < NG; ++x)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const float now = fmaxf(m[x][h], head_max(fmaxf(s[x][h], s[x][2 + h])));
+              float top = -INFINITY, topv = -INFINITY;
+#pragma unroll
+              for (int t = 0; t < 2 * MB; ++t) {
+                const float v = s[t >> 1][x][2 * (t & 1) + h];
+                top = fmaxf(top, v);
+                if (on[t]) topv = fmaxf(topv, v + lv[t]);
+              }
+              const float now = fmaxf(m[x][h], head_max(top));
               float keep = ex2(m[x][h] - ref_of(now));
               l[x][h] *= keep;
               m[x][h] = now;
               if constexpr (kE4M3) {
-                const float nowv = fmaxf(mv[x][h], head_max(fmaxf(on[0] ? s[x][h] + lv[0] : -INFINITY,
-                                                                 on[1] ? s[x][2 + h] + lv[1] : -INFINITY)));
+                const float nowv = fmaxf(mv[x][h], head_max(topv));
                 keep = ex2(mv[x][h] - ref_of(nowv));
                 mv[x][h] = nowv;
               }
@@ -702,57 +726,61 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
               }
             }
         }
-        uint32_t hi[NG][2], lo[NG][2];  // P as 16 tokens x 8 heads
+        uint32_t hi[MB][NG][2], lo[MB][NG][2];   // P as 16 tokens x 8 heads
 #pragma unroll
         for (int x = 0; x < NG; ++x) {
           const float ref[2] = {ref_of(m[x][0]), ref_of(m[x][1])};
           const float refv[2] = {ref_of(mv[x][0]), ref_of(mv[x][1])};
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
+          for (int t = 0; t < 2 * MB; ++t) {
+            uint32_t& to_hi = hi[t >> 1][x][t & 1];
+            uint32_t& to_lo = lo[t >> 1][x][t & 1];
             float w[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const float v = s[x][2 * t + h], p = ex2(v - ref[h]);
+              const float v = s[t >> 1][x][2 * (t & 1) + h], p = ex2(v - ref[h]);
               l[x][h] += p;
               w[h] = kE4M3 ? (on[t] ? ex2(v + lv[t] - refv[h]) : 0.f) : p * kLift;
             }
             if constexpr (kTwoParts) {
-              split2<kBf16>(w[0], w[1], hi[x][t], lo[x][t]);
-              lo[x][t] = transposed(lo[x][t]);
+              split2<kBf16>(w[0], w[1], to_hi, to_lo);
+              to_lo = transposed(to_lo);
             } else {
-              hi[x][t] = pack2<kBf16>(w[0], w[1]);
+              to_hi = pack2<kBf16>(w[0], w[1]);
             }
-            hi[x][t] = transposed(hi[x][t]);
+            to_hi = transposed(to_hi);
           }
         }
 #pragma unroll
-        for (int j = 0; j < KS; j += kE4M3 ? 2 : 1) {
-          uint32_t r[4], r2[4];
-          const uint32_t from = chunk(v_at, kE4M3 ? j : 2 * j);
-          if constexpr (kE4M3) {
-            // bytes of w: (token 2 qd: elements 2 g, 2 g + 1), (token 2 qd + 1: the same), so row g
-            // of the product is element 2 g and row g + 8 element 2 g + 1
-            uint32_t w[4];
-            ldsm4t(w, from);
+        for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-            for (int t = 0; t < 4; ++t) w[t] = __byte_perm(w[t], 0, 0x3120);
-            r[0] = e4m3x2_f16x2(w[0]), r[1] = e4m3x2_f16x2(w[0] >> 16);
-            r[2] = e4m3x2_f16x2(w[1]), r[3] = e4m3x2_f16x2(w[1] >> 16);
-            r2[0] = e4m3x2_f16x2(w[2]), r2[1] = e4m3x2_f16x2(w[2] >> 16);
-            r2[2] = e4m3x2_f16x2(w[3]), r2[3] = e4m3x2_f16x2(w[3] >> 16);
-          } else {
-            ldsm4t(r, from);
-          }
-#pragma unroll
-          for (int x = 0; x < NG; ++x) {
-            mma<kBf16>(o[x][j], r, hi[x][0], hi[x][1]);
-            if constexpr (kTwoParts) mma<kBf16>(o[x][j], r, lo[x][0], lo[x][1]);
+          for (int j = 0; j < KS; j += kE4M3 ? 2 : 1) {
+            uint32_t r[4], r2[4];
+            const uint32_t from = chunk(v_at + mb * 16 * S::kPitch, kE4M3 ? j : 2 * j);
             if constexpr (kE4M3) {
-              mma<kBf16>(o[x][j + 1], r2, hi[x][0], hi[x][1]);
-              if constexpr (kTwoParts) mma<kBf16>(o[x][j + 1], r2, lo[x][0], lo[x][1]);
+              // bytes of w: (token 2 qd: elements 2 g, 2 g + 1), (token 2 qd + 1: the same), so row
+              // g of the product is element 2 g and row g + 8 element 2 g + 1
+              uint32_t w[4];
+              ldsm4t(w, from);
+#pragma unroll
+              for (int t = 0; t < 4; ++t) w[t] = __byte_perm(w[t], 0, 0x3120);
+              r[0] = e4m3x2_f16x2(w[0]), r[1] = e4m3x2_f16x2(w[0] >> 16);
+              r[2] = e4m3x2_f16x2(w[1]), r[3] = e4m3x2_f16x2(w[1] >> 16);
+              r2[0] = e4m3x2_f16x2(w[2]), r2[1] = e4m3x2_f16x2(w[2] >> 16);
+              r2[2] = e4m3x2_f16x2(w[3]), r2[3] = e4m3x2_f16x2(w[3] >> 16);
+            } else {
+              ldsm4t(r, from);
+            }
+#pragma unroll
+            for (int x = 0; x < NG; ++x) {
+              mma<kBf16>(o[x][j], r, hi[mb][x][0], hi[mb][x][1]);
+              if constexpr (kTwoParts) mma<kBf16>(o[x][j], r, lo[mb][x][0], lo[mb][x][1]);
+              if constexpr (kE4M3) {
+                mma<kBf16>(o[x][j + 1], r2, hi[mb][x][0], hi[mb][x][1]);
+                if constexpr (kTwoParts) mma<kBf16>(o[x][j + 1], r2, lo[mb][x][0], lo[mb][x][1]);
+              }
             }
           }
-        }
       }
     }
 
@@ -761,7 +789,7 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
     Place next = at;
     next.tile = end - 1;
     next.rem = at.rem - (end - 1 - at.tile);
-    advance(a, next);
+    advance<kTile>(a, next);
     if (next.rem > 0) load_q(next);
     {
       // ---- the warps' results of the segment, joined: half of 8 heads' elements at a time
@@ -959,7 +987,7 @@ __global__ void __launch_bounds__(kJoinBlock) attention_join_kernel(const __grid
 struct Kernels {
   const void* main;
   const void* join;
-  int smem, ctas, rows;
+  int smem, ctas, rows, warp_tokens;
   std::atomic<bool>* ready;   // per device: the shared-memory limit has been raised
 };
 constexpr int kMaxDevices = 64;
@@ -969,7 +997,8 @@ Kernels kernels() {
   static std::atomic<bool> ready[kMaxDevices];
   return Kernels{reinterpret_cast<const void*>(attention_kernel<TQ, kE4M3, D, NG>),
                  reinterpret_cast<const void*>(attention_join_kernel<TQ, D, NG>),
-                 Shape<D, kE4M3, NG>::kSmem, Shape<D, kE4M3, NG>::kCtas, 8 * NG, ready};
+                 Shape<D, kE4M3, NG>::kSmem, Shape<D, kE4M3, NG>::kCtas, 8 * NG,
+                 Shape<D, kE4M3, NG>::kTok, ready};
 }
 template <typename TQ, bool kE4M3, int NG>
 Kernels kernels_of(int d) {
@@ -1005,18 +1034,18 @@ Kernels find_kernels(const rmsnorm_paged_attention_args* a) {
 int row_groups_of(const rmsnorm_paged_attention_args* a, const Kernels& k) {
   return (a->q_heads / a->cache->kv_heads + k.rows - 1) / k.rows;
 }
-// Whether each segment gets a CTA of its own and there is no join: up to 8 tiles (512
-// tokens) of capacity. Divided and undivided, device time of 4 sequences of one kv head of
+// Whether each segment gets a CTA of its own and there is no join: up to 512 tokens of
+// capacity. Divided and undivided, device time of 4 sequences of one kv head of
 // 128: 7.9 and 5.9 us at 256 tokens, 8.4 and 10.5 at 512, 8.2 and 13.3 at 768, where the
 // second launch and the workspace cost the host 4 us; 128 such segments: 9.9 and 7.9, 12.9
 // and 10.7, 14.4 and 13.7.
 bool undivided(const rmsnorm_paged_attention_args* a, const Kernels& k) {
-  const int64_t tiles = (a->max_pages * a->cache->page_size + kTile - 1) / kTile;
-  return tiles <= 8 && a->batch * a->cache->kv_heads * row_groups_of(a, k) < (int64_t(1) << 30);
+  return a->max_pages * a->cache->page_size <= 512 && a->batch * a->cache->kv_heads * row_groups_of(a, k) < (int64_t(1) << 30);
 }
 // CTAs of the main kernel: one resident wave, or a tile each of the longest lengths.
 int64_t worker_count(const rmsnorm_paged_attention_args* a, const Kernels& k, int sms) {
-  const int64_t tiles = (a->max_pages * a->cache->page_size + kTile - 1) / kTile;
+  const int tile = k.warp_tokens * kWarps;
+  const int64_t tiles = (a->max_pages * a->cache->page_size + tile - 1) / tile;
   const int64_t most = tiles * a->batch * a->cache->kv_heads * row_groups_of(a, k);
   const int64_t wave = (int64_t)sms * k.ctas;
   return most < 1 ? 1 : most < wave ? most : wave;
@@ -1055,7 +1084,7 @@ int check_attention(const char* who, const rmsnorm_paged_attention_args* a) {
   if (a->max_pages < 0 || a->max_pages * (int64_t)c->page_size > kMostTokens)
     return refuse(RMSNORM_TP_ERR_INVALID, "%s: %lld pages of %d tokens: a sequence holds at most 2^31 - 128",
                   who, (long long)a->max_pages, c->page_size);
-  if ((a->max_pages * (int64_t)c->page_size / kTile + 2) * a->batch * a->q_heads > kMostTiles)
+  if ((a->max_pages * (int64_t)c->page_size / 64 + 2) * a->batch * a->q_heads > kMostTiles)
     return refuse(RMSNORM_TP_ERR_INVALID, "%s: %lld sequences of %d heads and %lld tokens: too many", who,
                   (long long)a->batch, a->q_heads, (long long)(a->max_pages * (int64_t)c->page_size));
   if (a->device < 0) return refuse(RMSNORM_TP_ERR_INVALID, "%s: device %d", who, a->device);
@@ -1136,7 +1165,7 @@ int rmsnorm_paged_attention(const rmsnorm_paged_attention_args* in, void* stream
   if (k.main != nullptr) {
     a.row_groups = row_groups_of(in, k);
     a.segments = a.hk * a.row_groups;
-    a.whole_pages = a.page % 16 == 0;
+    a.whole_pages = a.page % k.warp_tokens == 0;
     a.page_div = FastDiv::of(a.page);
     if (in->device >= kMaxDevices || !k.ready[in->device]) {
       const cudaError_t e =
