@@ -466,7 +466,7 @@ struct Ring {
 };
 
 using RopeRing = Ring<2, 4>;             // x
-using BackRing = Ring<4, 3>;             // dy and x
+using BackRing = Ring<4, 2>;             // dy and x
 
 // `run` groups of 32 / L rows of one operand. kTurned: normed and turned (else as they are:
 // the values on their way to the cache).
