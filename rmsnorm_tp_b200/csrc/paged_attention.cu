@@ -209,17 +209,20 @@ struct Shape {
   // lanes that load one row, and rows of one load instruction
   static constexpr int kLanes = kChunks % 8 == 0 ? 8 : kChunks % 4 == 0 ? 4 : 2;
   static constexpr int kRowsAtOnce = 32 / kLanes;
-  static constexpr int kJoinPitch = D / 2 + 4;
-  static constexpr int kJoin = kWarps * 8 * kJoinPitch * 4;
-  // three CTAs of at most 73 KB on an SM (and 168 registers a thread: NG = 1) where at
-  // least three stages fit, else two of 110 KB, else one
-  static constexpr int kThree = NG == 1 ? (73 * 1024 - kJoin) / (kWarps * kStage) : 0;
-  static constexpr int kTwo = (110 * 1024 - kJoin) / (kWarps * kStage);
-  static constexpr int kOne = (220 * 1024 - kJoin) / (kWarps * kStage);
+  // a segment's join goes through the stage that each warp has just left: 8 heads of fp32 at
+  // once where they fit it, else half their elements
+  static constexpr int kHalves = 8 * (D + 4) * 4 <= kTiles ? 1 : 2;
+  static constexpr int kJoinPitch = D / kHalves + 4;         // 8 heads' rows on all banks
+  static_assert(8 * kJoinPitch * 4 <= kTiles, "the join fits a stage");
+  // three CTAs of at most 74 KB on an SM (and 168 registers a thread: NG = 1) where at
+  // least three stages fit, else two of 111 KB, else one
+  static constexpr int kThree = NG == 1 ? 74 * 1024 / (kWarps * kStage) : 0;
+  static constexpr int kTwo = 111 * 1024 / (kWarps * kStage);
+  static constexpr int kOne = 222 * 1024 / (kWarps * kStage);
   static constexpr int kCtas = kThree >= 3 ? 3 : kTwo >= 3 ? 2 : 1;
   static constexpr int kFit = kCtas == 3 ? kThree : kCtas == 2 ? kTwo : kOne;
   static constexpr int kStages = kFit > 6 ? 6 : kFit;
-  static constexpr int kSmem = kJoin + kWarps * kStages * kStage;
+  static constexpr int kSmem = kWarps * kStages * kStage;
   static_assert(kStages >= 3, "the ring needs three stages");
 };
 
@@ -457,11 +460,10 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
     return;
   }
 
-  float* join = reinterpret_cast<float*>(smem);
-  static_assert(S::kJoin % 128 == 0 && (!S::kSwizzle || S::kPitch % 128 == 0),
-                "the swizzle's address bits are those of a chunk in 128 bytes");
-  const uint32_t ring = ptx::smem_addr(smem) + S::kJoin + warp * S::kStages * S::kTiles;
-  unsigned char* sides = smem + S::kJoin + kWarps * S::kStages * S::kTiles + warp * S::kStages * S::kSide;
+  static_assert(!S::kSwizzle || S::kPitch % 128 == 0, "the swizzle's address bits are those of a chunk in 128 bytes");
+  constexpr int kRing = S::kStages * S::kTiles;   // of a warp
+  const uint32_t ring = ptx::smem_addr(smem) + warp * kRing;
+  unsigned char* sides = smem + kWarps * kRing + warp * S::kStages * S::kSide;
 
   // ---- loads ----
   const int lr = lane / S::kLanes, lc = lane % S::kLanes;
@@ -792,7 +794,9 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
     advance<kTile>(a, next);
     if (next.rem > 0) load_q(next);
     {
-      // ---- the warps' results of the segment, joined: half of 8 heads' elements at a time
+      // ---- the warps' results of the segment, joined through the stages just left (the next
+      // copies into them are sent behind the last barrier)
+      unsigned char* left = smem + (stage == 0 ? S::kStages - 1 : stage - 1) * S::kTiles;
 #pragma unroll
       for (int x = 0; x < NG; ++x)
 #pragma unroll
@@ -812,18 +816,18 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
                   2ll * gridDim.x * kRows * 2 + slot * kRows * D;
       if (tid == 0 && began && !last)
         meta[1] = share_of(at, t1 - end);
-      constexpr int kHalf = D / 2;
+      constexpr int kPart = D / S::kHalves;   // elements of a head at a time
 #pragma unroll
       for (int x = 0; x < NG; ++x) {
         if (8 * x >= rows) break;
 #pragma unroll
-        for (int dh = 0; dh < 2; ++dh) {
-          float* to = join + (warp * 8 + 2 * qd) * S::kJoinPitch;
+        for (int dh = 0; dh < S::kHalves; ++dh) {
+          float* to = reinterpret_cast<float*>(left + warp * kRing) + 2 * qd * S::kJoinPitch;
 #pragma unroll
-          for (int j = 0; j < KS / 2; ++j)
+          for (int j = 0; j < KS / S::kHalves; ++j)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const float (&v)[4] = o[x][dh * (KS / 2) + j];
+              const float (&v)[4] = o[x][dh * (KS / S::kHalves) + j];
               float* p = to + h * S::kJoinPitch + 16 * j;
               if constexpr (kE4M3) {
                 *reinterpret_cast<float2*>(p + 2 * g) = make_float2(v[h], v[2 + h]);
@@ -833,8 +837,8 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
               }
             }
           __syncthreads();
-          for (int u = tid; u < 8 * (kHalf / 4); u += kBlock) {
-            const int r8 = u / (kHalf / 4), e = (u - r8 * (kHalf / 4)) * 4, r = 8 * x + r8;
+          for (int u = tid; u < 8 * (kPart / 4); u += kBlock) {
+            const int r8 = u / (kPart / 4), e = (u - r8 * (kPart / 4)) * 4, r = 8 * x + r8;
             if (r >= rows) continue;
             float mm = -INFINITY, ll = 0.f;
 #pragma unroll
@@ -845,18 +849,19 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
             for (int w = 0; w < kWarps; ++w) {
               ll += s_l[w][r] * ex2(s_m[w][r] - ref);
               const float f = s_v[w][r] == -INFINITY ? 0.f : ex2(s_v[w][r] - ref);
-              const float4 z = *reinterpret_cast<const float4*>(join + (w * 8 + r8) * S::kJoinPitch + e);
+              const float4 z =
+                  *reinterpret_cast<const float4*>(reinterpret_cast<float*>(left + w * kRing) + r8 * S::kJoinPitch + e);
               y.x = fmaf(f, z.x, y.x);
               y.y = fmaf(f, z.y, y.y);
               y.z = fmaf(f, z.z, y.z);
               y.w = fmaf(f, z.w, y.w);
             }
-            const int at_e = dh * kHalf + e;
+            const int at_e = dh * kPart + e;
             if (whole) {
-              const float d = ll == 0.f ? 1.f : ll;   // no weight at all: o is 0
+              const float over = 1.f / (ll == 0.f ? 1.f : ll);   // no weight at all: o is 0
               uint2 out;
-              out.x = pack2<kQBf16>(y.x / d, y.y / d);
-              out.y = pack2<kQBf16>(y.z / d, y.w / d);
+              out.x = pack2<kQBf16>(y.x * over, y.y * over);
+              out.y = pack2<kQBf16>(y.z * over, y.w * over);
               *reinterpret_cast<uint2*>(static_cast<TQ*>(a.out) + (out_row + r) * D + at_e) = out;
               if (a.lse && at_e == 0) a.lse[out_row + r] = kLn2 * (ref + log2f(ll));
             } else {
