@@ -103,8 +103,10 @@ def parse_args(argv=None):
     ap.add_argument("--no-cpu-baseline", action="store_true")
     ap.add_argument("--no-parity", action="store_true",
                     help="skip the untimed parity check (profiling runs)")
-    ap.add_argument("--op", choices=["norm", "linear"], default="norm",
-                    help="linear: the fused row-parallel linear -> reduce-scatter -> TP RMSNorm "
+    ap.add_argument("--op", choices=["norm", "linear", "attention"], default="norm",
+                    help="attention: what runs between the norms of a decode step on one rank's "
+                         "heads (head norms + rotation + cache write, attention over the cache), "
+                         "one JSON line per batch and cache type; linear: the fused row-parallel linear -> reduce-scatter -> TP RMSNorm "
                          "(Llama-70B o_proj rows: hidden 8192, in-features 8192 split over N), "
                          "one JSON line per row count, beside the unfused torch + NCCL pipeline")
     ap.add_argument("--emulated-tp", type=int, default=0,
@@ -1181,6 +1183,61 @@ def run_linear_bench(args):
     return 0
 
 
+def run_attention_bench(args):
+    """--op attention: a decode step of one rank's heads between its two norms -- head norms,
+    rotation and the write into a paged cache in one call, then the attention of the new
+    tokens over 2048 to 4096 cached tokens each -- on Llama-70B heads (64 query and 8 key
+    heads of 128, bf16) of a TP group of 8 and whole, over a bf16 and an e4m3 cache. Times a
+    CUDA graph of both calls; the caches of the calls in the graph are different ones, larger
+    than L2 together. Not a workload of the reference, which has the norms alone."""
+    import rmsnorm_tp_b200 as rtp
+
+    torch.cuda.set_device(0)
+    d, page, dtype = 128, 64, torch.bfloat16
+    hbm, _kind = measured_peak_hbm()
+    rope = rtp.rope_table(8192, d, base=500000.0, device="cuda")
+    weight = torch.ones(d, dtype=dtype, device="cuda")
+    for hq, hk in ((8, 1), (64, 8)):
+        for batch in ([args.rows] if args.rows else [1, 16, 128]):
+            for held in (torch.bfloat16, torch.float8_e4m3fn):
+                g = torch.Generator(device="cuda").manual_seed(100 + batch)
+                lens = torch.randint(2048, 4097, (batch,), generator=g, device="cuda")
+                row = d * (2 if held == dtype else 1) + (0 if held == dtype else 4)
+                nbytes = int(lens.sum()) * hk * 2 * row
+                n = max(2, min(64, math.ceil(300e6 / nbytes)))
+                table = torch.randperm(batch * 64, generator=g, device="cuda").view(batch, 64).to(torch.int32)
+                slots = table.gather(1, ((lens - 1) // page)[:, None])[:, 0].long() * page + (lens - 1) % page
+                lens32, pos = lens.to(torch.int32), lens - 1
+                qkv = torch.randn(batch, (hq + 2 * hk) * d, generator=g, device="cuda").to(dtype)
+                q, k, v = (t.unflatten(1, (-1, d)) for t in qkv.split([hq * d, hk * d, hk * d], 1))
+                caches = []
+                for _ in range(n):
+                    c = rtp.PagedKVCache(batch * 64, page, hk, d, held)
+                    fill = torch.arange(batch * 64 * page, device="cuda")
+                    some = torch.randn(64, hk, d, generator=g, device="cuda").to(dtype)[fill % 64]
+                    rtp.qk_norm_rope_write(some, some, some, None, None, rope, fill % 4096, c, fill)
+                    caches.append(c)
+
+                def step(i):
+                    c = caches[i % n]
+                    a = rtp.qk_norm_rope_write(q, k, v, weight, weight, rope, pos, c, slots)
+                    return rtp.paged_attention(a, c, table, lens32)
+
+                for i in range(max(args.warmup, 3)):
+                    step(i)
+                torch.cuda.synchronize()
+                ms, calls = time_graph(step, n, min(args.steps, 400), 1)
+                us = ms * 1e3
+                emit(args, 0, {"op": "decode_attention", "q_heads": hq, "kv_heads": hk, "head_dim": d,
+                               "batch": batch, "cached_tokens": int(lens.sum()), "page": page,
+                               "dtype": "bf16", "cache": "bf16" if held == dtype else "e4m3",
+                               "graph_us_per_step": round(us, 3), "calls": calls,
+                               "cache_GBps": round(nbytes / us / 1e3, 1),
+                               "frac_of_copy": round(nbytes / us / 1e3 / hbm, 4)})
+                del caches
+    return 0
+
+
 def run_emulated(args):
     """--emulated-tp N: every rank of a TP group of N on one GPU in one cooperative
     launch, the workload's rows and hidden split over the ranks; for ncu captures
@@ -1226,6 +1283,8 @@ def main(argv=None):
         return run_reference_arm(args)
     if args.op == "linear":
         return run_linear_bench(args)
+    if args.op == "attention":
+        return run_attention_bench(args)
     if args.emulated_tp:
         return run_emulated(args)
     return run_our_arm(args)
