@@ -21,6 +21,8 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 ROOT_DIR = os.path.dirname(PKG_DIR)
@@ -50,7 +52,6 @@ NVCC_FLAGS = [
     "-lineinfo",
     "-Xcompiler", "-fPIC",
     "-Xcompiler", "-Wall",
-    "-shared",
     "-cudart", "static",
 ]
 
@@ -75,14 +76,24 @@ def build(force: bool = False, verbose: bool = False) -> str:
         return LIB_PATH
     os.makedirs(OUT_DIR, exist_ok=True)
     tmp = LIB_PATH + ".tmp"
-    cmd = [find_nvcc(), *NVCC_FLAGS, "-I", os.path.join(ROOT_DIR, "include"), "-o", tmp, *SOURCES]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if res.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
-    if verbose and (res.stdout or res.stderr):
-        print(res.stdout + res.stderr, flush=True)
+
+    def run(args):
+        cmd = [find_nvcc(), *NVCC_FLAGS, *args]
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError(f"nvcc failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
+        if verbose and (res.stdout or res.stderr):
+            print(res.stdout + res.stderr, flush=True)
+
+    # the sources at the same time (each is minutes of one core), then the link
+    with tempfile.TemporaryDirectory(dir=OUT_DIR) as objs:
+        objects = [os.path.join(objs, os.path.basename(p) + ".o") for p in SOURCES]
+        with ThreadPoolExecutor(max_workers=os.cpu_count() or 1) as pool:
+            list(pool.map(lambda so: run(["-I", os.path.join(ROOT_DIR, "include"), "-c", "-o", so[1], so[0]]),
+                          zip(SOURCES, objects)))
+        run(["-shared", "-o", tmp, *objects])
     os.replace(tmp, LIB_PATH)
     return LIB_PATH
 

@@ -176,8 +176,8 @@ __global__ void __launch_bounds__(kAnyBlock) attention_join_any_kernel(const __g
 //
 // Measured (device): 64 sequences of up to 16384 tokens, 32 + 8 heads of 128, e4m3 (1085 MB)
 // 170 us, 6.4 TB/s; one sequence of 262144 tokens, 8 + 1 heads of 128, bf16 (134 MB) 30 us:
-// 20 of streaming at 6.2 TB/s, 6 before the first tiles arrive (lengths, place, pages, rows:
-// four memory round trips), 4 of the join; 48 of up to 2011, 16 + 16 heads of 64, fp16
+// 21 of streaming at 6.2 TB/s, 4 before the first tiles arrive (lengths, place, pages, rows:
+// four memory round trips), 4.6 of the join; 48 of up to 2011, 16 + 16 heads of 64, fp16
 // (185 MB) 38 us. Groups of 9 to 16 query heads over e4m3 are bound by issue (0.6 of a copy).
 constexpr int kWarps = 4;
 constexpr int kBlock = 32 * kWarps;
@@ -890,7 +890,7 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
 
 // Joins what the CTAs left of a segment: every CTA that had a part of it takes an equal
 // share of its elements over all parts (one CTA for all of one head took 16 us of one long
-// sequence, this 4). A thread adds 4 elements of a head over some of the
+// sequence, this 4.6). A thread adds 4 elements of a head over some of the
 // parts (neighbouring threads the others), then the threads and warps of these
 // elements are added in a fixed order. Bound by latency (a few L2 round trips), so it is
 // kept short rather than unrolled.
