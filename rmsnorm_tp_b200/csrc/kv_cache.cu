@@ -209,7 +209,8 @@ extern "C" int rmsnorm_kv_read(const rmsnorm_kv_cache* c, void* k_out, void* v_o
   if (dtype != RMSNORM_TP_F32 && dtype != RMSNORM_TP_BF16 && dtype != RMSNORM_TP_F16)
     return refuse(RMSNORM_TP_ERR_INVALID, "%s: unknown dtype %d", who, dtype);
   // a thread for every 8 elements of 4 tokens, numbered in 31 bits
-  if (count < 0 || (count + kTokens) * (int64_t)c->kv_heads * (c->head_dim / 8) / kTokens >= (int64_t(1) << 31) - kBlock)
+  const int64_t units = (int64_t)c->kv_heads * (c->head_dim / 8);
+  if (count < 0 || count / kTokens >= ((int64_t(1) << 31) - kBlock) / units - 1)   // (no product that wraps)
     return refuse(RMSNORM_TP_ERR_INVALID, "%s: %lld slots of %d heads of %d: at most 2^36 elements", who,
                   (long long)count, c->kv_heads, c->head_dim);
   if (count == 0) return RMSNORM_TP_OK;

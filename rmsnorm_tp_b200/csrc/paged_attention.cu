@@ -383,7 +383,7 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
   // this CTA's run of shares [t0, t1): every thread sums those of a run of sequences
   int64_t each = 0, more = 0, t0 = 0, t1 = 0;
   const int64_t me = blockIdx.x;
-  Share* meta = reinterpret_cast<Share*>(a.part) + 2 * me;   // (divided) of the segment that began before, and one left open
+  Share* meta = reinterpret_cast<Share*>(a.part) + 2 * me;   // divided: of the segment that began before, of one left open
   Place at;
   int hs;
   if (a.undivided) {
@@ -1053,7 +1053,8 @@ int row_groups_of(const rmsnorm_paged_attention_args* a, const Kernels& k) {
 // second launch and the workspace cost the host 4 us; 128 such segments: 9.9 and 7.9, 12.9
 // and 10.7, 14.4 and 13.7.
 bool undivided(const rmsnorm_paged_attention_args* a, const Kernels& k) {
-  return a->max_pages * a->cache->page_size <= 512 && a->batch * a->cache->kv_heads * row_groups_of(a, k) < (int64_t(1) << 30);
+  return a->max_pages * a->cache->page_size <= 512 &&
+         a->batch * a->cache->kv_heads * row_groups_of(a, k) < (int64_t(1) << 30);
 }
 // CTAs of the main kernel: one resident wave, or a tile each of the longest lengths.
 int64_t worker_count(const rmsnorm_paged_attention_args* a, const Kernels& k, int sms) {
@@ -1094,7 +1095,7 @@ int check_attention(const char* who, const rmsnorm_paged_attention_args* a) {
                   a->q_heads, c->kv_heads);
   if (a->batch < 0 || a->batch > 65535)
     return refuse(RMSNORM_TP_ERR_INVALID, "%s: batch %lld outside [0, 65535]", who, (long long)a->batch);
-  if (a->max_pages < 0 || a->max_pages * (int64_t)c->page_size > kMostTokens)
+  if (a->max_pages < 0 || a->max_pages > kMostTokens / c->page_size)   // (no product that wraps)
     return refuse(RMSNORM_TP_ERR_INVALID, "%s: %lld pages of %d tokens: a sequence holds at most 2^31 - 128",
                   who, (long long)a->max_pages, c->page_size);
   if ((a->max_pages * (int64_t)c->page_size / 64 + 2) * a->batch * a->q_heads > kMostTiles)
@@ -1188,7 +1189,8 @@ int rmsnorm_paged_attention(const rmsnorm_paged_attention_args* in, void* stream
     }
     a.undivided = undivided(in, k);
     if (a.undivided) {
-      const cudaError_t e = launch_dependent(k.main, dim3((unsigned)(a.batch * a.segments)), dim3(kBlock), k.smem, args, st);
+      const cudaError_t e =
+          launch_dependent(k.main, dim3((unsigned)(a.batch * a.segments)), dim3(kBlock), k.smem, args, st);
       return e == cudaSuccess ? RMSNORM_TP_OK : launch_failed(e, who);
     }
     const unsigned n = (unsigned)worker_count(in, k, sms);

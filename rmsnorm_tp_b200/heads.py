@@ -389,7 +389,7 @@ def paged_attention(q: torch.Tensor, cache: PagedKVCache, page_table: torch.Tens
     head_dim], with ``return_lse`` also the fp32 logarithm of each head's sum of
     exponentials [batch, q_heads]. A sequence without tokens gives zeros and -inf; pages
     outside the cache are left out, lengths cut to max_pages * page_size. ``scale`` is
-    head_dim^-0.5 unless given."""
+    head_dim^-0.5 unless given. A serving operator: not recorded for autograd."""
     qs, device, q_dtype = q.shape, q.get_device(), q.dtype
     if device < 0 or len(qs) != 3 or q.stride(2) != 1:
         raise AssertionError("q must be a CUDA tensor [batch, q_heads, head_dim] with stride 1 in the last "

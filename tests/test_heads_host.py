@@ -125,7 +125,7 @@ def _attn(cache, q=Q, out=QO, table=TABLE, lens=POS, ws=V, nbytes=1 << 30, qs=(2
 def test_attention_refuses_before_any_cuda_call():
     keep, at = _cache()
     for kw in (dict(hq=3), dict(hq=0), dict(dtype=_lib.F16), dict(dtype=9), dict(batch=-1), dict(batch=65536),
-               dict(pages=-1), dict(pages=1 << 27), dict(q=0), dict(out=0), dict(lens=0), dict(table=0),
+               dict(pages=-1), dict(pages=1 << 27), dict(pages=1 << 60), dict(q=0), dict(out=0), dict(lens=0), dict(table=0),
                dict(out=Q), dict(qs=(-256, 64)), dict(out=QO + 8), dict(ws=V + 4),
                dict(batch=65535, hq=65536, pages=1 << 26)):
         assert L.rmsnorm_paged_attention(_attn(at, **kw), None) == _lib.ERR_INVALID, kw
@@ -139,7 +139,7 @@ def test_read_refuses_before_any_cuda_call():
     keep, at = _cache()
     read = lambda k=Q, v=K, slots=SLOTS, n=4, dtype=1: L.rmsnorm_kv_read(at, k, v, slots, n, dtype, -1, None)  # noqa: E731
     assert read() == _lib.ERR_CUDA and read(n=0, k=0) == _lib.OK
-    assert read(k=0) == read(slots=0) == read(n=-1) == read(n=1 << 31) == read(dtype=3) == read(k=Q + 2) == \
+    assert read(k=0) == read(slots=0) == read(n=-1) == read(n=1 << 31) == read(n=1 << 62) == read(dtype=3) == read(k=Q + 2) == \
         _lib.ERR_INVALID
 
 
