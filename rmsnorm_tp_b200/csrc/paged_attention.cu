@@ -286,17 +286,27 @@ __device__ __forceinline__ void unpack2(uint32_t u, float& lo, float& hi) {
   if constexpr (kBf16) bf16x2_unpack(u, lo, hi);
   else f16x2_unpack(u, lo, hi);
 }
-// Two 16-bit parts of numerators x, y >= 0, together exact to 2^-16 of them: the value cut
-// off, and what is left. Neither is negative, and the second never 0 beside a first that is
-// not, so that a numerator meets an infinity in V as one positive number would.
+// Two 16-bit parts of numerators x, y >= 0, together exact to 2^-16 of them (fp16 to 2^-20,
+// or 2^-25 where that is more): the value cut off, and what is left. Neither is negative,
+// and the second never 0 beside a first that is not, so that a numerator meets an infinity
+// in V as one positive number would. fp16's smallest number 2^-24 is not far below the
+// numerators, so there the second part is not raised to it, which would add it to every
+// token behind a long sequence's few that count: instead the first is cut from a value
+// that is less than x by 2^-24 and 2^-20 of it, or is 0, and the second is rounded to nearest.
 template <bool kBf16>
 __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
-  constexpr float kLeast = kBf16 ? 1.17549435e-38f : 5.9604644775390625e-8f;   // 2^-126, 2^-24
   float hx, hy;
-  if constexpr (kBf16) hi = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
-  else asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(y), "f"(x));
-  unpack2<kBf16>(hi, hx, hy);
-  lo = pack2<kBf16>(fmaxf(x - hx, kLeast), fmaxf(y - hy, kLeast));
+  if constexpr (kBf16) {
+    constexpr float kLeast = 1.17549435e-38f;   // 2^-126
+    hi = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
+    unpack2<kBf16>(hi, hx, hy);
+    lo = pack2<kBf16>(fmaxf(x - hx, kLeast), fmaxf(y - hy, kLeast));
+  } else {
+    constexpr float kLess = 1.f - 9.5367431640625e-7f, kLeast = 5.9604644775390625e-8f;   // 1 - 2^-20, 2^-24
+    asm("cvt.rz.relu.f16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(fmaf(y, kLess, -kLeast)), "f"(fmaf(x, kLess, -kLeast)));
+    unpack2<kBf16>(hi, hx, hy);
+    lo = pack2<kBf16>(x - hx, y - hy);
+  }
 }
 // Over the lanes that hold one head (lane / 4 differs).
 __device__ __forceinline__ float head_max(float v) {
@@ -362,9 +372,9 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
   // the numerators as two 16-bit parts where their rounding to one would be of the output's
   // own size; one fp16 part (2^-11) beside a bf16 output (2^-8)
   constexpr bool kTwoParts = !kE4M3 || !kQBf16;
-  // fp16 numerators run up to 2^15, so that fp16's smallest number is 2^-39 of the largest
-  constexpr float kLiftLog2 = kBf16 || kE4M3 ? 0.f : 15.f - kSlack;
-  constexpr float kLift = kBf16 || kE4M3 ? 1.f : 128.f;
+  // fp16 numerators (e4m3: times V's scale) run up to 2^15, so that fp16's smallest number is
+  // 2^-31 of the reference's: an element that is 0 in the tokens of weight is made of the others
+  constexpr float kLiftLog2 = kBf16 ? 0.f : 15.f - kSlack, kLift = kBf16 ? 1.f : 128.f;
   constexpr int KS = D / 16, MB = S::kBlocks, kTok = S::kTok, kTile = S::kTile;
   constexpr unsigned kAll = kTok == 32 ? ~0u : 0xFFFFu;
   constexpr int kRows = 8 * NG;
@@ -739,7 +749,7 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
 #pragma unroll
         for (int x = 0; x < NG; ++x) {
           const float ref[2] = {ref_of(m[x][0]), ref_of(m[x][1])};
-          const float refv[2] = {ref_of(mv[x][0]), ref_of(mv[x][1])};
+          const float refv[2] = {ref_of(mv[x][0]) - kLiftLog2, ref_of(mv[x][1]) - kLiftLog2};
 #pragma unroll
           for (int t = 0; t < 2 * MB; ++t) {
             uint32_t& to_hi = hi[t >> 1][x][t & 1];
@@ -811,7 +821,7 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
           const float sum = head_sum(l[x][h]);
           if (g == 0) {
             s_m[warp][8 * x + 2 * qd + h] = m[x][h];
-            s_v[warp][8 * x + 2 * qd + h] = kE4M3 ? mv[x][h] : m[x][h] - kLiftLog2;
+            s_v[warp][8 * x + 2 * qd + h] = kE4M3 ? mv[x][h] : m[x][h];
             s_l[warp][8 * x + 2 * qd + h] = sum;
           }
         }
@@ -855,7 +865,7 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
               ll += s_l[w][r] * ex2(s_m[w][r] - ref);
-              const float f = s_v[w][r] == -INFINITY ? 0.f : ex2(s_v[w][r] - ref);
+              const float f = s_v[w][r] == -INFINITY ? 0.f : ex2(s_v[w][r] - ref) * (1.f / kLift);
               const float4 z =
                   *reinterpret_cast<const float4*>(reinterpret_cast<float*>(left + w * kRing) + r8 * S::kJoinPitch + e);
               y.x = fmaf(f, z.x, y.x);

@@ -1,6 +1,7 @@
 """GPU parity of the operators on query / key heads, the paged cache and the single-token
 attention against the formulas in 64 bits (heads_oracle), at sizes, strides, masks and
 values where they can go wrong; the run of them together between the package's norms."""
+import math
 import subprocess
 import sys
 
@@ -399,6 +400,53 @@ def test_attention_large_and_small_numbers(dtype, held):
         cache.k[table[0, 1].long(), :, 3, 5] = float("nan")
         got, lse = rtp.paged_attention(q, cache, table, lens, return_lse=True)
         assert got.isnan().all() and lse.isnan().all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_attention_elements_that_the_heaviest_token_lacks(dtype):
+    """Half of the heaviest token's elements are 0, and its V scale is 64 times the others':
+    these elements are made of tokens whose weights lie near fp16's smallest number."""
+    d, page = 128, 16
+    cache = _filled(51, 2, page, 1, d, E4M3)
+    n, want_s = 3, torch.tensor([16.0, 8.0, 7.0], device="cuda")
+    cache.k[0, 0, :n] = torch.ones(n, d, device="cuda").to(E4M3)
+    cache.k_scale[0, 0, :n] = want_s / d
+    codes = 448 * torch.rand(n, d, generator=_gen(52), device="cuda")
+    codes[0, ::2] = 0
+    cache.v[0, 0, :n] = codes.to(E4M3)
+    cache.v_scale[0, 0, :n] = torch.tensor([0.5, 1 / 128, 1 / 128], device="cuda")
+    q = torch.ones(1, 8, d, device="cuda", dtype=dtype)
+    got = rtp.paged_attention(q, cache, torch.zeros(1, 1, dtype=torch.int32, device="cuda"),
+                              torch.tensor([n], dtype=torch.int32, device="cuda"), 1.0)
+    p, vs = torch.softmax(want_s.double(), 0), cache.v_scale[0, 0, :n].double()
+    v = codes.to(E4M3).double() * vs[:, None]
+    want = (p[:, None] * v).sum(0).expand(1, 8, d)
+    # the scores are off by (d + 8) units of 2^-24 at most; a weight by half a step of its
+    # type, or, where it is small, by 2^-25 beside a heaviest one of 2^7 (codes up to 448)
+    rel = 2 * (d + 24) * H.U32 * 16 + 64 * H.U32 + (2.0 ** -11 if dtype == BF16 else 2.0 ** -16)
+    slop = (rel * (p[:, None] * v.abs()).sum(0) + (n - 1) * 2.0 ** -32 * 448 * (p * vs).max()).expand(1, 8, d)
+    H.within(got, want, slop, "out")
+
+
+@pytest.mark.parametrize("held", [F16, E4M3])
+def test_attention_many_tokens_without_weight(held):
+    """One token takes all the weight and its values are 0: the others, each under 2^-40 of
+    it, add up to less than half of fp16's smallest number, so nothing is left of them."""
+    d, page, n = 128, 64, 200000
+    pages = -(-n // page)
+    k = torch.zeros(pages, 1, page, d, device="cuda")
+    k[7, 0, 3] = 1.0
+    v = torch.ones(pages, 1, page, d, device="cuda")
+    v[7, 0, 3] = 0
+    if held == E4M3:
+        one = torch.ones(pages, 1, page, device="cuda")
+        cache = rtp.PagedKVCache.from_tensors(k.to(E4M3), v.to(E4M3), one, one.clone())
+    else:
+        cache = rtp.PagedKVCache.from_tensors(k.to(held), v.to(held))
+    q = torch.full((1, 8, d), 0.25, device="cuda", dtype=F16)              # scores: 32 and 0
+    got = rtp.paged_attention(q, cache, torch.arange(pages, dtype=torch.int32, device="cuda")[None],
+                              torch.tensor([n], dtype=torch.int32, device="cuda"), 1.0)
+    assert n * math.exp(-32) < 2.0 ** -25 and (got == 0).all()
 
 
 def test_cache_offsets_past_32_bits():
