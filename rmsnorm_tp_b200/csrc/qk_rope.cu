@@ -736,7 +736,8 @@ qk_rope_backward_kernel(const __grid_constant__ QkBackArgs a, int q_blocks) {
         sg = fma2(mul2(ga.v[e], wa.v[e]), xa.v[e], fma2(mul2(gb.v[e], wb.v[e]), xb.v[e], sg));
       }
       const float sum = lanes_sum<L>(f2_sum(ss)), dot = lanes_sum<L>(f2_sum(sg));
-      const float inv = rsqrtf(sum * rd + a.eps);
+      // behind the last row nothing: the root of an eps of 0 would make 0 * inf of it in dw
+      const float inv = live ? rsqrtf(sum * rd + a.eps) : 0.f;
       const float k = -inv * inv * inv * (dot * rd);
       const f2 inv2 = f2_of(inv, inv), k2 = f2_of(k, k);
 #pragma unroll
