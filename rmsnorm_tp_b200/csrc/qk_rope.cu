@@ -271,7 +271,7 @@ qk_rope_backward_any_kernel(const __grid_constant__ QkBackArgs a, int q_blocks) 
       ss = warp_allreduce_sum(ss);
       sg = warp_allreduce_sum(sg);
       inv = rsqrtf(ss / (float)a.d + a.eps);
-      k = inv * inv * inv * (sg / (float)a.d);
+      k = (sg / (float)a.d * inv) * inv * inv;   // in this order: inv^3 alone leaves fp32's range
     }
     T* y = dx + row * a.d;
     for (int u = lane; u < pairs; u += 32) {
@@ -738,7 +738,7 @@ qk_rope_backward_kernel(const __grid_constant__ QkBackArgs a, int q_blocks) {
       const float sum = lanes_sum<L>(f2_sum(ss)), dot = lanes_sum<L>(f2_sum(sg));
       // behind the last row nothing: the root of an eps of 0 would make 0 * inf of it in dw
       const float inv = live ? rsqrtf(sum * rd + a.eps) : 0.f;
-      const float k = -inv * inv * inv * (dot * rd);
+      const float k = -(dot * rd * inv) * inv * inv;   // in this order: inv^3 alone leaves fp32's range
       const f2 inv2 = f2_of(inv, inv), k2 = f2_of(k, k);
 #pragma unroll
       for (int e = 0; e < N; ++e) {

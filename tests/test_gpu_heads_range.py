@@ -40,3 +40,15 @@ def _check_backward(operands, weights, rope, pos, eps, interleaved=False):
 def test_backward_without_epsilon(tokens, hq, hk, d, dtype, odd):
     """eps = 0 where the rows leave a part of a warp idle: the idle part adds nothing to dw."""
     _check_backward(*_operands(61, tokens, hq, hk, d, dtype, odd), eps=0.0)
+
+
+@pytest.mark.parametrize("odd", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("tokens", [8, 3000])
+@pytest.mark.parametrize("power,eps", [(50, 1e-6), (60, 0.0), (-50, 0.0), (-60, 0.0)])
+def test_backward_of_rows_far_from_one(power, eps, tokens, dtype, odd):
+    """Rows whose inverse root cubed is no normal fp32 number, while the root and dx are."""
+    operands, *rest = _operands(62, tokens, 8, 4, 128, dtype, odd)
+    for x in operands[:2]:
+        x *= 2.0 ** power
+    _check_backward(operands, *rest, eps=eps)
