@@ -172,7 +172,8 @@ __global__ void __launch_bounds__(kAnyBlock) attention_join_any_kernel(const __g
 //
 // The softmax's reference is a score seen, not the maximum: it moves only when a score
 // passes it by more than 2^8, so most tiles need no maximum over the warp and no
-// rescaling; exponentials are then at most 2^8.
+// rescaling. Exponentials are taken of what is left over reference + 8, so they are at most
+// 1 and a weighted V element is no larger than the element.
 //
 // Measured (device): 64 sequences of up to 16384 tokens, 32 + 8 heads of 128, e4m3 (1085 MB)
 // 170 us, 6.4 TB/s; one sequence of 262144 tokens, 8 + 1 heads of 128, bf16 (134 MB) 30 us:
@@ -181,7 +182,7 @@ __global__ void __launch_bounds__(kAnyBlock) attention_join_any_kernel(const __g
 // (185 MB) 38 us. Groups of 9 to 16 query heads over e4m3 are bound by issue (0.6 of a copy).
 constexpr int kWarps = 4;
 constexpr int kBlock = 32 * kWarps;
-constexpr float kSlack = 8.f;           // log2 of the largest exponential
+constexpr float kSlack = 8.f;           // how far scores may pass the reference (log2)
 constexpr int kJoinBlock = 256;         // threads of the join kernel
 constexpr int kSegment = 1;             // cost of a segment's begin and end, in tiles
 
@@ -289,10 +290,12 @@ __device__ __forceinline__ void unpack2(uint32_t u, float& lo, float& hi) {
 // Two 16-bit parts of numerators x, y >= 0, together exact to 2^-16 of them (fp16 to 2^-20,
 // or 2^-25 where that is more): the value cut off, and what is left. Neither is negative,
 // and the second never 0 beside a first that is not, so that a numerator meets an infinity
-// in V as one positive number would. fp16's smallest number 2^-24 is not far below the
-// numerators, so there the second part is not raised to it, which would add it to every
-// token behind a long sequence's few that count: instead the first is cut from a value
-// that is less than x by 2^-24 and 2^-20 of it, or is 0, and the second is rounded to nearest.
+// in V as one positive number would (a numerator that is 0 in both parts makes NaN of it, as
+// an exponential that underflows does; fp16: weights under 2^-32 of the reference's). fp16's
+// smallest number 2^-24 is not far below the numerators, so there the second part is not
+// raised to it, which would add it to every token behind a long sequence's few that count:
+// instead the first is cut from a value that is less than x by 2^-24 and 2^-20 of it, or is
+// 0, and the second is rounded to nearest.
 template <bool kBf16>
 __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
   float hx, hy;
@@ -374,7 +377,7 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
   constexpr bool kTwoParts = !kE4M3 || !kQBf16;
   // fp16 numerators (e4m3: times V's scale) run up to 2^15, so that fp16's smallest number is
   // 2^-31 of the reference's: an element that is 0 in the tokens of weight is made of the others
-  constexpr float kLiftLog2 = kBf16 ? 0.f : 15.f - kSlack, kLift = kBf16 ? 1.f : 128.f;
+  constexpr float kLiftLog2 = kBf16 ? 0.f : 15.f, kLift = kBf16 ? 1.f : 32768.f;
   constexpr int KS = D / 16, MB = S::kBlocks, kTok = S::kTok, kTile = S::kTile;
   constexpr unsigned kAll = kTok == 32 ? ~0u : 0xFFFFu;
   constexpr int kRows = 8 * NG;
@@ -748,8 +751,8 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
         uint32_t hi[MB][NG][2], lo[MB][NG][2];   // P as 16 tokens x 8 heads
 #pragma unroll
         for (int x = 0; x < NG; ++x) {
-          const float ref[2] = {ref_of(m[x][0]), ref_of(m[x][1])};
-          const float refv[2] = {ref_of(mv[x][0]) - kLiftLog2, ref_of(mv[x][1]) - kLiftLog2};
+          const float ref[2] = {ref_of(m[x][0]) + kSlack, ref_of(m[x][1]) + kSlack};
+          const float refv[2] = {ref_of(mv[x][0]) + (kSlack - kLiftLog2), ref_of(mv[x][1]) + (kSlack - kLiftLog2)};
 #pragma unroll
           for (int t = 0; t < 2 * MB; ++t) {
             uint32_t& to_hi = hi[t >> 1][x][t & 1];
@@ -820,8 +823,9 @@ attention_kernel(const __grid_constant__ AttnArgs a) {
         for (int h = 0; h < 2; ++h) {
           const float sum = head_sum(l[x][h]);
           if (g == 0) {
-            s_m[warp][8 * x + 2 * qd + h] = m[x][h];
-            s_v[warp][8 * x + 2 * qd + h] = kE4M3 ? mv[x][h] : m[x][h];
+            // what the sums are relative to (-inf: nothing seen)
+            s_m[warp][8 * x + 2 * qd + h] = m[x][h] + kSlack;
+            s_v[warp][8 * x + 2 * qd + h] = (kE4M3 ? mv[x][h] : m[x][h]) + kSlack;
             s_l[warp][8 * x + 2 * qd + h] = sum;
           }
         }
