@@ -299,6 +299,15 @@ class PagedKVCache:
             self.head_dim, self._code))
         self._address = ctypes.addressof(self._struct)
 
+    # deepcopy and pickle make other tensors (copy.copy the same): the native structure is
+    # made anew over them, or the copy would go on reading and writing this cache's
+    def __getstate__(self):
+        return {n: v for n, v in self.__dict__.items() if n not in ("_struct", "_address")}
+
+    def __setstate__(self, state) -> None:
+        self.__dict__.update(state)
+        self._adopt(*state["_tensors"])
+
     k = _held(0, "keys, or their codes")
     v = _held(1, "values, or their codes")
     k_scale = _held(2, "scales of the keys' codes, or None")

@@ -1,0 +1,56 @@
+"""Ways to use the operators on heads beside the plain call: copied and stored caches, layouts
+of the projection, operands that share memory."""
+import copy
+import io
+
+import pytest
+import torch
+
+import heads_oracle as H
+import rmsnorm_tp_b200 as rtp
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32, E4M3 = torch.bfloat16, torch.float16, torch.float32, torch.float8_e4m3fn
+
+
+def _normal(seed, *n):
+    return torch.randn(*n, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda")
+
+
+def _stored(cache):
+    buf = io.BytesIO()
+    torch.save(cache, buf)
+    buf.seek(0)
+    return torch.load(buf, weights_only=False)
+
+
+@pytest.mark.parametrize("held", [BF16, E4M3])
+@pytest.mark.parametrize("how", [copy.deepcopy, _stored])
+def test_copies_of_a_cache_are_caches_of_their_own(how, held):
+    tokens, d = 20, 64
+    rope, pos = rtp.rope_table(64, d, device="cuda"), torch.arange(tokens, device="cuda")
+    cache = rtp.PagedKVCache(4, 16, 2, d, held)
+    rows = [_normal(i, tokens, 2, d).to(BF16) for i in range(2)]
+    rtp.qk_norm_rope_write(rows[0], rows[0], rows[0], None, None, rope, pos, cache, pos)
+    before = [t.clone() for t in cache.read(pos)]
+    cache.note = "kept"
+    other = how(cache)
+    assert other.note == "kept" and other.k.data_ptr() != cache.k.data_ptr() and other.dtype == held
+    for a, b in zip(other.read(pos), before):
+        assert torch.equal(a, b)
+    rtp.qk_norm_rope_write(rows[1], rows[1], rows[1], None, None, rope, pos, other, pos)
+    for a, b in zip(cache.read(pos), before):                    # the first as it was
+        assert torch.equal(a, b)
+    table, lens = torch.arange(4, dtype=torch.int32, device="cuda")[None], torch.tensor([tokens], dtype=torch.int32, device="cuda")
+    want = [rtp.paged_attention(rows[1][-1:], c, table, lens) for c in (cache, other)]
+    assert not torch.equal(*want)
+    del cache
+    torch.cuda.empty_cache()
+    assert torch.equal(rtp.paged_attention(rows[1][-1:], other, table, lens), want[1])
+
+
+def test_a_shallow_copy_shares_the_tensors():
+    cache = rtp.PagedKVCache(2, 16, 1, 64)
+    other = copy.copy(cache)
+    assert other.k is cache.k and other._address != cache._address
