@@ -295,7 +295,8 @@ int rmsnorm_qk_rope_forward(const rmsnorm_qk_rope_args* args, void* stream);
 
 /* The same pass; the key heads go into the cache instead of k_out, and v beside
  * them. The cache is of the call's dtype, or e4m3 (quantised from the fp32
- * values, so K is rounded once). */
+ * values, so K is rounded once). q, k, v and q_out lie outside the cache, and
+ * its k and v apart. */
 int rmsnorm_qk_rope_write(const rmsnorm_qk_rope_args* args, void* stream);
 
 /* Gradients of rmsnorm_qk_rope_forward, with g = R^T dy and inv the forward's

@@ -76,6 +76,11 @@ inline View view_of(const void* p, int64_t tokens, int64_t heads, int64_t dim, c
               heads > 1 ? st[1] : dim, eb};
 }
 
+// `bytes` bytes in one piece.
+inline View span_of(const void* p, int64_t bytes) {
+  return View{reinterpret_cast<uintptr_t>(p), bytes > 0, 1, bytes, bytes, bytes, 1};
+}
+
 // Whether two views may share an element. Exact for column blocks of one matrix
 // (the same token stride), else by their extents.
 inline bool views_overlap(const View& a, const View& b) {

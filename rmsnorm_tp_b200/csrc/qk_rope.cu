@@ -923,6 +923,19 @@ int check_forward(const char* who, const rmsnorm_qk_rope_args* a, bool write) {
       if (!(i == j && views_same(outs[i], in[j])) && views_overlap(outs[i], in[j]))
         return refuse(RMSNORM_TP_ERR_INVALID, "%s: %s overlaps an input", who, i ? "k_out" : "q_out");
   }
+  if (write) {
+    // rows of the cache that one warp writes must not be rows that another reads
+    const rmsnorm_kv_cache* c = a->cache;
+    const int64_t rows = c->num_pages * c->kv_heads * c->page_size;
+    const int ceb = c->dtype == RMSNORM_KV_E4M3 ? 1 : eb, seb = c->dtype == RMSNORM_KV_E4M3 ? 4 : 0;
+    const View held[4] = {span_of(c->k, rows * c->head_dim * ceb), span_of(c->v, rows * c->head_dim * ceb),
+                          span_of(c->k_scale, rows * seb), span_of(c->v_scale, rows * seb)};
+    if (views_overlap(held[0], held[1]))
+      return refuse(RMSNORM_TP_ERR_INVALID, "%s: the cache's k overlaps its v", who);
+    for (const View& h : held)
+      if (views_overlap(h, in[0]) || views_overlap(h, in[1]) || views_overlap(h, in[2]) || views_overlap(h, outs[0]))
+        return refuse(RMSNORM_TP_ERR_INVALID, "%s: q, k, v or q_out overlaps the cache", who);
+  }
   if (!write && views_overlap(outs[0], outs[1]))
     return refuse(RMSNORM_TP_ERR_INVALID, "%s: q_out overlaps k_out", who);
   return RMSNORM_TP_OK;

@@ -291,6 +291,9 @@ class PagedKVCache:
         if self.head_dim % 16 or not 16 <= self.head_dim <= 256:
             raise AssertionError(f"head_dim {self.head_dim} must be a multiple of 16, at most 256")
         self._tensors = k, v, k_scale, v_scale
+        # a cache whose keys are its values (one tensor for both) can be read, not written
+        ends = sorted((t.data_ptr(), t.data_ptr() + t.nbytes) for t in (k, v, k_scale, v_scale) if t is not None)
+        self._apart = all(a[1] <= b[0] for a, b in zip(ends, ends[1:]))
         self.dtype, self.device, self._index = k.dtype, k.device, k.get_device()
         self._code = _CACHE_DTYPES[k.dtype]
         self._struct = ctypes.create_string_buffer(_CACHE.pack(
@@ -338,7 +341,9 @@ def qk_norm_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weig
     """``qk_norm_rope`` whose keys go into ``cache`` with ``v`` beside them; returns the
     queries. ``slots`` int64 [tokens] are distinct within a call; a token whose slot lies
     outside the cache (-1: padding) leaves the cache as it is. The cache has q's dtype, or
-    float8_e4m3fn (quantised from the fp32 values)."""
+    float8_e4m3fn (quantised from the fp32 values); its tensors share no memory with q, k, v,
+    ``q_out`` or one another (cached keys turned where they lie: ``qk_norm_rope`` on a view of
+    their pages, with ``k_out`` that view)."""
     device, dtype, tokens, hq, hk, d, most, r = _turn_sizes(q, k, q_weight, k_weight, rope, positions)
     if not _rows_fit(v, tokens, hk, d, dtype, device):
         _explain_rows("v", v, q, hk)
@@ -349,6 +354,8 @@ def qk_norm_rope_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weig
                              f"{cache.device}, the call has {hk} of {d} on {q.device}")
     if cache.dtype is not dtype and cache._code != _lib.KV_E4M3:
         raise AssertionError(f"a {cache.dtype} cache does not take {dtype}")
+    if not cache._apart:
+        raise AssertionError("the cache's tensors share memory: it can be read, not written")
     if q_out is None:
         q_out = torch.empty_like(q)
     elif not _rows_fit(q_out, tokens, hq, d, dtype, device):

@@ -54,3 +54,28 @@ def test_a_shallow_copy_shares_the_tensors():
     cache = rtp.PagedKVCache(2, 16, 1, 64)
     other = copy.copy(cache)
     assert other.k is cache.k and other._address != cache._address
+
+
+def test_write_refuses_shared_memory_and_cached_keys_turn_in_place():
+    tokens, d, page = 16, 64, 16
+    rope, pos = rtp.rope_table(64, d, device="cuda"), torch.arange(tokens, device="cuda") + 5
+    cache = rtp.PagedKVCache.from_tensors(_normal(3, 3, 2, page, d).to(BF16), _normal(4, 3, 2, page, d).to(BF16))
+    q, v = _normal(5, tokens, 4, d).to(BF16), _normal(6, tokens, 2, d).to(BF16)
+    row = cache.k[1].transpose(0, 1)                             # a page's keys, [tokens, heads, d]
+    for bad in ((q, row, v), (q, v, row), (cache.k.view(-1, 4, d)[:tokens], v, v)):
+        with pytest.raises(rtp.RMSNormTPError, match="overlaps the cache"):
+            rtp.qk_norm_rope_write(*bad, None, None, rope, pos, cache, pos)
+    one = rtp.PagedKVCache.from_tensors(cache.k, cache.k)        # keys that are the values: to read
+    with pytest.raises(AssertionError, match="share memory"):
+        rtp.qk_norm_rope_write(q, v, v, None, None, rope, pos, one, pos)
+    for a, b in zip(one.read(pos), (cache.read(pos)[0],) * 2):
+        assert torch.equal(a, b)
+    codes, scale = torch.zeros(2, 1, 1, 16, d, device="cuda").to(E4M3), torch.ones(1, 1, 16, device="cuda")
+    with pytest.raises(AssertionError, match="share memory"):
+        rtp.qk_norm_rope_write(q[:, :1], v[:, :1], v[:, :1], None, None, rope, pos,
+                               rtp.PagedKVCache.from_tensors(codes[0], codes[1], scale, scale), pos)
+    want = H.forward(row.clone(), None, rope, pos, 1e-6, False)
+    before = cache.k.clone()
+    rtp.qk_norm_rope(q, row, None, None, rope, pos, k_out=row)
+    H.within(cache.k[1].transpose(0, 1), *want, "keys turned in place")
+    assert torch.equal(cache.k[0], before[0]) and torch.equal(cache.k[2], before[2])
