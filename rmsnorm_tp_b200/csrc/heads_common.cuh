@@ -81,8 +81,18 @@ inline View span_of(const void* p, int64_t bytes) {
   return View{reinterpret_cast<uintptr_t>(p), bytes > 0, 1, bytes, bytes, bytes, 1};
 }
 
+// Whether b's rows lie between a's, both views' rows being multiples of `stride` apart.
+inline bool rows_between(const View& a, const View& b, int64_t stride) {
+  const int64_t step = stride * a.eb;
+  int64_t d = (int64_t)(b.base - a.base) % step;
+  if (d < 0) d += step;
+  return d >= a.dim * a.eb && d + b.dim * b.eb <= step;
+}
+
 // Whether two views may share an element. Exact for column blocks of one matrix
-// (the same token stride), else by their extents.
+// (the same token stride) and for heads that lie between one another's (q, k and v of a head
+// side by side: the same head stride, of which the token stride is a multiple, or the other
+// way round), else by their extents.
 inline bool views_overlap(const View& a, const View& b) {
   const uintptr_t an = a.bytes(), bn = b.bytes();
   if (an == 0 || bn == 0) return false;
@@ -93,6 +103,12 @@ inline bool views_overlap(const View& a, const View& b) {
     int64_t d = ((int64_t)(b.base - a.base)) % step;
     if (d < 0) d += step;
     if (ra <= step && rb <= step && d >= ra && d + rb <= step) return false;
+  }
+  if (a.eb == b.eb) {
+    const bool heads = a.n1 > 1 && b.n1 > 1 && a.s1 == b.s1, tokens = a.n0 > 1 && b.n0 > 1 && a.s0 == b.s0;
+    const auto whole = [](int64_t n, int64_t stride, int64_t of) { return n <= 1 || stride % of == 0; };
+    if (heads && a.s1 > 0 && whole(a.n0, a.s0, a.s1) && whole(b.n0, b.s0, a.s1) && rows_between(a, b, a.s1)) return false;
+    if (tokens && a.s0 > 0 && whole(a.n1, a.s1, a.s0) && whole(b.n1, b.s1, a.s0) && rows_between(a, b, a.s0)) return false;
   }
   return true;
 }

@@ -79,3 +79,23 @@ def test_write_refuses_shared_memory_and_cached_keys_turn_in_place():
     rtp.qk_norm_rope(q, row, None, None, rope, pos, k_out=row)
     H.within(cache.k[1].transpose(0, 1), *want, "keys turned in place")
     assert torch.equal(cache.k[0], before[0]) and torch.equal(cache.k[2], before[2])
+
+
+@pytest.mark.parametrize("d,r", [(128, 128), (96, 32), (50, 20)])
+@pytest.mark.parametrize("tokens", [1, 77])
+def test_turned_in_place_where_q_k_and_v_of_a_head_lie_side_by_side(tokens, d, r):
+    heads = 5
+    qkv = _normal(7, tokens, heads, 3, d).to(BF16)
+    q, k, v = qkv.unbind(2)
+    w = [(1 + 0.2 * _normal(8 + i, d)).to(BF16) for i in range(2)]
+    rope, pos = rtp.rope_table(128, r, device="cuda"), torch.arange(tokens, device="cuda")
+    want, v0 = rtp.qk_norm_rope(q, k, *w, rope, pos), v.clone()
+    cache = rtp.PagedKVCache(8, 16, heads, d, BF16) if d % 16 == 0 else None
+    rtp.qk_norm_rope(q, k, *w, rope, pos, q_out=q, k_out=k)
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1]) and torch.equal(v, v0)
+    if cache is not None:
+        want, held = rtp.qk_norm_rope(q, k, *w, rope, pos), k.clone()
+        rtp.qk_norm_rope_write(q, k, v, *w, rope, pos, cache, pos, q_out=q)
+        assert torch.equal(q, want[0]) and torch.equal(k, held) and torch.equal(v, v0)
+        for a, b in zip(cache.read(pos), (want[1], v0)):
+            assert torch.equal(a, b)
