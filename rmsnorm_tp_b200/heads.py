@@ -224,7 +224,10 @@ def qk_norm_rope_with_grad(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[
                            k_weight: Optional[torch.Tensor], rope: torch.Tensor, positions: torch.Tensor,
                            eps: float = 1e-6, interleaved: bool = False):
     """``qk_norm_rope`` recorded for autograd; its backward runs the backward kernel (once:
-    it is not differentiable itself)."""
+    it is not differentiable itself). q, k and the weights get gradients; a table that wants
+    one is refused."""
+    if rope.requires_grad and torch.is_grad_enabled():
+        raise AssertionError("rope gets no gradient: give a table that does not require one")
     return _QkNormRopeFunction.apply(q, k, q_weight, k_weight, rope, positions, eps, interleaved)
 
 

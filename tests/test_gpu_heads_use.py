@@ -99,3 +99,14 @@ def test_turned_in_place_where_q_k_and_v_of_a_head_lie_side_by_side(tokens, d, r
         assert torch.equal(q, want[0]) and torch.equal(k, held) and torch.equal(v, v0)
         for a, b in zip(cache.read(pos), (want[1], v0)):
             assert torch.equal(a, b)
+
+
+def test_a_table_that_wants_a_gradient_is_refused():
+    q = _normal(9, 3, 2, 64).requires_grad_()
+    rope, pos = rtp.rope_table(8, 64, device="cuda").requires_grad_(), torch.arange(3, device="cuda")
+    with pytest.raises(AssertionError, match="rope"):
+        rtp.qk_norm_rope_with_grad(q, q, None, None, rope, pos)
+    with torch.no_grad():
+        rtp.qk_norm_rope_with_grad(q, q, None, None, rope, pos)
+    rtp.qk_norm_rope_with_grad(q, q, None, None, rope.detach(), pos)[0].sum().backward()
+    assert q.grad is not None and rope.grad is None
