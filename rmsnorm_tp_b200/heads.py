@@ -280,6 +280,8 @@ class PagedKVCache:
             raise AssertionError(f"unsupported cache dtype {k.dtype}")
         if not k.is_cuda or k.dim() != 4:
             raise AssertionError("k must be a CUDA tensor [num_pages, kv_heads, page_size, head_dim]")
+        if k.shape[1] < 1 or k.shape[2] < 1:
+            raise AssertionError(f"kv_heads and page_size must be positive, got {tuple(k.shape)}")
         for name, t in (("k", k), ("v", v)):
             if t.shape != k.shape or t.dtype != k.dtype or t.device != k.device or not t.is_contiguous():
                 raise AssertionError(f"{name} must be contiguous with k's shape, dtype and device")

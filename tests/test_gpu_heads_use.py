@@ -110,3 +110,9 @@ def test_a_table_that_wants_a_gradient_is_refused():
         rtp.qk_norm_rope_with_grad(q, q, None, None, rope, pos)
     rtp.qk_norm_rope_with_grad(q, q, None, None, rope.detach(), pos)[0].sum().backward()
     assert q.grad is not None and rope.grad is None
+
+
+@pytest.mark.parametrize("shape", [(2, 0, 16, 64), (2, 1, 0, 64)])
+def test_a_cache_without_heads_or_rows_is_refused(shape):
+    with pytest.raises(AssertionError, match="positive"):
+        rtp.PagedKVCache.from_tensors(*(torch.zeros(shape, device="cuda") for _ in range(2)))
