@@ -1183,13 +1183,63 @@ def run_linear_bench(args):
     return 0
 
 
+def attention_parity(q, k, v, weight, rope, pos, cache, slots, table, lens, turned, out, eps=1e-6):
+    """A decode step's outputs against the formulas in 64 bits, for the first, middle and last
+    sequence: the turned queries, the rows that the write left in the cache (as `cache.read`
+    gives them) and the attention over the rows that the cache holds. Counts elements off by
+    more than their type's half step and the fp32 arithmetic before it (a score's sum of
+    head_dim terms, the softmax's of the length, 2^-11 for the 16-bit weights of the values)."""
+    batch, hq, d = q.shape
+    group, page = hq // k.shape[1], cache.page_size
+    some = sorted({0, batch // 2, batch - 1})
+    half = rope.shape[1] // 2
+    bad = checked = 0
+    worst = 0.0
+
+    def count(got, want, slop):
+        nonlocal bad, checked, worst
+        over = (got.double() - want).abs() / (torch.finfo(got.dtype).eps / 2 * (want.abs() + slop) + slop + 1e-30)
+        bad += int((~(over <= 1)).sum())
+        checked += over.numel()
+        worst = max(worst, float(over.nan_to_num(nan=float("inf")).max()))
+
+    def turn(x, b):
+        x = x[b].double()
+        x = x * (x.square().mean(-1, keepdim=True) + eps).rsqrt() * weight.double()
+        cos, sin = rope[pos[b]].double().split(half)
+        u, w = x[:, :half], x[:, half:]
+        size = (u.abs() + w.abs()).repeat(1, 2)
+        return torch.cat([u * cos - w * sin, u * sin + w * cos], 1), (d / 2 + 16) * 2.0 ** -24 * size
+
+    for b in some:
+        count(turned[b], *turn(q, b))
+        n = int(lens[b])
+        t = torch.arange(n, device=q.device)
+        rows = [x.double() for x in cache.read(table[b][t // page].long() * page + t % page, torch.float32)]
+        assert int(slots[b]) == int(table[b][(n - 1) // page]) * page + (n - 1) % page
+        for got, (want, slop) in zip(rows, (turn(k, b), (v[b].double(), 0.0))):
+            # the cache's own rounding: bf16's half step, or e4m3's (2^-4, 2^-10 of the scale)
+            step = 2.0 ** -8 * want.abs() if cache.dtype == torch.bfloat16 else \
+                2.0 ** -4 * want.abs() + 2.0 ** -10 * want.abs().amax(-1, keepdim=True) / 448
+            count(got[-1], want, 1.01 * (step + slop))
+        kk, vv = (x.transpose(0, 1).repeat_interleave(group, 0) for x in rows)
+        x = turned[b].double()
+        size = torch.einsum("hd,hnd->hn", x.abs(), kk.abs()).amax(-1) * d ** -0.5
+        p = torch.softmax(torch.einsum("hd,hnd->hn", x, kk) * d ** -0.5, -1)
+        rel = 2 * (d + 24) * 2.0 ** -24 * size + (2 * n + 64) * 2.0 ** -24 + 2.0 ** -11
+        count(out[b], torch.einsum("hn,hnd->hd", p, vv), rel[:, None] * torch.einsum("hn,hnd->hd", p, vv.abs()))
+    return {"bad": bad, "checked": checked, "worst_of_bound": round(worst, 4), "sequences": len(some),
+            "against": "norm, rotation, cache rows and attention in 64 bits"}
+
+
 def run_attention_bench(args):
     """--op attention: a decode step of one rank's heads between its two norms -- head norms,
     rotation and the write into a paged cache in one call, then the attention of the new
     tokens over 2048 to 4096 cached tokens each -- on Llama-70B heads (64 query and 8 key
     heads of 128, bf16) of a TP group of 8 and whole, over a bf16 and an e4m3 cache. Times a
     CUDA graph of both calls; the caches of the calls in the graph are different ones, larger
-    than L2 together. Not a workload of the reference, which has the norms alone."""
+    than L2 together. After the timed replays its outputs are checked (--no-parity: not). Not a
+    workload of the reference, which has the norms alone."""
     import rmsnorm_tp_b200 as rtp
 
     torch.cuda.set_device(0)
@@ -1218,23 +1268,30 @@ def run_attention_bench(args):
                     rtp.qk_norm_rope_write(some, some, some, None, None, rope, fill % 4096, c, fill)
                     caches.append(c)
 
+                last = [None] * n
+
                 def step(i):
                     c = caches[i % n]
                     a = rtp.qk_norm_rope_write(q, k, v, weight, weight, rope, pos, c, slots)
-                    return rtp.paged_attention(a, c, table, lens32)
+                    last[i % n] = a, rtp.paged_attention(a, c, table, lens32)
 
                 for i in range(max(args.warmup, 3)):
                     step(i)
                 torch.cuda.synchronize()
-                ms, calls = time_graph(step, n, min(args.steps, 400), 1)
+                graph = capture_graph(step, n)
+                ms, calls = time_graph(step, n, min(args.steps, 400), 1, graph)
                 us = ms * 1e3
+                # of the replayed calls, the last over each end of the caches
+                parity = None if args.no_parity else [
+                    attention_parity(q, k, v, weight, rope, pos, caches[i], slots, table, lens, *last[i])
+                    for i in (0, n - 1)]
                 emit(args, 0, {"op": "decode_attention", "q_heads": hq, "kv_heads": hk, "head_dim": d,
                                "batch": batch, "cached_tokens": int(lens.sum()), "page": page,
                                "dtype": "bf16", "cache": "bf16" if held == dtype else "e4m3",
                                "graph_us_per_step": round(us, 3), "calls": calls,
                                "cache_GBps": round(nbytes / us / 1e3, 1),
-                               "frac_of_copy": round(nbytes / us / 1e3 / hbm, 4)})
-                del caches
+                               "frac_of_copy": round(nbytes / us / 1e3 / hbm, 4), "parity": parity})
+                del caches, last, graph
     return 0
 
 
