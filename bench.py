@@ -1242,7 +1242,10 @@ def run_attention_bench(args):
     workload of the reference, which has the norms alone."""
     import rmsnorm_tp_b200 as rtp
 
-    torch.cuda.set_device(0)
+    _world, rank, local = dist_env()
+    if rank != 0:                       # one rank's heads, and nothing exchanged
+        return 0
+    torch.cuda.set_device(local)
     d, page, dtype = 128, 64, torch.bfloat16
     hbm, _kind = measured_peak_hbm()
     rope = rtp.rope_table(8192, d, base=500000.0, device="cuda")

@@ -74,3 +74,10 @@ def test_the_check_passes_right_outputs_and_counts_mistakes(held):
         else:
             cache.rows["kv".index(plant)][slots[0], 1] = cache.rows["kv".index(plant)][slots[2], 1]
         assert bench.attention_parity(*a)["bad"] > 0, plant
+
+
+def test_other_ranks_leave_before_a_gpu_is_asked_for(monkeypatch):
+    monkeypatch.setenv("WORLD_SIZE", "2")
+    monkeypatch.setenv("RANK", "1")
+    monkeypatch.setenv("LOCAL_RANK", "1")
+    assert bench.run_attention_bench(bench.parse_args(["--op", "attention"])) == 0
