@@ -237,8 +237,9 @@ int rmsnorm_local_backward(void* dx, void* dw, const void* dy, const void* x, co
  * contiguous, of `dtype` (enum rmsnorm_tp_dtype) or RMSNORM_KV_E4M3, then with
  * k_scale and v_scale [num_pages, kv_heads, page_size] fp32. A row x is held as
  *   scale = max(amax|x|, 2^-100) / 448, code = e4m3(x * (448 / max(amax|x|, 2^-100)))
- * and stands for code * scale. head_dim a multiple of 16, at most 256; k and v
- * 16-byte aligned. */
+ * and stands for code * scale (amax over the numbers of x; a NaN stays where it
+ * is, an infinity makes the row NaN). head_dim a multiple of 16, at most 256; k
+ * and v 16-byte aligned. */
 typedef struct rmsnorm_kv_cache {
   void* k;
   void* v;
@@ -304,7 +305,8 @@ int rmsnorm_qk_rope_write(const rmsnorm_qk_rope_args* args, void* stream);
  * g x inv (without weights dx = g, and q, k may be NULL). dq and dk are
  * contiguous [tokens, heads, head_dim] and overlap no input. workspace: with
  * weights, rmsnorm_qk_rope_backward_workspace_bytes(sizes) bytes of device memory (fp32
- * partials of dw; 0: none is used). The sums of dw run in a fixed order. */
+ * partials of dw; 0: none is used, the call runs as one cluster of 16 CTAs, for
+ * which a whole B200 has room). The sums of dw run in a fixed order. */
 typedef struct rmsnorm_qk_rope_backward_args {
   const void* dq_out;         /* [tokens, q_heads, head_dim] */
   const void* dk_out;         /* [tokens, kv_heads, head_dim] */
@@ -351,10 +353,13 @@ int rmsnorm_kv_read(const rmsnorm_kv_cache* cache, void* k_out, void* v_out, con
  * h' = h / (q_heads / kv_heads); token j of sequence b lies in page
  * page_table[b][j / page_size]. A length is cut to max_pages * page_size; tokens
  * in a page outside [0, num_pages) are left out; a sequence with no tokens gives
- * zeros and lse = -inf; max_pages * page_size is at most 2^31 - 128. lse (optional): the natural logarithm of the sum of the
- * exponentials. Scores, softmax and sums in fp32. The work is divided over the
- * cached length as the lengths on the device say. q and the cache of one dtype,
- * or an e4m3 cache. workspace: rmsnorm_paged_attention_workspace_bytes(args)
+ * zeros and lse = -inf; max_pages * page_size is at most 2^31 - 128. lse
+ * (optional): the natural logarithm of the sum of the exponentials. Scores,
+ * softmax and sums in fp32. The work is divided over the cached length as the
+ * lengths on the device say. q and the cache of one dtype, or an e4m3 cache.
+ * Tensor cores serve 16-bit q with head_dim 64, 96, 128, 192 or 256; fp32 and
+ * the other head_dims take a plain kernel, some 40 times slower on a long
+ * sequence. workspace: rmsnorm_paged_attention_workspace_bytes(args)
  * bytes of device memory (16-byte aligned; 0: none is used, or the arguments are
  * refused), of its own for every call in flight. */
 typedef struct rmsnorm_paged_attention_args {

@@ -150,8 +150,9 @@ __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// Division of 32-bit numbers under 2^31 by a number that the host knows:
-// n / by = (umulhi(n, mul) + n) >> shift, with mul = floor(2^32 (2^shift - by) / by) + 1.
+// Division of 32-bit numbers under 2^31 by a number that the host knows, by the multiplier
+// rounded up (Granlund and Montgomery, Division by Invariant Integers using Multiplication,
+// 1994): n / by = (umulhi(n, mul) + n) >> shift, with mul = floor(2^32 (2^shift - by) / by) + 1.
 struct FastDiv {
   unsigned by, mul, shift;
   static FastDiv of(unsigned by) {

@@ -45,9 +45,9 @@ __device__ __forceinline__ int64_t length_of(const AttnArgs& a, int64_t b) {
 }
 
 // ---- any type and head_dim --------------------------------------------------------
-// (fp32, and head_dims that the tensor-core kernel has no shape for.) One CTA per (query
-// head, sequence, split): a thread per token for the scores, a thread per element for the
-// values. Reads the keys' rows uncoalesced and the cache once for each query head: one
+// (fp32, and the multiples of 16 that the tensor-core kernel has no shape for.) One CTA per
+// (query head, sequence, split): a thread per token for the scores, a thread per element for
+// the values. Reads the keys' rows uncoalesced and the cache once for each query head: one
 // sequence of 262144 tokens, 8 heads of 128 over one (bf16), 1133 us against 30 there.
 constexpr int kAnyBlock = 128;
 
@@ -157,11 +157,12 @@ __global__ void __launch_bounds__(kAnyBlock) attention_join_any_kernel(const __g
 // The bound is HBM: a token's K and V rows are read once for its whole group of query
 // heads. The products are K Q^T and V^T P with the tokens (then the elements) as the 16
 // rows of mma.sync and 8 query heads as its columns, so a group of up to 8 pads nothing
-// but itself; tcgen05's 128-row tiles would be 1/16 used, and warp-level mma.sync gives
-// ten times the rate that the bytes ask for. A CTA of 4 warps takes tiles of 64 tokens,
-// 16 for each warp, which runs its own softmax and its own cp.async ring (no CTA barrier
-// in the loop; the loads run ahead over the borders of sequences); the warps' results are
-// joined at a sequence's end.
+// but itself, and over 16-bit caches mma.sync keeps up with the bytes (0.74 to 1.0 of a copy
+// for groups of up to 16). tcgen05, with the tokens as its 128 rows and the heads as its
+// columns, has not been tried; where the products are the larger part (the figures below) it
+// may be worth it. A CTA of 4 warps takes tiles of 64 tokens, 16 for each warp, which runs its
+// own softmax and its own cp.async ring (no CTA barrier in the loop; the loads run ahead over
+// the borders of sequences); the warps' results are joined at a sequence's end.
 //
 // All (sequence, kv head, 8 or 16 query heads) are laid behind one another in tiles, each
 // with one share more for its begin and end, and each CTA takes an equal run of shares, from
@@ -179,7 +180,12 @@ __global__ void __launch_bounds__(kAnyBlock) attention_join_any_kernel(const __g
 // 170 us, 6.4 TB/s; one sequence of 262144 tokens, 8 + 1 heads of 128, bf16 (134 MB) 30 us:
 // 21 of streaming at 6.2 TB/s, 4 before the first tiles arrive (lengths, place, pages, rows:
 // four memory round trips), 4.6 of the join; 48 of up to 2011, 16 + 16 heads of 64, fp16
-// (185 MB) 38 us. Groups of 9 to 16 query heads over e4m3 are bound by issue (0.6 of a copy).
+// (185 MB) 38 us. Short of a copy (64 sequences of 4096, 4 kv heads): e4m3 with up to 8 query
+// heads a kv head at head_dim 64 and 96 (0.56 to 0.62), with 9 to 16 (0.39, 0.45, 0.59, 0.65,
+// 0.61 at 64, 96, 128, 192, 256) and, past 16 heads, all of them, as K and V are read once for
+// each 16 (32 heads: 16-bit 0.42 to 0.49, e4m3 0.22 to 0.36). There 8 or 12 warps an SM issue
+// in half of the cycles (46 to 54 %): a warp's turn is one chain of products, softmax and
+// products, and too few warps hide it.
 constexpr int kWarps = 4;
 constexpr int kBlock = 32 * kWarps;
 constexpr float kSlack = 8.f;           // how far scores may pass the reference (log2)
@@ -290,12 +296,11 @@ __device__ __forceinline__ void unpack2(uint32_t u, float& lo, float& hi) {
 // Two 16-bit parts of numerators x, y >= 0, together exact to 2^-16 of them (fp16 to 2^-20,
 // or 2^-25 where that is more): the value cut off, and what is left. Neither is negative,
 // and the second never 0 beside a first that is not, so that a numerator meets an infinity
-// in V as one positive number would (a numerator that is 0 in both parts makes NaN of it, as
-// an exponential that underflows does; fp16: weights under 2^-32 of the reference's). fp16's
-// smallest number 2^-24 is not far below the numerators, so there the second part is not
-// raised to it, which would add it to every token behind a long sequence's few that count:
-// instead the first is cut from a value that is less than x by 2^-24 and 2^-20 of it, or is
-// 0, and the second is rounded to nearest.
+// in V as one positive number would. fp16's smallest number 2^-24 is not far below the
+// numerators, so there the second part is not raised to it, which would add it to every
+// token behind a long sequence's few that count: instead the first is cut from a value
+// that is less than x by 2^-24 and 2^-20 of it, or is 0, and the second is rounded to
+// nearest; a weight under 2^-32 of the heaviest is then 0 in both, and makes NaN of an infinity.
 template <bool kBf16>
 __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
   float hx, hy;

@@ -86,7 +86,9 @@ __device__ __forceinline__ int64_t cache_row(int64_t slot, int head, const QkArg
 // Lane l holds the pairs l, l + 32, ...; a row is read twice (its sum of squares,
 // then its elements), the second time from L1. Scalar loads bound it: where both
 // could run, 8192 tokens of 40 heads of 128 (bf16) take 118 us here and 29.7 in the
-// vector kernel, the backward 472 and 52.8.
+// vector kernel, the backward 472 and 53.4. Sizes that only this takes: 8192 tokens of 40
+// heads of 80, 40 of them turned (bf16), 142 us and 450 for the backward, 8.8 and 19 times
+// their bytes.
 template <typename T, bool kWrite>
 __global__ void __launch_bounds__(kBlock) qk_rope_any_kernel(const __grid_constant__ QkArgs a) {
   ptx::grid_dep_wait();
@@ -643,7 +645,7 @@ qk_rope_kernel(const __grid_constant__ QkArgs a, const __grid_constant__ Split s
 // The backward: g and x in registers, dw summed per lane over the lane's rows, then over
 // the warp's row groups and the CTA's warps in a fixed order. CTAs [0, q_blocks) share the
 // queries' rows equally, the others the keys'. 8192 tokens of 32 + 8 heads of 128 (bf16,
-// 253.8 MB): 52.8 us, 4.8 TB/s, 73 % of a copy; cosines, weights, dw, g and x fill 128
+// 253.8 MB): 53.4 us, 4.75 TB/s, 73 % of a copy (fp32 88 us, 88 %); cosines, weights, dw, g and x fill 128
 // registers, and 16 warps an SM do not hide a row's chain of products and lane sums (issue
 // 51 % of the cycles; at 96 registers the spills cost more: 66 us).
 constexpr int kBackCtas = 4;               // resident on an SM (128 registers a thread)
@@ -857,8 +859,10 @@ const void* backward_fn(int lanes) {
 // memory (no second kernel, no workspace): rows for the vector kernel, at most 8 groups of
 // them for each warp. A decision by the sizes, so that the caller knows what the workspace
 // has to hold; on odd addresses the kernel for any row runs as that cluster. 333 tokens of 9
-// heads of 64 (fp16): 9.1 us on the device against 4.6 in two kernels, but 15.4 against 20.7
-// a call, as the host issues them.
+// heads of 64 (fp16): 9.2 us on the device against 4.6 in two kernels, but 15.9 against 20.7
+// a call, as the host issues them (a captured call has the device time: what it loses there is
+// the price). 16 CTAs are past the portable cluster size: a whole B200 has room for them, a
+// part of one may refuse the launch.
 constexpr int kCluster = 16;
 bool one_cluster(int64_t tokens, int hq, int hk, int d, int r, int dtype) {
   const int lanes = lanes_of(d, r, elem_bytes(dtype), 0, 0);
