@@ -77,8 +77,9 @@ inline View view_of(const void* p, int64_t tokens, int64_t heads, int64_t dim, c
 }
 
 // `bytes` bytes in one piece.
-inline View span_of(const void* p, int64_t bytes) {
-  return View{reinterpret_cast<uintptr_t>(p), bytes > 0, 1, bytes, bytes, bytes, 1};
+inline View span_of(const void* p, uint64_t bytes) {
+  const int64_t n = (int64_t)bytes;
+  return View{reinterpret_cast<uintptr_t>(p), n > 0, 1, n, n, n, 1};
 }
 
 // Whether b's rows lie between a's, both views' rows being multiples of `stride` apart.

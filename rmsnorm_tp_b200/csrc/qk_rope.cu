@@ -930,7 +930,7 @@ int check_forward(const char* who, const rmsnorm_qk_rope_args* a, bool write) {
   if (write) {
     // rows of the cache that one warp writes must not be rows that another reads
     const rmsnorm_kv_cache* c = a->cache;
-    const int64_t rows = c->num_pages * c->kv_heads * c->page_size;
+    const uint64_t rows = (uint64_t)c->num_pages * c->kv_heads * c->page_size;   // (sizes of no memory may wrap)
     const int ceb = c->dtype == RMSNORM_KV_E4M3 ? 1 : eb, seb = c->dtype == RMSNORM_KV_E4M3 ? 4 : 0;
     const View held[4] = {span_of(c->k, rows * c->head_dim * ceb), span_of(c->v, rows * c->head_dim * ceb),
                           span_of(c->k_scale, rows * seb), span_of(c->v_scale, rows * seb)};

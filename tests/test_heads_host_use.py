@@ -86,3 +86,10 @@ def test_no_views_that_share_an_element_are_taken():
                 if j != i and not (j == i - 2 and rows[i] == rows[j]):
                     assert not sets[i] & sets[j], (d, tokens, hq, hk, at, st)
     assert taken > 1000 and refused > 1000
+
+
+def test_write_takes_caches_of_the_largest_sizes_that_are_checked():
+    """Sizes whose bytes pass 64 bits are of no memory; the checks come to an end on them."""
+    keep, at = _cache(pages=(1 << 31) - 1, page=(1 << 31) - 1, heads_=65536)
+    assert L.rmsnorm_qk_rope_write(_rope(v=V, slots=SLOTS, cache=at, ko=0, hk=65536, tokens=1), None) in \
+        (_lib.ERR_CUDA, _lib.ERR_INVALID)
